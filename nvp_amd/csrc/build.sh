@@ -22,7 +22,9 @@ SRCS_EXPERIMENTS="$SRCS_PRODUCT encode_fwd_lds mlp_fwd_b3r mlp_bwd_b3 mlp_dw_gld
 # build_lib OUT.so OBJDIR "extra flags" "sources"
 build_lib() {
   local out=$1 objdir=$2 extra=$3 SRCS=$4
-  local FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wno-pass-failed -Wno-constant-logical-operand ${NVP_EXTRA_FLAGS:-} $extra"
+  # packed fp32 instructions stay off: some of their forms have given wrong results on this hardware, without an error (the host pass
+  # warns that it does not know the feature: harmless)
+  local FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wno-pass-failed -Wno-constant-logical-operand -Xclang -target-feature -Xclang -packed-fp32-ops ${NVP_EXTRA_FLAGS:-} $extra"
   local OBJS=() PIDS=() NAMES=()
   mkdir -p "$objdir"
   # a change of flags invalidates every object of that directory
