@@ -322,6 +322,25 @@ typedef struct nvp_adamw_seg {
 int nvp_adamw_step(const nvp_adamw_seg* segs, int32_t n_segs, double lr, double beta1, double beta2,
                    double eps, double weight_decay, int64_t step, double grad_scale, void* stream);
 
+/* ---- conditioning operators: element types of their streams ---------------------------------------------------------------- */
+#define NVP_F32 0
+#define NVP_BF16 1
+#define NVP_F16 2
+
+/* ---- 8-bit linear layer with one power-of-two scale per block of 128 (no counterpart in the reference, whose eval.py:19-109 quantises
+ * the grids only) -----------------------------------------------------------------------------------------------------------------
+ * Block form of a matrix v [rows][k]: q e4m3 bytes [rows][128 * ceil(k / 128)] (zeros behind column k), e exponent bytes
+ * [ceil(rows / block_rows)][ceil(k / 128)], v ~ q * 2^(e - 127), block_rows 1 or 128.  The exponent is the smallest that brings the
+ * block's largest finite |v| to 448 or below (at least 2^-127; 127 for a block of zeros); infinities and NaN become NaN bytes. */
+int nvp_quantize_blocks(const void* x, int32_t type, uint8_t* q, uint8_t* e, int64_t rows, int64_t k, int32_t block_rows, void* stream);
+int nvp_dequantize_blocks(const uint8_t* q, const uint8_t* e, void* x, int32_t type, int64_t rows, int64_t k, int32_t block_rows, void* stream);
+/* y [rows][n] = q(x) w^T (+ bias [n]): x [rows][k] of `type` is quantised inside the call (block_rows 1), w [n][k] is given in block form
+ * with block_rows 128, q 16-byte aligned; bias (or NULL) and y are of x's type.  fp32 accumulation, one rounding.  workspace:
+ * nvp_linear8_workspace_bytes() bytes, 16-byte aligned (0 for up to 16 rows).  rows == 0 is a no-op. */
+int64_t nvp_linear8_workspace_bytes(int64_t rows, int64_t k, int64_t n);
+int nvp_linear8(const void* x, int32_t type, const uint8_t* q, const uint8_t* e, const void* bias, void* y, int64_t rows, int64_t k, int64_t n,
+                void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -6,6 +6,7 @@ the call raises - the product path never silently runs on anything but the HIP k
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import math
 import os
@@ -107,6 +108,10 @@ SIGNATURES = {
     "nvp_order_by_rows": [_p, _p, _i64, C.POINTER(Levels), C.POINTER(Levels), _vp, _i64, _vp],
     "nvp_sample_gather": [_p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i32, _i32, _i32, _vp],
     "nvp_adamw_step": [C.POINTER(AdamwSeg), _i32, C.c_double, C.c_double, C.c_double, C.c_double, C.c_double, _i64, C.c_double, _vp],
+    "nvp_quantize_blocks": [_p, _i32, _p, _p, _i64, _i64, _i32, _vp],
+    "nvp_dequantize_blocks": [_p, _p, _p, _i32, _i64, _i64, _i32, _vp],
+    "nvp_linear8_workspace_bytes": [_i64, _i64, _i64],
+    "nvp_linear8": [_p, _i32, _p, _p, _p, _p, _i64, _i64, _i64, _vp, _i64, _vp],
     "nvp_packed_fwd_floats": [_i32],
     "nvp_packed_bwd_floats": [_i32],
     "nvp_dw_partial_floats": [_i32, _i32],
@@ -116,6 +121,7 @@ SIGNATURES = {
     "nvp_mlp_mfma_products": [],
 }
 _RESTYPES = {
+    "nvp_linear8_workspace_bytes": _i64,
     "nvp_packed_fwd_floats": _i64, "nvp_packed_bwd_floats": _i64, "nvp_dw_partial_floats": _i64, "nvp_sample_order_workspace_bytes": _i64, "nvp_order_by_rows_workspace_bytes": _i64,
     "nvp_mlp_param_floats": _i64, "nvp_latent_rows": _i32, "nvp_version": C.c_char_p,
     "nvp_encode_bwd_workspace_bytes": _i64, "nvp_dz_stride": _i32, "nvp_dz_lm_supported": _i32, "nvp_mlp_mfma_products": _i32, "nvp_encode_mlp_fwd_supported": _i32, "nvp_encode_mlp_fwd_bwd_supported": _i32,
@@ -188,6 +194,35 @@ def ptr(t: Optional[torch.Tensor], dtype=torch.float32) -> Optional[int]:
     if not t.is_contiguous():
         raise RuntimeError("expected a contiguous tensor")
     return t.data_ptr()
+
+
+STREAM_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # NVP_F32 / NVP_BF16 / NVP_F16
+
+
+def stream_type(t: torch.Tensor, what: str) -> int:
+    """Type number of a stream of the conditioning operators."""
+    n = STREAM_TYPES.get(t.dtype)
+    if n is None:
+        raise RuntimeError(f"{what}: expected float32, bfloat16 or float16, got {t.dtype}")
+    return n
+
+
+_HERE_ALREADY = contextlib.nullcontext()
+
+
+def on_device_of(first: torch.Tensor, *others: Optional[torch.Tensor]):
+    """Context in which the (one) HIP device of these tensors is the current one: launches and workspaces then go to its current stream,
+    whichever device the caller had selected."""
+    dev = first.device
+    for t in (first,) + others:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise RuntimeError("nvp_amd kernels need tensors on a HIP device (got a CPU tensor); "
+                               "there is no CPU path in the product - move the module/inputs with .cuda()")
+        if t.device != dev:
+            raise RuntimeError(f"expected every tensor on {dev}, got one on {t.device}")
+    return _HERE_ALREADY if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
 
 
 def ntiles(n: int) -> int:

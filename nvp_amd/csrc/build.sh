@@ -1,5 +1,5 @@
 #!/usr/bin/env bash
-# Build libnvp_hip.so - the PRODUCT library, ten sources - for gfx950 in-tree (hipcc cross-compiles without a GPU), plus two pieces of
+# Build libnvp_hip.so - the PRODUCT library, thirteen sources - for gfx950 in-tree (hipcc cross-compiles without a GPU), plus two pieces of
 # TEST INFRASTRUCTURE built from the same sources:
 #   libnvp_hip_experiments.so  -DNVP_EXPERIMENTS=1 + four more sources: the measured-slower kernel variants kept as A/B evidence (LDS-staged
 #                              gather, forward weight ring, per-wave backward chain, merged / paired / grouped / DMA-fed dW jobs) and the
@@ -16,7 +16,7 @@
 set -euo pipefail
 cd "$(dirname "$0")"
 HIPCC=${HIPCC:-/opt/rocm/bin/hipcc}
-SRCS_PRODUCT="encode encode_bwd mlp_pack mlp_fwd mlp_fwd_b3 mlp_bwd mlp_bwd_b3r mlp_dw harness optim"
+SRCS_PRODUCT="encode encode_bwd mlp_pack mlp_fwd mlp_fwd_b3 mlp_bwd mlp_bwd_b3r mlp_dw harness optim linear8"
 SRCS_EXPERIMENTS="$SRCS_PRODUCT encode_fwd_lds mlp_fwd_b3r mlp_bwd_b3 mlp_dw_glds"
 
 # build_lib OUT.so OBJDIR "extra flags" "sources"

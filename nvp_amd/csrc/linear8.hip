@@ -1,0 +1,486 @@
+// Linear layer on 8-bit floating point with one power-of-two scale per block of 128:
+//     y[m][n] = sum_b 2^(sx[m][b] + sw[n / 128][b]) * sum_{k in block b} qx[m][k] qw[n][k]  (+ bias[n])
+// q = e4m3(v * 2^-s), s = the smallest power with max|v| <= 448 * 2^s over the block (one row x 128 columns of x, 128 x 128 of w), kept as the
+// byte s + 127.  A power of two costs a floating-point operand no precision, makes the quantised value exact to state (no rounding in the
+// scale or in v * 2^-s) and is what the matrix instruction multiplies with by itself (v_mfma_scale_f32_*_f8f6f4 takes one exponent byte per
+// row and 32 columns): the block scales cost no vector instruction.
+//
+// Which matrix instruction.  The 8-bit ones add their products to a 32-bit accumulator, but inside each group of 8 products they drop what lies
+// more than 13 bits below the largest product's exponent (measured: 2^3 beside 2^16 is kept, 2^2 is not, in one group; across groups nothing is
+// lost; normal data: 1.5e-5 of the result's rms, whatever K).  That is an order of magnitude below the rounding of a 16-bit y (bf16 1.7e-3,
+// fp16 2e-4 rms), so 16-bit streams take them.  A 32-bit y would show it: fp32 streams widen both operands to bf16 in registers - exact, the
+// scale goes into the exponent (v_cvt_scalef32_pk_bf16_fp8) - and use the bf16 instructions, whose sums are fp32 throughout (2e-7), at half the rate.
+#include "stream_types.h"
+
+namespace {
+
+typedef int v8i __attribute__((ext_vector_type(8)));
+typedef int v4i __attribute__((ext_vector_type(4)));
+
+__host__ __device__ inline int64_t kblocks(int64_t k) { return (k + 127) / 128; }
+__host__ __device__ inline int64_t kb4(int64_t k) { return (kblocks(k) + 3) / 4 * 4; }       // a row's scale bytes, padded to whole dwords
+
+// exponent byte of a block from the bit pattern of its largest finite |v|: 448 = 1.75 * 2^8
+__device__ __forceinline__ unsigned scale_byte(unsigned amax_bits) {
+    if (amax_bits == 0u) return 127u;
+    const int e = (int)(amax_bits >> 23) - 8 + ((amax_bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+    return (unsigned)max(e, 0);
+}
+// 2^-(byte - 127); bytes of scale_byte() are at most 247, so the result is a normal number
+__device__ __forceinline__ float inv_scale(unsigned byte) { return __uint_as_float((254u - byte) << 23); }
+__device__ __forceinline__ unsigned finite_bits(float v) {                                  // |v|, 0 for infinities and NaN
+    const unsigned b = __float_as_uint(v) & 0x7fffffffu;
+    return b < 0x7f800000u ? b : 0u;
+}
+// four values -> four e4m3 bytes, round to nearest even; |v * inv| <= 448, so nothing saturates; infinities and NaN become NaN (0x7f)
+__device__ __forceinline__ int quant4(const float* v, float inv) {
+    int p = 0;
+    p = __builtin_amdgcn_cvt_pk_fp8_f32(v[0] * inv, v[1] * inv, p, false);
+    p = __builtin_amdgcn_cvt_pk_fp8_f32(v[2] * inv, v[3] * inv, p, true);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if ((__float_as_uint(v[e]) & 0x7f800000u) == 0x7f800000u) p = (p & ~(0xff << (8 * e))) | (0x7f << (8 * e));
+    return p;
+}
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+
+// one lane's 32 operand bytes of a matrix instruction and their block's scale byte; WIDE: widened to 4 x 8 bf16, scale applied
+template <bool WIDE> struct frag;
+template <> struct frag<false> {
+    v8i q;
+    int s;
+    __device__ __forceinline__ void set(v8i raw, int byte) { q = raw; s = byte; }
+};
+template <> struct frag<true> {
+    bf16x8 h[4];
+    __device__ __forceinline__ void set(v8i raw, int byte) {
+        const float f = __uint_as_float((unsigned)(byte & 0xff) << 23);                      // only the exponent field counts: byte 0 is 2^-127
+#pragma unroll
+        for (int p = 0; p < 8; ++p) {
+            const bf16x2 lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(raw[p], f, false), hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(raw[p], f, true);
+            h[p >> 1][4 * (p & 1) + 0] = lo[0];
+            h[p >> 1][4 * (p & 1) + 1] = lo[1];
+            h[p >> 1][4 * (p & 1) + 2] = hi[0];
+            h[p >> 1][4 * (p & 1) + 3] = hi[1];
+        }
+    }
+};
+// c += a b^T over 128 (16 x 16 tile) or 64 (32 x 32 tile) values of k.  Which k a register byte stands for is the same in a and b and cancels.
+__device__ __forceinline__ f32x4 mma(const frag<false>& a, const frag<false>& b, f32x4 c) {
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a.q, b.q, c, 0, 0, 0, a.s, 0, b.s);
+}
+__device__ __forceinline__ f32x16 mma(const frag<false>& a, const frag<false>& b, f32x16 c) {
+    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a.q, b.q, c, 0, 0, 0, a.s, 0, b.s);
+}
+__device__ __forceinline__ f32x4 mma(const frag<true>& a, const frag<true>& b, f32x4 c) {
+#pragma unroll
+    for (int p = 0; p < 4; ++p) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.h[p], b.h[p], c, 0, 0, 0);
+    return c;
+}
+__device__ __forceinline__ f32x16 mma(const frag<true>& a, const frag<true>& b, f32x16 c) {
+#pragma unroll
+    for (int p = 0; p < 4; ++p) c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.h[p], b.h[p], c, 0, 0, 0);
+    return c;
+}
+
+// ---- x -> workspace: 16 lanes per block of 128, 8 values each -----------------------------------------------------------------------------
+// q [rows][128 * KB], scales [rows][KB4] (bytes); the launch's last workgroups copy the weights' scales to dword-padded rows [NB][KB4].
+template <typename T, bool VEC>
+__global__ __launch_bounds__(256) void quant_rows_kernel(const T* __restrict__ x, uint8_t* __restrict__ q, uint8_t* __restrict__ ex, int64_t rows, int64_t k,
+                                                         int64_t x_groups, const uint8_t* __restrict__ ew, uint8_t* __restrict__ ew_pad, int64_t ew_bytes) {
+    const int64_t kb = kblocks(k), kb_pad = kb4(k);
+    const int lane16 = threadIdx.x & 15;
+    if ((int64_t)blockIdx.x >= x_groups) {
+        const int64_t i = ((int64_t)blockIdx.x - x_groups) * 256 + threadIdx.x;
+        if (i < ew_bytes) {
+            const int64_t r = i / kb_pad, b = i - r * kb_pad;
+            ew_pad[i] = b < kb ? ew[r * kb + b] : 127;
+        }
+        return;
+    }
+    const int64_t g = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);                         // block number: row * KB + b
+    if (g >= rows * kb) return;                                                              // whole 16-lane groups leave together
+    const int64_t row = g / kb, b = g - row * kb, c0 = b * 128 + lane16 * 8;
+    float v[8];
+    if (VEC && c0 + 8 <= k) {
+        nvp_load<T, 8>(x + row * k + c0, v);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = c0 + e < k ? (float)x[row * k + c0 + e] : 0.f;
+    }
+    unsigned top = 0u;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = max(top, finite_bits(v[e]));
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, o));
+    const unsigned byte = scale_byte(top);
+    const float inv = inv_scale(byte);
+    int2 p;
+    p.x = quant4(v, inv);
+    p.y = quant4(v + 4, inv);
+    *reinterpret_cast<int2*>(q + row * kb * 128 + c0) = p;
+    if (lane16 == 0) ex[row * kb_pad + b] = (uint8_t)byte;
+}
+
+// ---- weights: one workgroup per block of block_rows x 128 (not a hot path: once per set of weights) ----------------------------------------
+template <typename T>
+__global__ __launch_bounds__(256) void quant_blocks_kernel(const T* __restrict__ x, uint8_t* __restrict__ q, uint8_t* __restrict__ e, int64_t rows, int64_t k, int block_rows) {
+    const int64_t kb = kblocks(k);
+    const int64_t rb = (int64_t)blockIdx.x / kb, b = (int64_t)blockIdx.x - rb * kb;
+    const int c = threadIdx.x & 127, r0 = threadIdx.x >> 7;
+    const int64_t col = b * 128 + c;
+    unsigned top = 0u;
+    for (int r = r0; r < block_rows; r += 2) {
+        const int64_t row = rb * block_rows + r;
+        if (row < rows && col < k) top = max(top, finite_bits((float)x[row * k + col]));
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, o));
+    __shared__ unsigned red[4];
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
+    __syncthreads();
+    const unsigned byte = scale_byte(max(max(red[0], red[1]), max(red[2], red[3])));
+    const float inv = inv_scale(byte);
+    for (int r = r0; r < block_rows; r += 2) {
+        const int64_t row = rb * block_rows + r;
+        if (row >= rows) break;
+        const float v[4] = {col < k ? (float)x[row * k + col] : 0.f, 0.f, 0.f, 0.f};
+        q[row * kb * 128 + col] = (uint8_t)(quant4(v, inv) & 0xff);
+    }
+    if (threadIdx.x == 0) e[rb * kb + b] = (uint8_t)byte;
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void dequant_blocks_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ e, T* __restrict__ x, int64_t rows, int64_t k, int block_rows) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= rows * k) return;
+    const int64_t row = i / k, col = i - row * k, kb = kblocks(k);
+    const float v = __builtin_amdgcn_cvt_f32_fp8((int)q[row * kb * 128 + col], 0);
+    const unsigned byte = e[row / block_rows * kb + col / 128];
+    // 2^(byte - 127) in two factors: byte 0 is 2^-127, below the smallest normal number
+    const float s = byte == 255u ? __uint_as_float(0x7fc00000u) : byte ? __uint_as_float(byte << 23) : __uint_as_float(0x00400000u);
+    x[i] = (T)(v * s);
+}
+
+// ---- few rows: every wave walks its share of K with operands straight from global memory ----------------------------------------------------
+// One workgroup: 16 MT rows x 16 NT columns; its eight waves take every eighth block of 128 and add their tiles up through LDS, so a single row
+// times 4096 columns is 256 workgroups x 8 waves that read disjoint weights: bound by the bytes of the weights.  FUSED (MT = 1): x is quantised
+// in registers by every wave (a lane group of 4 holds one row's block; its maximum is two shuffles), no workspace and no second launch.
+// Operand order: lane (i = lane & 15, g = lane >> 4) holds columns 16 g .. 16 g + 15 and 64 + 16 g .. of its row's block, the same for both
+// operands: which k a register byte stands for cancels in the sum, and each load instruction covers 64 contiguous bytes of a row.
+template <typename T, int MT, int NT, bool FUSED>
+__global__ __launch_bounds__(512) void linear8_rows_kernel(const T* __restrict__ x, const uint8_t* __restrict__ qx, const uint8_t* __restrict__ ex, const uint8_t* __restrict__ qw,
+                                                           const uint8_t* __restrict__ ew, const T* __restrict__ bias, T* __restrict__ y, int64_t rows, int64_t k, int64_t n, int xvec) {
+    constexpr bool kWide = sizeof(T) == 4;
+    __shared__ float part[8][MT * 16][NT * 16 + 1];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
+    const int64_t kb = kblocks(k), kp = kb * 128, kbp = kb4(k);
+    const int64_t n0 = (int64_t)blockIdx.x * (16 * NT), m0 = (int64_t)blockIdx.y * (16 * MT);
+    f32x4 acc[MT][NT];
+#pragma unroll
+    for (int a = 0; a < MT; ++a)
+#pragma unroll
+        for (int b = 0; b < NT; ++b) acc[a][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const uint8_t* wrow[NT];
+    const uint8_t* wexp[NT];
+#pragma unroll
+    for (int b = 0; b < NT; ++b) {
+        const int64_t nn = min(n0 + 16 * b + i, n - 1);                                      // rows behind the last one read the last one: their results are not stored
+        wrow[b] = qw + nn * kp + 16 * g;
+        wexp[b] = ew + nn / 128 * (FUSED ? kb : kbp);
+    }
+    const int64_t mrow = m0 + i;
+    for (int64_t b0 = wave; b0 < kb; b0 += 8) {
+        frag<kWide> wf[NT], xf[MT];
+#pragma unroll
+        for (int b = 0; b < NT; ++b) {
+            const v4i lo = *reinterpret_cast<const v4i*>(wrow[b] + b0 * 128), hi = *reinterpret_cast<const v4i*>(wrow[b] + b0 * 128 + 64);
+            wf[b].set(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), wexp[b][b0]);
+        }
+        if (FUSED) {
+            float v[2][16];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int64_t c = b0 * 128 + 64 * h + 16 * g;
+                if (mrow < rows && xvec && c + 16 <= k) {
+#pragma unroll
+                    for (int p = 0; p < 2; ++p) {
+                        float t[8];
+                        nvp_load<T, 8>(x + mrow * k + c + 8 * p, t);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) v[h][8 * p + e] = t[e];
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) v[h][e] = mrow < rows && c + e < k ? (float)x[mrow * k + c + e] : 0.f;
+                }
+            }
+            unsigned top = 0u;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) top = max(top, finite_bits(v[h][e]));
+            top = max(top, (unsigned)__shfl_xor((int)top, 16));
+            top = max(top, (unsigned)__shfl_xor((int)top, 32));
+            const unsigned byte = scale_byte(top);
+            const float inv = inv_scale(byte);
+            v8i raw;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int p = 0; p < 4; ++p) raw[4 * h + p] = quant4(&v[h][4 * p], inv);
+            xf[0].set(raw, (int)byte);
+        } else {
+#pragma unroll
+            for (int a = 0; a < MT; ++a) {
+                const int64_t mm = min(mrow + 16 * a, rows - 1);
+                const uint8_t* p = qx + mm * kp + b0 * 128 + 16 * g;
+                const v4i lo = *reinterpret_cast<const v4i*>(p), hi = *reinterpret_cast<const v4i*>(p + 64);
+                xf[a].set(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), ex[mm * kbp + b0]);
+            }
+        }
+#pragma unroll
+        for (int a = 0; a < MT; ++a)
+#pragma unroll
+            for (int b = 0; b < NT; ++b) acc[a][b] = mma(xf[a], wf[b], acc[a][b]);
+    }
+#pragma unroll
+    for (int a = 0; a < MT; ++a)
+#pragma unroll
+        for (int b = 0; b < NT; ++b)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) part[wave][16 * a + 4 * g + r][16 * b + i] = acc[a][b][r];      // D: row 4 (lane >> 4) + r, column lane & 15
+    __syncthreads();
+    for (int t = threadIdx.x; t < MT * 16 * NT * 16; t += 512) {
+        const int r = t / (NT * 16), c = t % (NT * 16);
+        if (m0 + r >= rows || n0 + c >= n) continue;
+        float s = 0.f;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) s += part[w][r][c];
+        if (bias) s += (float)bias[n0 + c];
+        y[(m0 + r) * n + n0 + c] = (T)s;
+    }
+}
+
+// ---- many rows: BM x BN tiles through LDS --------------------------------------------------------------------------------------------------
+// Two stages of (BM + BN) x 128 bytes, filled by direct-to-LDS loads one block ahead; a wave computes (BM / WM) x (BN / WN) with
+// 32x32x64 instructions.  LDS rows are 128 bytes; the 16-byte piece c of row r lies at place c ^ (r & 7), so the eight lanes that a
+// 128-byte LDS cycle serves (eight rows, one piece) fall on different banks; the load swizzles on its global side (LDS writes are linear).
+__device__ __forceinline__ void glds16(const void* ubase, unsigned lane_off, unsigned lds_byte) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(lane_off), "s"(ubase), "s"(lds_byte) : "memory");
+}
+// the stage's loads have landed and every wave is done with the other stage (its LDS reads have returned: lgkmcnt)
+__device__ __forceinline__ void stage_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+template <typename T, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN) void linear8_tile_kernel(const uint8_t* __restrict__ qx, const uint8_t* __restrict__ ex, const uint8_t* __restrict__ qw,
+                                                                    const uint8_t* __restrict__ ew, const T* __restrict__ bias, T* __restrict__ y, int64_t rows, int64_t k,
+                                                                    int64_t n, int tiles_m, int tiles_n) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    constexpr bool kWide = sizeof(T) == 4;
+    constexpr int kWaves = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32;
+    constexpr int kStage = (BM + BN) * 128;
+    constexpr int kLoads = (BM + BN) / 8 / kWaves;                                           // one load instruction: 8 rows x 128 bytes
+    static_assert((BM + BN) % (8 * kWaves) == 0 && BN / WN <= 128, "tile shape");
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave / WN, wn = wave % WN, i = lane & 31, h = lane >> 5;
+    const int64_t kb = kblocks(k), kp = kb * 128, kbp = kb4(k);
+
+    // workgroups go to the eight XCDs in turn: give each XCD a contiguous run of tiles, walked in groups of 8 tile rows, so that the
+    // tiles an XCD works on at one time share operand rows in its own L2
+    const int total = tiles_m * tiles_n;
+    int id = blockIdx.x;
+    {
+        const int per = total / 8, more = total % 8, xcd = id % 8, at = id / 8;
+        id = xcd * per + min(xcd, more) + at;
+    }
+    const int gsz = 8 * tiles_n, grp = id / gsz, in = id - grp * gsz, gm = min(8, tiles_m - grp * 8);
+    const int tm = grp * 8 + in % gm, tn = in / gm;
+    const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
+
+    // this lane's source rows: row r of the stage is x row m0 + r (r < BM) or weight row n0 + r - BM; beyond the end the last row is read
+    const int lr = lane >> 3, lp = lane & 7, lc = lp ^ lr;
+    const uint8_t* base[kLoads];
+    unsigned off[kLoads];
+#pragma unroll
+    for (int q = 0; q < kLoads; ++q) {
+        const int r = (wave * kLoads + q) * 8;                                               // wave-uniform first row: a group of 8 never straddles BM
+        const bool isx = r < BM;
+        const int64_t first = isx ? min(m0 + r, rows - 1) : min(n0 + r - BM, n - 1);
+        const int64_t row = isx ? min(m0 + r + lr, rows - 1) : min(n0 + r - BM + lr, n - 1);
+        base[q] = (isx ? qx : qw) + first * kp;
+        off[q] = (unsigned)((row - first) * kp) + 16u * lc;                                  // < 8 rows * kp: fits 32 bits for every accepted k
+    }
+    const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
+    auto fill = [&](int64_t b, int stage) {
+#pragma unroll
+        for (int q = 0; q < kLoads; ++q) glds16(base[q] + b * 128, off[q], lds0 + stage * kStage + (wave * kLoads + q) * 1024);
+    };
+    f32x16 acc[TM][TN];
+#pragma unroll
+    for (int a = 0; a < TM; ++a)
+#pragma unroll
+        for (int b = 0; b < TN; ++b) acc[a][b] = nvp_zero16();
+
+    const int64_t nbl = (n0 + wn * (BN / WN)) / 128;                                         // the wave's columns lie in one weight block row
+    const uint32_t* xsrc[TM];
+#pragma unroll
+    for (int a = 0; a < TM; ++a) xsrc[a] = reinterpret_cast<const uint32_t*>(ex + min(m0 + wm * (BM / WM) + 32 * a + i, rows - 1) * kbp);
+    const uint32_t* wsrc = reinterpret_cast<const uint32_t*>(ew + min(nbl, (n - 1) / 128) * kbp);
+    // a scale dword holds four blocks' bytes; the next dwords are loaded one block ahead, in front of that block's fill, so that the stage
+    // barrier waits for them and no other wait (which would drain the fill in flight) is needed
+    uint32_t xs[TM], wsc, xs_next[TM], wsc_next;
+#pragma unroll
+    for (int a = 0; a < TM; ++a) xs_next[a] = xsrc[a][0];
+    wsc_next = wsrc[0];
+    fill(0, 0);
+    for (int64_t b = 0; b < kb; ++b) {
+        stage_barrier();
+        if ((b & 3) == 0) {
+#pragma unroll
+            for (int a = 0; a < TM; ++a) {
+                asm volatile("" : "+v"(xs_next[a]));
+                xs[a] = xs_next[a];
+            }
+            asm volatile("" : "+v"(wsc_next));
+            wsc = wsc_next;
+        }
+        if ((b & 3) == 3 && b + 1 < kb) {
+#pragma unroll
+            for (int a = 0; a < TM; ++a) xs_next[a] = xsrc[a][(b + 1) >> 2];
+            wsc_next = wsrc[(b + 1) >> 2];
+        }
+        if (b + 1 < kb) fill(b + 1, (int)((b + 1) & 1));
+        const uint8_t* st = lds + (b & 1) * kStage;
+        const int sh = 8 * (int)(b & 3);
+        const int sw = (int)(wsc >> sh);
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            frag<kWide> wf[TN];
+#pragma unroll
+            for (int t = 0; t < TN; ++t) {
+                const int r = BM + wn * (BN / WN) + 32 * t + i, c = 4 * kk + 2 * h;
+                const v4i lo = *reinterpret_cast<const v4i*>(st + r * 128 + 16 * (c ^ (r & 7))), hi = *reinterpret_cast<const v4i*>(st + r * 128 + 16 * ((c + 1) ^ (r & 7)));
+                wf[t].set(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), sw);
+            }
+#pragma unroll
+            for (int a = 0; a < TM; ++a) {
+                const int r = wm * (BM / WM) + 32 * a + i, c = 4 * kk + 2 * h;
+                const v4i lo = *reinterpret_cast<const v4i*>(st + r * 128 + 16 * (c ^ (r & 7))), hi = *reinterpret_cast<const v4i*>(st + r * 128 + 16 * ((c + 1) ^ (r & 7)));
+                frag<kWide> xf;
+                xf.set(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), (int)(xs[a] >> sh));
+#pragma unroll
+                for (int t = 0; t < TN; ++t) acc[a][t] = mma(xf, wf[t], acc[a][t]);
+            }
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < TN; ++t) {
+        const int64_t col = n0 + wn * (BN / WN) + 32 * t + i;
+        if (col >= n) continue;
+        const float bv = bias ? (float)bias[col] : 0.f;
+#pragma unroll
+        for (int a = 0; a < TM; ++a)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int64_t row = m0 + wm * (BM / WM) + 32 * a + nvp_frag_row(r, h);
+                if (row < rows) y[row * n + col] = (T)(acc[a][t][r] + bv);
+            }
+    }
+}
+
+template <typename T, int BM, int BN, int WM, int WN>
+int launch_tile(const uint8_t* qx, const uint8_t* ex, const uint8_t* qw, const uint8_t* ew, const void* bias, void* y, int64_t rows, int64_t k, int64_t n, hipStream_t st) {
+    const int64_t tm = (rows + BM - 1) / BM, tn = (n + BN - 1) / BN;
+    if (tm * tn > 0x3fffffff) return NVP_ERR_UNSUPPORTED;
+    constexpr size_t lds = 2 * (BM + BN) * 128;
+    // (HIP on gfx950 takes more than 64 KiB of dynamic LDS with or without the attribute: a refusal must not fail the call)
+    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(linear8_tile_kernel<T, BM, BN, WM, WN>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    if (attr != hipSuccess) (void)hipGetLastError();
+    hipLaunchKernelGGL((linear8_tile_kernel<T, BM, BN, WM, WN>), dim3((unsigned)(tm * tn)), dim3(64 * WM * WN), lds, st, qx, ex, qw, ew, (const T*)bias, (T*)y, rows, k, n, (int)tm, (int)tn);
+    NVP_LAUNCH_CHECK();
+    return 0;
+}
+
+template <typename T, int MT, int NT, bool FUSED>
+int launch_rows(const T* x, const uint8_t* qx, const uint8_t* ex, const uint8_t* qw, const uint8_t* ew, const void* bias, void* y, int64_t rows, int64_t k, int64_t n, int xvec, hipStream_t st) {
+    const int64_t gx = (n + 16 * NT - 1) / (16 * NT), gy = (rows + 16 * MT - 1) / (16 * MT);
+    if (gy > 65535 || gx > 0x7fffffff) return NVP_ERR_UNSUPPORTED;
+    hipLaunchKernelGGL((linear8_rows_kernel<T, MT, NT, FUSED>), dim3((unsigned)gx, (unsigned)gy), dim3(512), 0, st, x, qx, ex, qw, ew, (const T*)bias, (T*)y, rows, k, n, xvec);
+    NVP_LAUNCH_CHECK();
+    return 0;
+}
+
+template <typename T>
+int linear8(const T* x, const uint8_t* qw, const uint8_t* ew, const void* bias, void* y, int64_t rows, int64_t k, int64_t n, uint8_t* ws, hipStream_t st) {
+    const int64_t kb = kblocks(k), kp = kb * 128, kbp = kb4(k), nb = (n + 127) / 128;
+    const bool vec = nvp_vec_width(k, sizeof(T), (uintptr_t)x, 8) == 8;
+    if (rows <= 16) return launch_rows<T, 1, 1, true>(x, nullptr, nullptr, qw, ew, bias, y, rows, k, n, vec ? 1 : 0, st);
+    uint8_t* qx = ws;
+    uint8_t* ex = qx + rows * kp;
+    uint8_t* ewp = ex + rows * kbp;                                                          // rows * kbp is a multiple of 4
+    const int64_t groups = (rows * kb + 15) / 16, tail = (nb * kbp + 255) / 256;
+    if (groups + tail > 0x7fffffff) return NVP_ERR_UNSUPPORTED;
+    if (vec) hipLaunchKernelGGL((quant_rows_kernel<T, true>), dim3((unsigned)(groups + tail)), dim3(256), 0, st, x, qx, ex, rows, k, groups, ew, ewp, nb * kbp);
+    else hipLaunchKernelGGL((quant_rows_kernel<T, false>), dim3((unsigned)(groups + tail)), dim3(256), 0, st, x, qx, ex, rows, k, groups, ew, ewp, nb * kbp);
+    NVP_LAUNCH_CHECK();
+    const int64_t big = ((rows + 255) / 256) * ((n + 255) / 256);
+    if (big >= 128) return launch_tile<T, 256, 256, 2, 4>(qx, ex, qw, ewp, bias, y, rows, k, n, st);
+    if (rows <= 512) return launch_rows<T, 4, 2, false>(x, qx, ex, qw, ewp, bias, y, rows, k, n, 0, st);
+    return launch_tile<T, 128, 128, 2, 2>(qx, ex, qw, ewp, bias, y, rows, k, n, st);
+}
+
+bool sizes_ok(int64_t rows, int64_t k, int64_t n) { return rows >= 0 && n >= 1 && k >= 1 && rows <= (1ll << 31) - 1 && n <= (1ll << 31) - 1 && k <= (1ll << 24); }
+
+}  // namespace
+
+extern "C" int64_t nvp_linear8_workspace_bytes(int64_t rows, int64_t k, int64_t n) {
+    if (!sizes_ok(rows, k, n)) return NVP_ERR_BADARG;
+    if (rows <= 16) return 0;
+    return rows * kblocks(k) * 128 + rows * kb4(k) + (n + 127) / 128 * kb4(k);
+}
+
+extern "C" int nvp_linear8(const void* x, int32_t type, const uint8_t* q, const uint8_t* e, const void* bias, void* y, int64_t rows, int64_t k, int64_t n, void* workspace,
+                           int64_t workspace_bytes, void* stream) {
+    if (!sizes_ok(rows, k, n) || !nvp_type_size(type)) return NVP_ERR_BADARG;
+    if (rows == 0) return 0;
+    if (!x || !q || !e || !y || ((uintptr_t)q & 15)) return NVP_ERR_BADARG;
+    const int64_t need = nvp_linear8_workspace_bytes(rows, k, n);
+    if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15))) return NVP_ERR_BADARG;
+    const hipStream_t st = (hipStream_t)stream;
+    if (type == NVP_F32) return linear8<float>((const float*)x, q, e, bias, y, rows, k, n, (uint8_t*)workspace, st);
+    if (type == NVP_BF16) return linear8<nvp_bf16>((const nvp_bf16*)x, q, e, bias, y, rows, k, n, (uint8_t*)workspace, st);
+    return linear8<nvp_f16>((const nvp_f16*)x, q, e, bias, y, rows, k, n, (uint8_t*)workspace, st);
+}
+
+extern "C" int nvp_quantize_blocks(const void* x, int32_t type, uint8_t* q, uint8_t* e, int64_t rows, int64_t k, int32_t block_rows, void* stream) {
+    if (!sizes_ok(rows, k, 1) || !nvp_type_size(type) || (block_rows != 1 && block_rows != 128)) return NVP_ERR_BADARG;
+    if (rows == 0) return 0;
+    if (!x || !q || !e) return NVP_ERR_BADARG;
+    const int64_t g = (rows + block_rows - 1) / block_rows * kblocks(k);
+    if (g > 0x7fffffff) return NVP_ERR_UNSUPPORTED;
+    const hipStream_t st = (hipStream_t)stream;
+    const dim3 grid((unsigned)g), wg(256);
+    if (type == NVP_F32) hipLaunchKernelGGL((quant_blocks_kernel<float>), grid, wg, 0, st, (const float*)x, q, e, rows, k, block_rows);
+    else if (type == NVP_BF16) hipLaunchKernelGGL((quant_blocks_kernel<nvp_bf16>), grid, wg, 0, st, (const nvp_bf16*)x, q, e, rows, k, block_rows);
+    else hipLaunchKernelGGL((quant_blocks_kernel<nvp_f16>), grid, wg, 0, st, (const nvp_f16*)x, q, e, rows, k, block_rows);
+    NVP_LAUNCH_CHECK();
+    return 0;
+}
+
+extern "C" int nvp_dequantize_blocks(const uint8_t* q, const uint8_t* e, void* x, int32_t type, int64_t rows, int64_t k, int32_t block_rows, void* stream) {
+    if (!sizes_ok(rows, k, 1) || !nvp_type_size(type) || (block_rows != 1 && block_rows != 128)) return NVP_ERR_BADARG;
+    if (rows == 0) return 0;
+    if (!x || !q || !e) return NVP_ERR_BADARG;
+    const int64_t g = (rows * k + 255) / 256;
+    if (g > 0x7fffffff) return NVP_ERR_UNSUPPORTED;
+    const hipStream_t st = (hipStream_t)stream;
+    const dim3 grid((unsigned)g), wg(256);
+    if (type == NVP_F32) hipLaunchKernelGGL((dequant_blocks_kernel<float>), grid, wg, 0, st, q, e, (float*)x, rows, k, block_rows);
+    else if (type == NVP_BF16) hipLaunchKernelGGL((dequant_blocks_kernel<nvp_bf16>), grid, wg, 0, st, q, e, (nvp_bf16*)x, rows, k, block_rows);
+    else hipLaunchKernelGGL((dequant_blocks_kernel<nvp_f16>), grid, wg, 0, st, q, e, (nvp_f16*)x, rows, k, block_rows);
+    NVP_LAUNCH_CHECK();
+    return 0;
+}

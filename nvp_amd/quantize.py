@@ -7,7 +7,15 @@ torch ops, any device); arithmetic order is the reference's so results are bit-i
     x' = (max - min) * (float(q) / 255) + min
 
 with min/max taken per feature and per LEVEL for the keyframes, per feature over the whole
-[T,X,Y] volume for the sparse grid."""
+[T,X,Y] volume for the sparse grid.
+
+The second half of the file is 8-bit evaluation of LINEAR layers (no counterpart in the reference, whose bit budget counts the network
+at 32 bits per weight, eval.py:189-190), on HIP kernels: e4m3 values with one power-of-two scale per block of 128,
+
+    v ~ q * 2^(e - 127),  q = e4m3(v * 2^(127 - e)),  e = the smallest byte that brings the block's largest |v| to 448 or below
+
+with a block of 128 x 128 for weights (`quantize_blocks(w, 128)`, once) and of one row x 128 columns for activations (inside the call).
+`linear8(x, q, e, bias)` is the layer, `Linear8.from_linear(layer)` the module.  Inference only: there is no gradient."""
 from __future__ import annotations
 
 import torch
@@ -54,3 +62,111 @@ def quantized_bpp(model: nn.Module, n_frames: int, height: int, width: int) -> f
     n_all = sum(p.numel() for p in model.parameters())
     n_mlp = sum(p.numel() for p in model.wrapper.parameters())
     return (n_all * 8 + n_mlp * 24) / (n_frames * height * width)
+
+
+# --------------------------------------------------------------------------------------
+# 8-bit linear layers: e4m3 with one power-of-two scale per block of 128
+# --------------------------------------------------------------------------------------
+BLOCK = 128
+
+
+def _kblocks(k: int) -> int:
+    return (k + BLOCK - 1) // BLOCK
+
+
+def quantize_blocks(v: torch.Tensor, rows: int = 1):
+    """v [R, K] (fp32 / bf16 / fp16) -> (q, e): q float8_e4m3fn [R, K rounded up to a multiple of 128] with zeros behind column K, e uint8
+    [ceil(R / rows), ceil(K / 128)], v ~ q * 2^(e - 127) over blocks of `rows` (1 or 128) x 128.  Infinities and NaN become NaN and do not
+    count for the block's scale; a block of zeros has e = 127."""
+    if v.dim() != 2 or v.shape[1] < 1:
+        raise RuntimeError(f"quantize_blocks expects a matrix with at least one column, got shape {tuple(v.shape)}")
+    if rows not in (1, BLOCK):
+        raise RuntimeError(f"quantize_blocks: a block has 1 or {BLOCK} rows, got {rows}")
+    ty = L.stream_type(v, "quantize_blocks")
+    with L.on_device_of(v):
+        v = v.detach().contiguous()
+        r, k = v.shape
+        q = torch.empty((r, _kblocks(k) * BLOCK), device=v.device, dtype=torch.float8_e4m3fn)
+        e = torch.empty(((r + rows - 1) // rows, _kblocks(k)), device=v.device, dtype=torch.uint8)
+        L.check(L.load().nvp_quantize_blocks(L.ptr(v, v.dtype), ty, L.ptr(q, q.dtype), L.ptr(e, e.dtype), r, k, rows, L.stream_ptr()), "nvp_quantize_blocks")
+    return q, e
+
+
+def _check_blocks(q: torch.Tensor, e: torch.Tensor, k: int, rows: int, what: str) -> None:
+    if q.dtype != torch.float8_e4m3fn or e.dtype != torch.uint8 or q.dim() != 2 or e.dim() != 2:
+        raise RuntimeError(f"{what}: expected a float8_e4m3fn matrix and its uint8 scales, got {q.dtype} {tuple(q.shape)} and {e.dtype} {tuple(e.shape)}")
+    if k < 1 or q.shape[1] != _kblocks(k) * BLOCK or tuple(e.shape) != ((q.shape[0] + rows - 1) // rows, _kblocks(k)):
+        raise RuntimeError(f"{what}: {k} columns in blocks of {rows} x {BLOCK} need q [R, {_kblocks(max(k, 1)) * BLOCK}] and e [ceil(R / {rows}), {_kblocks(max(k, 1))}], "
+                           f"got {tuple(q.shape)} and {tuple(e.shape)}")
+
+
+def dequantize_blocks(q: torch.Tensor, e: torch.Tensor, k: int, rows: int = 1, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """The matrix [R, k] that (q, e) of quantize_blocks(v, rows) stands for."""
+    _check_blocks(q, e, k, rows, "dequantize_blocks")
+    if rows not in (1, BLOCK):
+        raise RuntimeError(f"dequantize_blocks: a block has 1 or {BLOCK} rows, got {rows}")
+    with L.on_device_of(q, e):
+        out = torch.empty((q.shape[0], k), device=q.device, dtype=dtype)
+        ty = L.stream_type(out, "dequantize_blocks")
+        L.check(L.load().nvp_dequantize_blocks(L.ptr(q.contiguous(), q.dtype), L.ptr(e.contiguous(), e.dtype), L.ptr(out, dtype), ty, q.shape[0], k, rows, L.stream_ptr()),
+                "nvp_dequantize_blocks")
+    return out
+
+
+def linear8(x: torch.Tensor, q: torch.Tensor, e: torch.Tensor, bias: torch.Tensor | None = None) -> torch.Tensor:
+    """x [..., K] (fp32 / bf16 / fp16) -> [..., N] of the same type: the linear layer whose weight [N, K] is (q, e) of
+    quantize_blocks(weight, 128), on x quantised row by row in blocks of 128 (inside the call); products in 8 bits, sums in fp32, bias of x's
+    type added before the one rounding.  A row with an infinity or a NaN gives a row of NaN.  Inference only."""
+    if x.dim() < 1:
+        raise RuntimeError("linear8 expects x [..., K]")
+    k = x.shape[-1]
+    _check_blocks(q, e, k, BLOCK, "linear8")
+    n = q.shape[0]
+    if n < 1:
+        raise RuntimeError("linear8: the weight has no rows")
+    ty = L.stream_type(x, "linear8")
+    if bias is not None and (bias.dtype != x.dtype or tuple(bias.shape) != (n,)):
+        raise RuntimeError(f"linear8: bias must be {x.dtype} [{n}], got {bias.dtype} {tuple(bias.shape)}")
+    if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
+        raise NotImplementedError("linear8 is an inference-only path: call it under torch.no_grad() or on tensors that need no gradient")
+    with L.on_device_of(x, q, e, bias):
+        lib = L.load()
+        xc = x.contiguous()
+        rows = xc.numel() // k
+        y = torch.empty(x.shape[:-1] + (n,), device=x.device, dtype=x.dtype)
+        need = lib.nvp_linear8_workspace_bytes(rows, k, n)
+        if need < 0:
+            L.check(int(need), "nvp_linear8_workspace_bytes")
+        ws = torch.empty(need, device=x.device, dtype=torch.uint8) if need else None
+        L.check(lib.nvp_linear8(L.ptr(xc, x.dtype), ty, L.ptr(q, q.dtype), L.ptr(e, e.dtype), L.ptr(bias.contiguous(), x.dtype) if bias is not None else None,
+                                L.ptr(y, x.dtype), rows, k, n, L.ptr(ws, torch.uint8), need, L.stream_ptr()), "nvp_linear8")
+    return y
+
+
+class Linear8(nn.Module):
+    """nn.Linear for 8-bit evaluation: holds the weight in block form (buffers `q`, `e`; 8 + 1 / 2048 bits per weight) and the bias."""
+
+    def __init__(self, in_features: int, out_features: int, bias: bool = True, dtype: torch.dtype = torch.float32, device=None):
+        super().__init__()
+        if in_features < 1 or out_features < 1:
+            raise ValueError("Linear8 needs at least one input and one output feature")
+        self.in_features, self.out_features = in_features, out_features
+        self.register_buffer("q", torch.zeros((out_features, _kblocks(in_features) * BLOCK), device=device, dtype=torch.float8_e4m3fn))
+        self.register_buffer("e", torch.full((_kblocks(out_features), _kblocks(in_features)), 127, device=device, dtype=torch.uint8))
+        self.register_buffer("bias", torch.zeros(out_features, device=device, dtype=dtype) if bias else None)
+
+    @classmethod
+    def from_linear(cls, layer: nn.Module) -> "Linear8":
+        """`layer`: anything with `.weight` [N, K] and `.bias` ([N] or None) on a HIP device (nn.Linear, modulation.Siren's linear part)."""
+        w, b = layer.weight.detach(), layer.bias
+        m = cls(w.shape[1], w.shape[0], bias=b is not None, dtype=w.dtype, device=w.device)
+        m.q, m.e = quantize_blocks(w, BLOCK)
+        if b is not None:
+            m.bias = b.detach().clone()
+        return m
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return linear8(x, self.q, self.e, self.bias)
+
+    def extra_repr(self) -> str:
+        return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}"
