@@ -327,6 +327,43 @@ int nvp_adamw_step(const nvp_adamw_seg* segs, int32_t n_segs, double lr, double 
 #define NVP_BF16 1
 #define NVP_F16 2
 
+/* ---- learned codes looked up by number (the discrete sibling of the grids; no counterpart in the reference) ---------------------------
+ * table [codes][dim], ids [n] int64 (ids64 != 0) or int32, out / dout [n][dim]; table_type NVP_F32 with any out_type, or a 16-bit type
+ * with the same out_type.  fwd: out[i] = scale * table[ids[i]]; a negative id is an empty slot (zeros), an id >= codes gives NaN.
+ * bwd: dtable[v] = scale * (sum of dout over the i with ids[i] == v), fp32 sums in a fixed order (sorted by id, then by position: no
+ * atomics, bit-reproducible); every element of dtable is OVERWRITTEN, rows no id points to with zeros; ids outside [0, codes) give
+ * no gradient.  workspace: nvp_lookup_bwd_workspace_bytes() bytes, 16-byte aligned. */
+int nvp_lookup_fwd(const void* ids, int32_t ids64, const void* table, int32_t table_type, void* out, int32_t out_type, int64_t n,
+                   int64_t codes, int64_t dim, float scale, void* stream);
+int64_t nvp_lookup_bwd_workspace_bytes(int64_t n, int64_t codes, int64_t dim);
+int nvp_lookup_bwd(const void* ids, int32_t ids64, const void* dout, int32_t out_type, void* dtable, int32_t table_type, int64_t n,
+                   int64_t codes, int64_t dim, float scale, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ---- gated residual step with the norms on both sides of a block (no counterpart in the reference, whose SirenNet only multiplies by
+ * the modulation, modulation.py:83-92) ---------------------------------------------------------------------------------------------
+ *   y = x + scale * act(gate) * h / rms(h) * post        rms(v) = sqrt(mean(v^2) + eps) over the row
+ *   u = y / rms(y) * next                                (y before it is rounded to its type)
+ * x, h, y, u [rows][dim]; gate [gate_rows][dim] (NULL: 1), row r of x uses gate row r / (rows / gate_rows); post, next [dim].
+ * h == NULL (then post, gate NULL): y = x is not written, u = x / rms(x) * next - the norm in front of the first block.
+ * next == NULL: no u.  gate_act 0: act(g) = g, 1: sigmoid.  weight_type: NVP_F32 or `type`.  dim up to 8192 (NVP_ERR_UNSUPPORTED). */
+typedef struct nvp_residual {
+    const void* x;
+    const void* h;
+    const void* gate;
+    const void* post;
+    const void* next;
+    int64_t rows, gate_rows;
+    int32_t dim, type, weight_type, gate_act;
+    float scale, eps;
+} nvp_residual;
+/* stats (fp32 [rows][2], the two 1 / rms) may be NULL when no backward pass follows. */
+int nvp_residual_fwd(const nvp_residual* a, void* y, void* u, float* stats, void* stream);
+/* Gradients; dy / du NULL: zero; every output may be NULL (not wanted).  Weight and shared-gate gradients are fp32 sums in a fixed order.
+ * workspace: nvp_residual_bwd_workspace_bytes() bytes, 16-byte aligned. */
+int64_t nvp_residual_bwd_workspace_bytes(const nvp_residual* a);
+int nvp_residual_bwd(const nvp_residual* a, const float* stats, const void* dy, const void* du, void* dx, void* dh, void* dgate, void* dpost,
+                     void* dnext, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* ---- 8-bit linear layer with one power-of-two scale per block of 128 (no counterpart in the reference, whose eval.py:19-109 quantises
  * the grids only) -----------------------------------------------------------------------------------------------------------------
  * Block form of a matrix v [rows][k]: q e4m3 bytes [rows][128 * ceil(k / 128)] (zeros behind column k), e exponent bytes

@@ -6,6 +6,9 @@ Module surface mirrors the reference's importable names:
 `nvp_amd.compat.install()` puts them on sys.modules under the reference's own top-level
 names (modules, tinycudann, sparsegrid, modulation, loss_functions) so the reference's
 train_video.py / eval.py import them unmodified.
+Next to that surface, without a counterpart in the reference, stand the conditioning operators: nvp_amd.codes.{lookup,
+CodeTable}, nvp_amd.trunk.{pre_norm, gated_residual, Trunk}, nvp_amd.quantize.{linear8, Linear8, quantize_blocks,
+dequantize_blocks}.
 """
 from . import _lib  # noqa: F401
 

@@ -65,6 +65,15 @@ class AdamwSeg(C.Structure):
     """struct nvp_adamw_seg - one tensor of an AdamW step."""
     _fields_ = [("param", C.c_void_p), ("grad", C.c_void_p), ("exp_avg", C.c_void_p), ("exp_avg_sq", C.c_void_p), ("n", C.c_int64)]
 
+
+class Residual(C.Structure):
+    """struct nvp_residual - one gated residual step (nvp_residual_fwd / _bwd)."""
+    _fields_ = [("x", C.c_void_p), ("h", C.c_void_p), ("gate", C.c_void_p), ("post", C.c_void_p), ("next", C.c_void_p),
+                ("rows", C.c_int64), ("gate_rows", C.c_int64),
+                ("dim", C.c_int32), ("type", C.c_int32), ("weight_type", C.c_int32), ("gate_act", C.c_int32),
+                ("scale", C.c_float), ("eps", C.c_float)]
+
+
 _p, _i64, _i32, _vp = C.c_void_p, C.c_int64, C.c_int32, C.c_void_p
 
 # name -> argtypes; every entry point returns int unless listed in _RESTYPES
@@ -108,6 +117,12 @@ SIGNATURES = {
     "nvp_order_by_rows": [_p, _p, _i64, C.POINTER(Levels), C.POINTER(Levels), _vp, _i64, _vp],
     "nvp_sample_gather": [_p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i32, _i32, _i32, _vp],
     "nvp_adamw_step": [C.POINTER(AdamwSeg), _i32, C.c_double, C.c_double, C.c_double, C.c_double, C.c_double, _i64, C.c_double, _vp],
+    "nvp_lookup_fwd": [_p, _i32, _p, _i32, _p, _i32, _i64, _i64, _i64, C.c_float, _vp],
+    "nvp_lookup_bwd_workspace_bytes": [_i64, _i64, _i64],
+    "nvp_lookup_bwd": [_p, _i32, _p, _i32, _p, _i32, _i64, _i64, _i64, C.c_float, _vp, _i64, _vp],
+    "nvp_residual_fwd": [C.POINTER(Residual), _p, _p, _p, _vp],
+    "nvp_residual_bwd_workspace_bytes": [C.POINTER(Residual)],
+    "nvp_residual_bwd": [C.POINTER(Residual), _p, _p, _p, _p, _p, _p, _p, _p, _vp, _i64, _vp],
     "nvp_quantize_blocks": [_p, _i32, _p, _p, _i64, _i64, _i32, _vp],
     "nvp_dequantize_blocks": [_p, _p, _p, _i32, _i64, _i64, _i32, _vp],
     "nvp_linear8_workspace_bytes": [_i64, _i64, _i64],
@@ -121,7 +136,7 @@ SIGNATURES = {
     "nvp_mlp_mfma_products": [],
 }
 _RESTYPES = {
-    "nvp_linear8_workspace_bytes": _i64,
+    "nvp_linear8_workspace_bytes": _i64, "nvp_lookup_bwd_workspace_bytes": _i64, "nvp_residual_bwd_workspace_bytes": _i64,
     "nvp_packed_fwd_floats": _i64, "nvp_packed_bwd_floats": _i64, "nvp_dw_partial_floats": _i64, "nvp_sample_order_workspace_bytes": _i64, "nvp_order_by_rows_workspace_bytes": _i64,
     "nvp_mlp_param_floats": _i64, "nvp_latent_rows": _i32, "nvp_version": C.c_char_p,
     "nvp_encode_bwd_workspace_bytes": _i64, "nvp_dz_stride": _i32, "nvp_dz_lm_supported": _i32, "nvp_mlp_mfma_products": _i32, "nvp_encode_mlp_fwd_supported": _i32, "nvp_encode_mlp_fwd_bwd_supported": _i32,

@@ -16,7 +16,7 @@
 set -euo pipefail
 cd "$(dirname "$0")"
 HIPCC=${HIPCC:-/opt/rocm/bin/hipcc}
-SRCS_PRODUCT="encode encode_bwd mlp_pack mlp_fwd mlp_fwd_b3 mlp_bwd mlp_bwd_b3r mlp_dw harness optim linear8"
+SRCS_PRODUCT="encode encode_bwd mlp_pack mlp_fwd mlp_fwd_b3 mlp_bwd mlp_bwd_b3r mlp_dw harness optim linear8 codes trunk"
 SRCS_EXPERIMENTS="$SRCS_PRODUCT encode_fwd_lds mlp_fwd_b3r mlp_bwd_b3 mlp_dw_glds"
 
 # build_lib OUT.so OBJDIR "extra flags" "sources"

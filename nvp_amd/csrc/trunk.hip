@@ -1,0 +1,437 @@
+// The gated residual step of a conditioning stack with the norms on both sides of its block, forward and backward (rows of D values):
+//     r1 = (mean h^2 + eps)^-1/2   n = h r1   y = x + s a(g) n p        (p: the norm behind the block, g: its gate, s: the residual scale)
+//     r2 = (mean y^2 + eps)^-1/2   v = y r2   u = v w                   (w: the norm in front of the next block; from y before it is rounded)
+// FORM both: y and u; last: y only; first: no h, u = norm(x) only.  a is the identity or the sigmoid; a gate row serves `share` rows of x.
+// Backward, E = dL/dy in all:  dv = du w,  c2 = mean(dv v),  E = dy + r2 (dv - v c2),  dx = E,
+//     dn = s a p E,  c1 = mean(dn n),  dh = r1 (dn - n c1),  dg = s E n p a'(g),  dp = sum s a E n,  dw = sum du v.
+// c1 needs E and so c2; written out it is s [sum q (dy + r2 dv) - r2 c2 sum q v] / D with q = a p n: three sums that need neither, so both means come from
+// ONE reduction per row instead of two in sequence.  r1, r2 are kept from forward (8 bytes per row); n, a, y, v are computed again from x, h, g.
+// All arithmetic and every sum is fp32; each result is rounded once to its type.  Bound by memory: 4-5 streams forward, 8-9 backward, each touched once.
+// One row is held in registers by a team of TEAM lanes, 8 values each (16-byte accesses: V = 8 of 16 bits, 4 of 32; V = 1 for widths or addresses that
+// do not allow it).
+#include "stream_types.h"
+
+namespace {
+
+enum { kBoth = 0, kFirst = 1, kLast = 2 };
+constexpr int kVals = 8;
+
+// sum over a team of `TEAM` consecutive lanes; every lane gets the result, bit-identical in every lane (butterfly; across waves: same order everywhere)
+template <int TEAM, int N> __device__ __forceinline__ void team_sum(float (&s)[N], float* red, int& flip) {
+#pragma unroll
+    for (int o = (TEAM < 64 ? TEAM : 64) / 2; o > 0; o >>= 1)
+#pragma unroll
+        for (int k = 0; k < N; ++k) s[k] += __shfl_xor(s[k], o);
+    if (TEAM > 64) {
+        constexpr int W = TEAM / 64;
+        float* r = red + flip * (W * N);                       // two alternating buffers: one barrier per reduction
+        flip ^= 1;
+        if ((threadIdx.x & 63) == 0)
+#pragma unroll
+            for (int k = 0; k < N; ++k) r[(threadIdx.x >> 6) * N + k] = s[k];
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            float t = 0.f;
+#pragma unroll
+            for (int w = 0; w < W; ++w) t += r[w * N + k];
+            s[k] = t;
+        }
+    }
+}
+
+// column of value j of this lane: vectors of V, team-strided, so that a wave's access is contiguous
+template <int TEAM, int V> __device__ __forceinline__ int col_of(int lane, int j) { return (j / V * TEAM + lane) * V + j % V; }
+
+template <typename T, int TEAM, int V> __device__ __forceinline__ void load_row(const T* __restrict__ p, int lane, int dim, float (&f)[kVals]) {
+#pragma unroll
+    for (int q = 0; q < kVals / V; ++q) {
+        const int c = (q * TEAM + lane) * V;
+        float t[V];
+        if (c < dim) nvp_load<T, V>(p + c, t);
+#pragma unroll
+        for (int e = 0; e < V; ++e) f[q * V + e] = c < dim ? t[e] : 0.f;
+    }
+}
+template <typename T, int TEAM, int V> __device__ __forceinline__ void store_row(T* __restrict__ p, int lane, int dim, const float (&f)[kVals]) {
+#pragma unroll
+    for (int q = 0; q < kVals / V; ++q) {
+        const int c = (q * TEAM + lane) * V;
+        float t[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) t[e] = f[q * V + e];
+        if (c < dim) nvp_store<T, V>(p + c, t);
+    }
+}
+
+__device__ __forceinline__ float sigmoid(float g) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504f * g)); }
+__device__ __forceinline__ float inv_rms(float sum, float inv_dim, float eps) { return 1.f / sqrtf(sum * inv_dim + eps); }
+
+struct Rows {
+    int64_t rows, share;
+    int dim, act;
+    float scale, eps, inv_dim;
+};
+
+template <typename T, typename W, int FORM, int TEAM, int V>
+__global__ __launch_bounds__(TEAM > 256 ? TEAM : 256) void residual_fwd_kernel(const T* __restrict__ x, const T* __restrict__ h, const T* __restrict__ gate, const W* __restrict__ post,
+                                                                               const W* __restrict__ next, T* __restrict__ y, T* __restrict__ u, float* __restrict__ stats, Rows R) {
+    constexpr int kTeams = TEAM > 256 ? 1 : 256 / TEAM;
+    __shared__ float red[TEAM > 64 ? 2 * TEAM / 64 : 1];
+    int flip = 0;
+    const int lane = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
+    float p[kVals], w[kVals];
+    if (FORM != kFirst) load_row<W, TEAM, V>(post, lane, R.dim, p);
+    if (FORM != kLast) load_row<W, TEAM, V>(next, lane, R.dim, w);
+    for (int64_t row = (int64_t)blockIdx.x * kTeams + team; row < R.rows; row += (int64_t)gridDim.x * kTeams) {
+        float yv[kVals], r1 = 0.f, r2 = 0.f;
+        load_row<T, TEAM, V>(x + row * R.dim, lane, R.dim, yv);
+        if (FORM != kFirst) {
+            float hv[kVals], gv[kVals], s[1] = {0.f};
+            load_row<T, TEAM, V>(h + row * R.dim, lane, R.dim, hv);
+            if (gate) load_row<T, TEAM, V>(gate + (R.share == 1 ? row : (int64_t)((uint32_t)row / (uint32_t)R.share)) * R.dim, lane, R.dim, gv);
+#pragma unroll
+            for (int j = 0; j < kVals; ++j) s[0] = __fmaf_rn(hv[j], hv[j], s[0]);
+            team_sum<TEAM, 1>(s, red, flip);
+            r1 = inv_rms(s[0], R.inv_dim, R.eps);
+#pragma unroll
+            for (int j = 0; j < kVals; ++j) {
+                const float a = gate ? (R.act ? sigmoid(gv[j]) : gv[j]) : 1.f;
+                yv[j] = __fmaf_rn(R.scale * a * p[j], hv[j] * r1, yv[j]);
+            }
+            store_row<T, TEAM, V>(y + row * R.dim, lane, R.dim, yv);
+        }
+        if (FORM != kLast) {
+            float s[1] = {0.f};
+#pragma unroll
+            for (int j = 0; j < kVals; ++j) s[0] = __fmaf_rn(yv[j], yv[j], s[0]);      // columns behind the last one hold zeros
+            team_sum<TEAM, 1>(s, red, flip);
+            r2 = inv_rms(s[0], R.inv_dim, R.eps);
+#pragma unroll
+            for (int j = 0; j < kVals; ++j) yv[j] = yv[j] * r2 * w[j];
+            store_row<T, TEAM, V>(u + row * R.dim, lane, R.dim, yv);
+        }
+        if (stats && lane == 0) *reinterpret_cast<float2*>(stats + 2 * row) = make_float2(r1, r2);
+    }
+}
+
+// Rows are cut into units of at most `unit` rows that lie within one gate row's share; a team walks whole units, so a shared gate's gradient is summed in
+// registers (a unit that is only a piece of the share leaves a partial sum).  dp and dw are summed over everything the workgroup has seen, the workgroup's
+// teams are added through LDS, and one partial row per workgroup goes to the workspace.  residual_reduce_kernel adds partial rows in a fixed order: no atomics,
+// results do not vary from run to run.
+struct Units {
+    int64_t units, per_share;      // units in all; units per group of rows that share a gate row (1 group of all rows where no gate row is shared)
+    int64_t share, unit;           // rows per such group, rows per unit
+};
+
+template <typename T, typename W, int FORM, int TEAM, int V>
+__global__ __launch_bounds__(TEAM > 256 ? TEAM : 256) void residual_bwd_kernel(const T* __restrict__ x, const T* __restrict__ h, const T* __restrict__ gate, const W* __restrict__ post,
+                                                                               const W* __restrict__ next, const float* __restrict__ stats, const T* __restrict__ dy,
+                                                                               const T* __restrict__ du, T* __restrict__ dx, T* __restrict__ dh, T* __restrict__ dgate,
+                                                                               float* __restrict__ dgate_part, float* __restrict__ dpost_part, float* __restrict__ dnext_part, Rows R,
+                                                                               Units U) {
+    constexpr int kTeams = TEAM > 256 ? 1 : 256 / TEAM, N = FORM == kBoth ? 3 : 1;
+    __shared__ float red[TEAM > 64 ? 2 * N * TEAM / 64 : 1];
+    __shared__ float comb[kTeams > 1 ? kTeams : 1][kTeams > 1 ? TEAM * kVals : 1];
+    int flip = 0;
+    const int lane = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
+    const bool summed = gate && R.share > 1;
+    float p[kVals], w[kVals], sp[kVals], sw[kVals], sg[kVals];
+#pragma unroll
+    for (int j = 0; j < kVals; ++j) sp[j] = sw[j] = 0.f;
+    if (FORM != kFirst) load_row<W, TEAM, V>(post, lane, R.dim, p);
+    if (FORM != kLast) load_row<W, TEAM, V>(next, lane, R.dim, w);
+    for (int64_t un = (int64_t)blockIdx.x * kTeams + team; un < U.units; un += (int64_t)gridDim.x * kTeams) {
+        const int64_t grp = un / U.per_share, piece = un - grp * U.per_share;
+        const int64_t first = grp * U.share + piece * U.unit, last = min(first + U.unit, (grp + 1) * U.share);
+        float a[kVals], da[kVals];                       // act(g) and its derivative
+#pragma unroll
+        for (int j = 0; j < kVals; ++j) {
+            a[j] = 1.f;
+            da[j] = sg[j] = 0.f;
+        }
+        for (int64_t row = first; row < last; ++row) {
+            float xv[kVals], n[kVals], e[kVals], dv[kVals];
+            const float2 st = *reinterpret_cast<const float2*>(stats + 2 * row);
+            if (FORM != kLast) load_row<T, TEAM, V>(x + row * R.dim, lane, R.dim, xv);
+            if (FORM != kFirst) load_row<T, TEAM, V>(h + row * R.dim, lane, R.dim, n);
+            if (FORM != kFirst && gate && (!summed || row == first)) {
+                load_row<T, TEAM, V>(gate + (summed ? grp : row) * R.dim, lane, R.dim, a);
+#pragma unroll
+                for (int j = 0; j < kVals; ++j) {
+                    da[j] = 1.f;
+                    if (R.act) {
+                        a[j] = sigmoid(a[j]);
+                        da[j] = a[j] * (1.f - a[j]);
+                    }
+                }
+            }
+            if (FORM != kFirst && dy) {
+                load_row<T, TEAM, V>(dy + row * R.dim, lane, R.dim, e);
+            } else {
+#pragma unroll
+                for (int j = 0; j < kVals; ++j) e[j] = 0.f;
+            }
+            if (FORM != kLast && du) {
+                load_row<T, TEAM, V>(du + row * R.dim, lane, R.dim, dv);
+            } else {
+#pragma unroll
+                for (int j = 0; j < kVals; ++j) dv[j] = 0.f;
+            }
+            float s[N];
+#pragma unroll
+            for (int k = 0; k < N; ++k) s[k] = 0.f;
+#pragma unroll
+            for (int j = 0; j < kVals; ++j) {
+                float q = 0.f;
+                if (FORM != kFirst) {
+                    n[j] *= st.x;
+                    q = a[j] * p[j] * n[j];
+                }
+                if (FORM == kLast) {
+                    s[0] = __fmaf_rn(q, e[j], s[0]);
+                } else {
+                    const float v = (FORM == kBoth ? __fmaf_rn(R.scale, q, xv[j]) : xv[j]) * st.y;
+                    xv[j] = v;
+                    sw[j] = __fmaf_rn(dv[j], v, sw[j]);
+                    dv[j] *= w[j];
+                    s[0] = __fmaf_rn(dv[j], v, s[0]);
+                    e[j] = __fmaf_rn(st.y, dv[j], e[j]);
+                    if constexpr (FORM == kBoth) {
+                        s[N - 2] = __fmaf_rn(q, e[j], s[N - 2]);
+                        s[N - 1] = __fmaf_rn(q, v, s[N - 1]);
+                    }
+                }
+            }
+            team_sum<TEAM, N>(s, red, flip);
+            float c1 = 0.f;                                // mean(dn n)
+            if (FORM != kLast) {
+                const float c2 = st.y * s[0] * R.inv_dim;
+#pragma unroll
+                for (int j = 0; j < kVals; ++j) e[j] = __fmaf_rn(-c2, xv[j], e[j]);
+                if constexpr (FORM == kBoth) c1 = R.scale * R.inv_dim * (s[N - 2] - c2 * s[N - 1]);
+            } else {
+                c1 = R.scale * R.inv_dim * s[0];
+            }
+            if (dx) store_row<T, TEAM, V>(dx + row * R.dim, lane, R.dim, e);
+            if (FORM != kFirst) {
+                float t[kVals];
+#pragma unroll
+                for (int j = 0; j < kVals; ++j) {
+                    const float en = R.scale * e[j] * n[j];
+                    sp[j] = __fmaf_rn(a[j], en, sp[j]);
+                    t[j] = en * p[j] * da[j];
+                    n[j] = st.x * __fmaf_rn(-c1, n[j], R.scale * a[j] * p[j] * e[j]);
+                }
+                if (dh) store_row<T, TEAM, V>(dh + row * R.dim, lane, R.dim, n);
+                if (summed) {
+#pragma unroll
+                    for (int j = 0; j < kVals; ++j) sg[j] += t[j];
+                } else if (dgate) {
+                    store_row<T, TEAM, V>(dgate + row * R.dim, lane, R.dim, t);
+                }
+            }
+        }
+        if (FORM != kFirst && summed && dgate) {
+            if (U.per_share == 1) store_row<T, TEAM, V>(dgate + grp * R.dim, lane, R.dim, sg);
+            else store_row<float, TEAM, V>(dgate_part + un * R.dim, lane, R.dim, sg);
+        }
+    }
+    // one partial row per workgroup for each weight
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+        float* out = which ? dnext_part : dpost_part;
+        if ((which ? FORM == kLast : FORM == kFirst) || !out) continue;
+        if (kTeams > 1) {
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < kVals; ++j) comb[team][col_of<TEAM, V>(lane, j)] = which ? sw[j] : sp[j];
+            __syncthreads();
+            for (int c = threadIdx.x; c < R.dim; c += 256) {
+                float t = 0.f;
+#pragma unroll
+                for (int k = 0; k < kTeams; ++k) t += comb[k][c];
+                out[(int64_t)blockIdx.x * R.dim + c] = t;
+            }
+        } else {
+            store_row<float, TEAM, V>(out + (int64_t)blockIdx.x * R.dim, lane, R.dim, which ? sw : sp);
+        }
+    }
+}
+
+// out[j][c] = sum over `rows_of(job)` partial rows.  Jobs: 0 dpost, 1 dnext (rows = workgroups of the kernel above), 2 + g gate row g (rows = pieces).
+// 32 columns x 32 row lanes per workgroup: every lane adds its rows in order, the lanes are added in order.
+template <typename T, typename W>
+__global__ __launch_bounds__(1024) void residual_reduce_kernel(const float* __restrict__ dpost_part, const float* __restrict__ dnext_part, const float* __restrict__ dgate_part,
+                                                               W* __restrict__ dpost, W* __restrict__ dnext, T* __restrict__ dgate, int dim, int64_t groups, int64_t pieces) {
+    __shared__ float part[32][33];
+    const int c = blockIdx.x * 32 + (threadIdx.x & 31), r0 = threadIdx.x >> 5;
+    const int job = blockIdx.y;
+    const float* src = job == 0 ? dpost_part : job == 1 ? dnext_part : dgate_part + (int64_t)(job - 2) * pieces * dim;
+    if ((job == 0 && !dpost) || (job == 1 && !dnext)) return;                  // uniform over the workgroup
+    const int64_t rows = job < 2 ? groups : pieces;
+    float s = 0.f;
+    if (c < dim)
+        for (int64_t r = r0; r < rows; r += 32) s += src[r * dim + c];
+    part[r0][threadIdx.x & 31] = s;
+    __syncthreads();
+    if (r0 == 0 && c < dim) {
+        float t = 0.f;
+#pragma unroll
+        for (int k = 0; k < 32; ++k) t += part[k][threadIdx.x & 31];
+        if (job == 0) dpost[c] = (W)t;
+        else if (job == 1) dnext[c] = (W)t;
+        else dgate[(int64_t)(job - 2) * dim + c] = (T)t;
+    }
+}
+
+constexpr int kMaxDim = 8192;
+int team_of(int dim) { return dim <= 128 ? 16 : dim <= 512 ? 64 : dim <= 2048 ? 256 : dim <= 4096 ? 512 : 1024; }
+
+struct Plan {
+    Units U;
+    int64_t groups;        // workgroups of the backward kernel
+    bool parts;            // gate gradients leave partial rows
+    int64_t gate_rows;
+};
+Plan plan_of(const nvp_residual* a) {
+    Plan P;
+    const int team = team_of(a->dim), teams = team > 256 ? 1 : 256 / team;
+    const bool shared = a->gate && a->gate_rows < a->rows;
+    P.gate_rows = shared ? a->gate_rows : 0;
+    P.U.share = shared ? a->rows / a->gate_rows : a->rows;
+    // enough workgroups to fill the chip (256 CUs, 1024 lanes of work each), few enough that their partial rows stay a small part of the traffic
+    const int64_t want = (int64_t)(team >= 512 ? 512 : 1024) * teams;
+    const int64_t rows_per = (a->rows + want - 1) / want;
+    P.U.unit = rows_per < P.U.share ? rows_per : P.U.share;
+    P.U.per_share = (P.U.share + P.U.unit - 1) / P.U.unit;
+    P.U.units = (shared ? a->gate_rows : 1) * P.U.per_share;
+    P.parts = shared && P.U.per_share > 1;
+    const int64_t g = (P.U.units + teams - 1) / teams;
+    P.groups = g < 1024 ? g : 1024;
+    return P;
+}
+
+int check(const nvp_residual* a) {
+    if (!a || a->rows < 0 || a->rows > (1ll << 31) - 1 || a->dim < 1 || !nvp_type_size(a->type) || !nvp_type_size(a->weight_type)) return NVP_ERR_BADARG;
+    if (a->weight_type != NVP_F32 && a->weight_type != a->type) return NVP_ERR_BADARG;
+    if (a->gate_act < 0 || a->gate_act > 1 || !(a->eps >= 0.f)) return NVP_ERR_BADARG;
+    if (!a->h && !a->next) return NVP_ERR_BADARG;
+    if ((a->h != nullptr) != (a->post != nullptr) || (a->gate && !a->h)) return NVP_ERR_BADARG;
+    if (a->gate && (a->gate_rows < 1 || (a->rows && (a->gate_rows > a->rows || a->rows % a->gate_rows)))) return NVP_ERR_BADARG;
+    return a->dim > kMaxDim ? NVP_ERR_UNSUPPORTED : 0;
+}
+
+struct Call {
+    const nvp_residual* a;
+    void *y, *u, *dx, *dh, *dgate, *dpost, *dnext;
+    float* stats;
+    const void *dy, *du;
+    float *dgate_part, *dpost_part, *dnext_part;
+    Plan P;
+    bool backward;
+    hipStream_t st;
+};
+
+template <typename T, typename W, int FORM, int TEAM, int V> int launch(const Call& c) {
+    const nvp_residual* a = c.a;
+    constexpr int kTeams = TEAM > 256 ? 1 : 256 / TEAM, kThreads = TEAM > 256 ? TEAM : 256;
+    const Rows R{a->rows, a->gate ? a->rows / a->gate_rows : 1, a->dim, a->gate_act, a->scale, a->eps, 1.f / (float)a->dim};
+    if (!c.backward) {
+        const int64_t need = (a->rows + kTeams - 1) / kTeams, cap = 256 * (2048 / kThreads);
+        hipLaunchKernelGGL((residual_fwd_kernel<T, W, FORM, TEAM, V>), dim3((unsigned)(need < cap ? need : cap)), dim3(kThreads), 0, c.st, (const T*)a->x, (const T*)a->h, (const T*)a->gate,
+                           (const W*)a->post, (const W*)a->next, (T*)c.y, (T*)c.u, c.stats, R);
+        NVP_LAUNCH_CHECK();
+        return 0;
+    }
+    hipLaunchKernelGGL((residual_bwd_kernel<T, W, FORM, TEAM, V>), dim3((unsigned)c.P.groups), dim3(kThreads), 0, c.st, (const T*)a->x, (const T*)a->h, (const T*)a->gate, (const W*)a->post,
+                       (const W*)a->next, c.stats, (const T*)c.dy, (const T*)c.du, (T*)c.dx, (T*)c.dh, (T*)c.dgate, c.dgate_part, c.dpost ? c.dpost_part : nullptr,
+                       c.dnext ? c.dnext_part : nullptr, R, c.P.U);
+    NVP_LAUNCH_CHECK();
+    const bool gsum = c.P.parts && c.dgate;
+    if (c.dpost || c.dnext || gsum) {
+        hipLaunchKernelGGL((residual_reduce_kernel<T, W>), dim3((unsigned)((a->dim + 31) / 32), (unsigned)(2 + (gsum ? c.P.gate_rows : 0))), dim3(1024), 0, c.st, c.dpost_part, c.dnext_part,
+                           c.dgate_part, (W*)c.dpost, (W*)c.dnext, (T*)c.dgate, a->dim, c.P.groups, c.P.U.per_share);
+        NVP_LAUNCH_CHECK();
+    }
+    return 0;
+}
+
+template <typename T, typename W, int FORM, int V> int by_team(const Call& c) {
+    switch (team_of(c.a->dim)) {
+        case 16: return launch<T, W, FORM, 16, V>(c);
+        case 64: return launch<T, W, FORM, 64, V>(c);
+        case 256: return launch<T, W, FORM, 256, V>(c);
+        case 512: return launch<T, W, FORM, 512, V>(c);
+        default: return launch<T, W, FORM, 1024, V>(c);
+    }
+}
+template <typename T, typename W> int by_form(const Call& c) {
+    constexpr int V = 16 / sizeof(T);
+    const nvp_residual* a = c.a;
+    uintptr_t all = 0;
+    for (const void* p : {a->x, a->h, a->gate, c.dy, c.du, (const void*)c.y, (const void*)c.u, (const void*)c.dx, (const void*)c.dh, (const void*)c.dgate}) all |= (uintptr_t)p;
+    const uintptr_t weights = (uintptr_t)a->post | (uintptr_t)a->next;
+    const bool vec = nvp_vec_width(a->dim, sizeof(T), all, V) == V && nvp_vec_width(a->dim, sizeof(W), weights, V) == V;      // W rows: 16 or 32 bytes
+    if (!a->h) return vec ? by_team<T, W, kFirst, V>(c) : by_team<T, W, kFirst, 1>(c);
+    if (!a->next) return vec ? by_team<T, W, kLast, V>(c) : by_team<T, W, kLast, 1>(c);
+    return vec ? by_team<T, W, kBoth, V>(c) : by_team<T, W, kBoth, 1>(c);
+}
+int by_type(const Call& c) {
+    const bool wide = c.a->weight_type == NVP_F32;
+    if (c.a->type == NVP_F32) return by_form<float, float>(c);
+    if (c.a->type == NVP_BF16) return wide ? by_form<nvp_bf16, float>(c) : by_form<nvp_bf16, nvp_bf16>(c);
+    return wide ? by_form<nvp_f16, float>(c) : by_form<nvp_f16, nvp_f16>(c);
+}
+
+int64_t gate_part_rows(const Plan& P) { return P.parts ? P.U.units : 0; }
+
+}  // namespace
+
+extern "C" int nvp_residual_fwd(const nvp_residual* a, void* y, void* u, float* stats, void* stream) {
+    const int rc = check(a);
+    if (rc) return rc;
+    if (a->rows == 0) return 0;
+    if (!a->x || (a->h && !y) || (a->next && !u)) return NVP_ERR_BADARG;
+    Call c{};
+    c.a = a;
+    c.y = y;
+    c.u = u;
+    c.stats = stats;
+    c.st = (hipStream_t)stream;
+    return by_type(c);
+}
+
+extern "C" int64_t nvp_residual_bwd_workspace_bytes(const nvp_residual* a) {
+    const int rc = check(a);
+    if (rc) return rc;
+    if (a->rows == 0) return 0;
+    const Plan P = plan_of(a);
+    return (gate_part_rows(P) + P.groups * ((a->h ? 1 : 0) + (a->next ? 1 : 0))) * a->dim * 4;
+}
+
+extern "C" int nvp_residual_bwd(const nvp_residual* a, const float* stats, const void* dy, const void* du, void* dx, void* dh, void* dgate, void* dpost, void* dnext, void* workspace,
+                                int64_t workspace_bytes, void* stream) {
+    const int rc = check(a);
+    if (rc) return rc;
+    if (a->rows == 0) return 0;
+    if (!a->x || !stats || workspace_bytes < nvp_residual_bwd_workspace_bytes(a) || !workspace || ((uintptr_t)workspace & 15)) return NVP_ERR_BADARG;
+    if ((!a->h && (dh || dpost || dy)) || (!a->next && (dnext || du)) || (!a->gate && dgate)) return NVP_ERR_BADARG;
+    Call c{};
+    c.a = a;
+    c.backward = true;
+    c.stats = const_cast<float*>(stats);
+    c.dy = dy;
+    c.du = du;
+    c.dx = dx;
+    c.dh = dh;
+    c.dgate = dgate;
+    c.dpost = dpost;
+    c.dnext = dnext;
+    c.P = plan_of(a);
+    c.dgate_part = (float*)workspace;
+    c.dpost_part = c.dgate_part + gate_part_rows(c.P) * a->dim;
+    c.dnext_part = c.dpost_part + (a->h ? c.P.groups * a->dim : 0);
+    c.st = (hipStream_t)stream;
+    return by_type(c);
+}

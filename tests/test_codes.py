@@ -1,0 +1,260 @@
+"""Learned codes by number (nvp_amd.codes) against a plain 64-bit evaluation, and their refusals.
+
+Tolerances.  Forward: one fp32 product (2^-24 of it) and one rounding to the output type (eps / 2); exact where scale is 1.  Gradient of a row that c
+positions point to: c - 1 fp32 additions and one product, each off by at most 2^-24 of a partial sum that never exceeds S = |scale| sum |dout|, then one
+rounding: |got - exact| <= (c + 1) 2^-24 S + eps / 2 |exact| (+ the smallest number of the type)."""
+import ctypes
+
+import pytest
+import torch
+
+from nvp_amd import _lib as L
+from nvp_amd import codes, functional
+
+F32, B16, F16 = torch.float32, torch.bfloat16, torch.float16
+PAIRS = [(F32, F32), (F32, B16), (F32, F16), (B16, B16), (F16, F16)]
+
+
+def dev():
+    return torch.device("cuda:0")
+
+
+def plain(ids, table, scale):
+    ids = ids.cpu().long()
+    out = table.detach().cpu().double()[ids.clamp(0, table.shape[0] - 1)] * scale
+    out[ids < 0] = 0.0
+    out[ids >= table.shape[0]] = float("nan")
+    return out
+
+
+def plain_grad(ids, dout, n_codes, scale):
+    """(gradient, S, positions per row) in float64"""
+    ids, d = ids.cpu().long().flatten(), dout.cpu().double().reshape(-1, dout.shape[-1]) * scale
+    ok = (ids >= 0) & (ids < n_codes)
+    g, s = torch.zeros(n_codes, d.shape[1], dtype=torch.float64), torch.zeros(n_codes, d.shape[1], dtype=torch.float64)
+    g.index_add_(0, ids[ok], d[ok])
+    s.index_add_(0, ids[ok], d[ok].abs())
+    return g, s, torch.bincount(ids[ok], minlength=n_codes)[:, None].double()
+
+
+def check(ids, table, scale, dtype):
+    t = table.clone().requires_grad_(True)
+    out = codes.lookup(ids, t, scale, dtype)
+    dtype = table.dtype if dtype is None else dtype
+    assert out.dtype == dtype and out.shape == ids.shape + (table.shape[1],)
+    want = plain(ids, table, scale)
+    half = torch.finfo(dtype).eps / 2
+    got = out.detach().double().cpu()
+    nan = want.isnan()
+    assert torch.equal(got.isnan(), nan)
+    err = (got - want).abs()[~nan]
+    assert bool((err <= (half + 2.0 ** -24 * (1 + half)) * want.abs()[~nan] + torch.finfo(dtype).tiny).all())
+    if scale == 1.0:
+        assert torch.equal(got[~nan], want.to(dtype).double()[~nan])
+    dout = torch.randn(out.shape, device=out.device).to(dtype)
+    g, = torch.autograd.grad(out, t, dout)
+    assert g.dtype == table.dtype and g.shape == table.shape
+    want, s, c = plain_grad(ids, dout, table.shape[0], scale)
+    gh = torch.finfo(table.dtype).eps / 2
+    err = (g.double().cpu() - want).abs()
+    assert bool((err <= (c + 1) * 2.0 ** -24 * s * (1 + gh) + gh * want.abs() + torch.finfo(table.dtype).tiny).all()), float(err.max())
+    assert not g.cpu()[(c == 0).flatten()].any()
+    again, = torch.autograd.grad(codes.lookup(ids, t, scale, dtype), t, dout)
+    assert torch.equal(g, again)
+    return g
+
+
+# ---- on the host -------------------------------------------------------------------------------------------------------------------------------
+def test_refusals_on_the_host(monkeypatch):
+    ids, table = torch.zeros(3, dtype=torch.int64), torch.zeros(4, 5)
+    with pytest.raises(RuntimeError, match="HIP device"):
+        codes.lookup(ids, table)
+    with pytest.raises(RuntimeError, match="int64 or int32"):
+        codes.lookup(ids.float(), table)
+    with pytest.raises(RuntimeError, match="int64 or int32"):
+        codes.lookup(ids.bool(), table)
+    for bad in (torch.zeros(5), torch.zeros(0, 5), torch.zeros(5, 0)):
+        with pytest.raises(RuntimeError, match="at least one code"):
+            codes.lookup(ids, bad)
+    with pytest.raises(RuntimeError, match="float32, bfloat16 or float16"):
+        codes.lookup(ids, table.double())
+    with pytest.raises(RuntimeError, match="cannot be read as"):
+        codes.lookup(ids, table.bfloat16(), dtype=torch.float32)
+    with pytest.raises(RuntimeError, match="cannot be read as"):
+        codes.lookup(ids, table, dtype=torch.float64)
+    with pytest.raises(RuntimeError, match="finite"):
+        codes.lookup(ids, table, scale=float("nan"))
+    with pytest.raises(ValueError):
+        codes.CodeTable(0, 4)
+    m = codes.CodeTable(6, 3, scale=2.0)
+    assert list(m.state_dict()) == ["codes"] and m.codes.shape == (6, 3) and float(m.codes.abs().max()) <= 1e-4
+
+
+def test_entry_points_refuse_bad_arguments_without_a_device():
+    lib, d = L.load(), ctypes.c_void_p(64)                             # never dereferenced
+    assert lib.nvp_lookup_fwd(None, 1, d, 0, d, 0, 5, 4, 3, 1.0, None) == L.ERR_BADARG
+    assert lib.nvp_lookup_fwd(d, 1, d, 1, d, 0, 5, 4, 3, 1.0, None) == L.ERR_BADARG           # a bf16 table read as fp32
+    assert lib.nvp_lookup_fwd(d, 1, d, 0, d, 0, 5, 0, 3, 1.0, None) == L.ERR_BADARG
+    assert lib.nvp_lookup_fwd(d, 1, d, 0, d, 0, 1 << 31, 4, 3, 1.0, None) == L.ERR_UNSUPPORTED
+    assert lib.nvp_lookup_fwd(None, 1, None, 0, None, 0, 0, 4, 3, 1.0, None) == 0
+    need = lib.nvp_lookup_bwd_workspace_bytes(5000, 70, 16)
+    assert need > 5000 * 4 * 4
+    assert lib.nvp_lookup_bwd(d, 1, d, 0, d, 0, 5000, 70, 16, 1.0, d, need - 1, None) == L.ERR_BADARG
+    assert lib.nvp_lookup_bwd(d, 1, d, 0, None, 0, 5000, 70, 16, 1.0, d, need, None) == L.ERR_BADARG
+    assert lib.nvp_lookup_bwd(d, 1, d, 0, d, 0, 5000, 70, 16, 1.0, ctypes.c_void_p(8), need, None) == L.ERR_BADARG
+    assert lib.nvp_lookup_bwd_workspace_bytes(-1, 70, 16) == L.ERR_BADARG
+
+
+# ---- on the device -----------------------------------------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("table_dtype,dtype", PAIRS)
+@pytest.mark.parametrize("n,n_codes,dim", [(1, 1, 1), (3, 2, 7), (50, 1000, 64), (1000, 13, 33), (4096, 600, 32), (4097, 1500, 114), (20000, 5, 1024), (70000, 300, 40), (40000, 70000, 24)])
+def test_lookup(n, n_codes, dim, table_dtype, dtype):
+    g = torch.Generator().manual_seed(n + n_codes + dim)
+    table = torch.randn(n_codes, dim, generator=g).to(table_dtype).to(dev())
+    ids = torch.randint(0, n_codes, (n,), generator=g).to(dev())
+    check(ids, table, 1.0 if n % 2 else 5.25, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [5, 300, 4096, 5000, 70000])
+@pytest.mark.parametrize("kind", ["one id", "all empty", "two", "frequent", "descending", "first and last", "outside"])
+def test_lookup_distributions(kind, n):
+    """Runs that cross every kind of boundary: one id everywhere (all levels), runs cut by chunks, ids at both ends of the table, slots without an id."""
+    n_codes, dim = 517, 20
+    g = torch.Generator().manual_seed(n)
+    i = torch.arange(n)
+    ids = {"one id": torch.full((n,), 300), "all empty": torch.full((n,), -1), "two": i % 2 * 516, "frequent": torch.where(torch.rand(n, generator=g) < 0.9, 7, i % n_codes),
+           "descending": (n - 1 - i) * n_codes // n, "first and last": torch.where(i < n // 3, 0, torch.where(i < n // 2, -1, 516)),
+           "outside": torch.randint(-100, 700, (n,), generator=g)}[kind]
+    table = torch.randn(n_codes, dim, generator=g).to(dev())
+    check(ids.to(dev()), table, 0.5, None)
+    check(ids.to(torch.int32).to(dev()), table, 1.0, torch.bfloat16)
+
+
+@pytest.mark.gpu
+def test_lookup_long_list_of_one_id_and_large_numbers():
+    """1.3 million positions in four levels; a table whose offsets pass 2^32 bytes and whose ids need three radix passes."""
+    table = torch.randn(3, 8, device=dev())
+    ids = torch.full((1300000,), 1, device=dev())
+    ids[5] = 2
+    check(ids, table, 1.0, None)
+    n_codes = (1 << 21) + 5
+    big = torch.zeros(n_codes, 640, device=dev(), dtype=torch.bfloat16).requires_grad_(True)     # 2.7 GB: 1.3e9 elements
+    at = torch.tensor([n_codes - 1, 0, n_codes - 1, 1 << 20, 77] + [n_codes - 2] * 5000, device=dev())
+    with torch.no_grad():
+        big[n_codes - 1] = 3.0
+        big[n_codes - 2] = 2.0
+    out = codes.lookup(at, big)
+    assert bool((out[0] == 3).all()) and bool((out[2] == 3).all()) and not out[1].any() and bool((out[5:] == 2).all())
+    d = torch.ones_like(out)
+    d[2] = 0.5
+    g, = torch.autograd.grad(out, big, d)
+    assert bool((g[n_codes - 1] == 1.5).all()) and bool((g[0] == 1).all()) and bool((g[77] == 1).all()) and bool((g[1 << 20] == 1).all())
+    assert bool((g[n_codes - 2] == 4992).all())                        # 5000 in bf16 (steps of 32)
+    assert int(torch.count_nonzero(g.sum(1))) == 5
+
+
+@pytest.mark.gpu
+def test_lookup_shapes_strides_and_empty_batches():
+    table = torch.randn(40, 12, device=dev())
+    ids = torch.randint(0, 40, (6, 10), device=dev())
+    assert torch.equal(codes.lookup(ids.t(), table), table[ids.t()])
+    assert torch.equal(codes.lookup(ids[:, ::3], table[:, 3:9]), table[:, 3:9][ids[:, ::3]])       # rows 12 apart: copied first
+    assert torch.equal(codes.lookup(torch.tensor(7, device=dev()), table), table[7])
+    t = table.clone().requires_grad_(True)
+    out = codes.lookup(ids[:0], t)
+    assert out.shape == (0, 10, 12)
+    g, = torch.autograd.grad(out, t, torch.zeros_like(out))
+    assert g.shape == t.shape and not g.any()
+    # a column slice of a gradient and an expanded one reach the kernel as they are
+    out = codes.lookup(ids, t)
+    g, = torch.autograd.grad(out.sum(), t)
+    want, s, c = plain_grad(ids, torch.ones(6, 10, 12), 40, 1.0)
+    assert torch.equal(g.cpu().double(), want)
+
+
+@pytest.mark.gpu
+def test_lookup_non_finite_values_stay_in_their_rows():
+    table = torch.randn(9, 6, device=dev())
+    table[4, 2] = float("inf")
+    ids = torch.tensor([4, 1, 4, 3, -1], device=dev())
+    t = table.clone().requires_grad_(True)
+    out = codes.lookup(ids, t)
+    assert bool(out[0, 2].isinf()) and int((~out.isfinite()).sum()) == 2
+    d = torch.ones_like(out)
+    d[4] = float("nan")                                                # the gradient of an empty slot reaches nothing
+    d[1, 0] = float("inf")
+    g, = torch.autograd.grad(out, t, d)
+    assert bool(g[1, 0].isinf()) and int((~g.isfinite()).sum()) == 1
+
+
+@pytest.mark.gpu
+def test_lookup_verifies_ids_on_request(monkeypatch):
+    monkeypatch.setattr(functional, "CHECK_IDS", True)
+    table = torch.randn(4, 4, device=dev())
+    codes.lookup(torch.tensor([3, -1], device=dev()), table)
+    with pytest.raises(IndexError, match="id 4 in a table of 4"):
+        codes.lookup(torch.tensor([1, 4], device=dev()), table)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [33, 3000, 9000])
+def test_lookup_gradient_captured_and_replayed(n):
+    """The plain calls inside a captured graph, replayed with other ids and other work between the replays."""
+    table = torch.randn(700, 48, device=dev())
+    ids, dout = torch.randint(0, 700, (n,), device=dev()), torch.randn(n, 48, device=dev())
+
+    def step():
+        t = table.detach().requires_grad_(True)
+        out = codes.lookup(ids, t, 2.0)
+        return out.detach(), torch.autograd.grad(out, t, dout)[0]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for k in range(4):
+        ids.copy_(torch.randint(-2, 700, (n,), device=dev()) // (1 + 300 * (k == 2)))
+        dout.copy_(torch.randn(n, 48, device=dev()))
+        graph.replay()
+        want = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
+def test_lookup_two_streams_at_once():
+    tables = [torch.randn(90, 64, device=dev()) for _ in range(2)]
+    ids = [torch.randint(0, 90, (9000,), device=dev()) for _ in range(2)]
+    dout = [torch.randn(9000, 64, device=dev()) for _ in range(2)]
+
+    def step(i):
+        t = tables[i].detach().requires_grad_(True)
+        return torch.autograd.grad(codes.lookup(ids[i], t), t, dout[i])[0]
+    want = [step(i) for i in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(4):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got.append((i, step(i)))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want[i]) for i, g in got)
+
+
+@pytest.mark.gpu
+def test_code_table_trains_with_the_one_launch_optimizer():
+    from nvp_amd.optim import AdamW
+    m = codes.CodeTable(30, 16, scale=4.0).to(dev())
+    opt = AdamW(m.parameters(), lr=1e-2)
+    ids = torch.arange(20, device=dev()).repeat(3)
+    before = m.codes.detach().clone()
+    m(ids).square().sum().backward()
+    opt.step()
+    moved = (m.codes.detach() - before).abs().amax(1)
+    assert bool((moved[:20] > 0).all()) and bool((moved[20:] <= 1e-2 * 1e-2 * 1e-4 * 1.01).all())   # rows no id points to only decay
