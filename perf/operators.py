@@ -185,8 +185,12 @@ def _residual(c, s):
         if c["form"] == "first":
             outs, seeds = [trunk.pre_norm(s["x"], s["next"], eps=EPS)], [s.get("du")]
         else:
-            r = trunk.gated_residual(s["x"], s["h"], s.get("gate"), s["post"], s.get("next"), scale=c["scale"], gate_act=act, eps=EPS)
+            x, h, gate = s["x"], s["h"], s.get("gate")
+            if c["gate"] == "shared":                                                        # [sequences, positions, dim] with a gate [sequences, 1, dim]
+                x, h, gate = x.view(-1, c["share"], c["dim"]), h.view(-1, c["share"], c["dim"]), gate.view(-1, 1, c["dim"])
+            r = trunk.gated_residual(x, h, gate, s["post"], s.get("next"), scale=c["scale"], gate_act=act, eps=EPS)
             outs, seeds = ([r], [s.get("dy")]) if c["form"] == "last" else (list(r), [s.get("dy"), s.get("du")])
+            outs = [o.view(c["rows"], c["dim"]) for o in outs]
         if not c["train"]:
             return outs
         leaves = [s[k] for k in ("x", "h", "gate", "post", "next") if k in s]
