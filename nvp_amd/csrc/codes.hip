@@ -33,7 +33,8 @@ __global__ __launch_bounds__(256) void lookup_fwd_kernel(const I* __restrict__ i
     int64_t id[kRows];
 #pragma unroll
     for (int r = 0; r < kRows; ++r) id[r] = r0 + r * kTeams < n ? (int64_t)ids[r0 + r * kTeams] : -1;
-    for (int c = lane * V; c < dim; c += TEAM * V) {
+    for (int c0 = lane * V; c0 < dim; c0 += TEAM * V) {
+        const int c = min(c0, dim - V);                              // the last vector of an odd width is moved back: its first columns are written twice, with the same values
         float f[kRows][V];
 #pragma unroll
         for (int r = 0; r < kRows; ++r) {
@@ -186,15 +187,15 @@ __global__ __launch_bounds__(256) void sum_runs_kernel(const unsigned* __restric
         while (todo) {
             const int64_t at = r0 + __ffsll((long long)todo) - 1;
             todo &= todo - 1;
-            for (int c = lane * V; c < cw; c += 64 * V) nvp_store<T, V>(dtable + at * dim + c0 + c, zero);
+            for (int c = lane * V; c < cw; c += 64 * V) nvp_store<T, V>(dtable + at * dim + min(c0 + c, dim - V), zero);
         }
         return;
     }
     const int lane = threadIdx.x % TEAM;
     const int64_t ch = (int64_t)blockIdx.x * kTeams + threadIdx.x / TEAM;
     if (ch >= chunks) return;
-    const int c = (blockIdx.y * TEAM + lane) * V;
-    const bool live = c < dim;
+    const bool live = (blockIdx.y * TEAM + lane) * V < dim;
+    const int c = min((int)(blockIdx.y * TEAM + lane) * V, dim - V);      // the last vector of an odd width is moved back: its first columns are summed and written twice, alike
     const int64_t lo = ch * per_chunk, hi = min(lo + per_chunk, m);
     const unsigned before = lo > 0 ? keys[lo - 1] : kEmpty, after = hi < m ? keys[hi] : kEmpty;
     unsigned cur = kEmpty, head_key = kEmpty, tail_key = kEmpty;
@@ -402,9 +403,7 @@ int bwd(const I* ids, const S* dout, T* dtable, int64_t n, int64_t codes, int di
         }
     }
     constexpr int V = vec_of<S, T>();
-    const uintptr_t all = (uintptr_t)dout | (uintptr_t)dtable;
-    const bool vec = nvp_vec_width(dim, 16 / V, all, V) == V;
-    if (vec) return sums<S, T, V, 4>(P, key[at], pos[at], dout, dtable, ws, codes, dim, scale, st);
+    if (dim >= (V > 4 ? V : 4)) return sums<S, T, V, 4>(P, key[at], pos[at], dout, dtable, ws, codes, dim, scale, st);
     return sums<S, T, 1, 1>(P, key[at], pos[at], dout, dtable, ws, codes, dim, scale, st);
 }
 
@@ -412,7 +411,7 @@ template <typename T, typename O>
 int any_ids(const void* ids, int ids64, const void* a, void* b, bool backward, int64_t n, int64_t codes, int dim, float scale, uint8_t* ws, hipStream_t st) {
     if (backward) return ids64 ? bwd<int64_t, O, T>((const int64_t*)ids, (const O*)a, (T*)b, n, codes, dim, scale, ws, st) : bwd<int32_t, O, T>((const int32_t*)ids, (const O*)a, (T*)b, n, codes, dim, scale, ws, st);
     constexpr int V = vec_of<T, O>();
-    const bool vec = nvp_vec_width(dim, 16 / V, (uintptr_t)a | (uintptr_t)b, V) == V;
+    const bool vec = dim >= V;
     if (ids64) return vec ? fwd<T, O, int64_t, V>((const int64_t*)ids, (const T*)a, (O*)b, n, codes, dim, scale, st) : fwd<T, O, int64_t, 1>((const int64_t*)ids, (const T*)a, (O*)b, n, codes, dim, scale, st);
     return vec ? fwd<T, O, int32_t, V>((const int32_t*)ids, (const T*)a, (O*)b, n, codes, dim, scale, st) : fwd<T, O, int32_t, 1>((const int32_t*)ids, (const T*)a, (O*)b, n, codes, dim, scale, st);
 }

@@ -87,7 +87,7 @@ __device__ __forceinline__ f32x16 mma(const frag<true>& a, const frag<true>& b, 
 
 // ---- x -> workspace: 16 lanes per block of 128, 8 values each -----------------------------------------------------------------------------
 // q [rows][128 * KB], scales [rows][KB4] (bytes); the launch's last workgroups copy the weights' scales to dword-padded rows [NB][KB4].
-template <typename T, bool VEC>
+template <typename T>
 __global__ __launch_bounds__(256) void quant_rows_kernel(const T* __restrict__ x, uint8_t* __restrict__ q, uint8_t* __restrict__ ex, int64_t rows, int64_t k,
                                                          int64_t x_groups, const uint8_t* __restrict__ ew, uint8_t* __restrict__ ew_pad, int64_t ew_bytes) {
     const int64_t kb = kblocks(k), kb_pad = kb4(k);
@@ -104,7 +104,7 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const T* __restrict__ x
     if (g >= rows * kb) return;                                                              // whole 16-lane groups leave together
     const int64_t row = g / kb, b = g - row * kb, c0 = b * 128 + lane16 * 8;
     float v[8];
-    if (VEC && c0 + 8 <= k) {
+    if (c0 + 8 <= k) {
         nvp_load<T, 8>(x + row * k + c0, v);
     } else {
 #pragma unroll
@@ -172,7 +172,7 @@ __global__ __launch_bounds__(256) void dequant_blocks_kernel(const uint8_t* __re
 // operands: which k a register byte stands for cancels in the sum, and each load instruction covers 64 contiguous bytes of a row.
 template <typename T, int MT, int NT, bool FUSED>
 __global__ __launch_bounds__(512) void linear8_rows_kernel(const T* __restrict__ x, const uint8_t* __restrict__ qx, const uint8_t* __restrict__ ex, const uint8_t* __restrict__ qw,
-                                                           const uint8_t* __restrict__ ew, const T* __restrict__ bias, T* __restrict__ y, int64_t rows, int64_t k, int64_t n, int xvec) {
+                                                           const uint8_t* __restrict__ ew, const T* __restrict__ bias, T* __restrict__ y, int64_t rows, int64_t k, int64_t n) {
     constexpr bool kWide = sizeof(T) == 4;
     __shared__ float part[8][MT * 16][NT * 16 + 1];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
@@ -204,7 +204,7 @@ __global__ __launch_bounds__(512) void linear8_rows_kernel(const T* __restrict__
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const int64_t c = b0 * 128 + 64 * h + 16 * g;
-                if (mrow < rows && xvec && c + 16 <= k) {
+                if (mrow < rows && c + 16 <= k) {
 #pragma unroll
                     for (int p = 0; p < 2; ++p) {
                         float t[8];
@@ -405,10 +405,10 @@ int launch_tile(const uint8_t* qx, const uint8_t* ex, const uint8_t* qw, const u
 }
 
 template <typename T, int MT, int NT, bool FUSED>
-int launch_rows(const T* x, const uint8_t* qx, const uint8_t* ex, const uint8_t* qw, const uint8_t* ew, const void* bias, void* y, int64_t rows, int64_t k, int64_t n, int xvec, hipStream_t st) {
+int launch_rows(const T* x, const uint8_t* qx, const uint8_t* ex, const uint8_t* qw, const uint8_t* ew, const void* bias, void* y, int64_t rows, int64_t k, int64_t n, hipStream_t st) {
     const int64_t gx = (n + 16 * NT - 1) / (16 * NT), gy = (rows + 16 * MT - 1) / (16 * MT);
     if (gy > 65535 || gx > 0x7fffffff) return NVP_ERR_UNSUPPORTED;
-    hipLaunchKernelGGL((linear8_rows_kernel<T, MT, NT, FUSED>), dim3((unsigned)gx, (unsigned)gy), dim3(512), 0, st, x, qx, ex, qw, ew, (const T*)bias, (T*)y, rows, k, n, xvec);
+    hipLaunchKernelGGL((linear8_rows_kernel<T, MT, NT, FUSED>), dim3((unsigned)gx, (unsigned)gy), dim3(512), 0, st, x, qx, ex, qw, ew, (const T*)bias, (T*)y, rows, k, n);
     NVP_LAUNCH_CHECK();
     return 0;
 }
@@ -416,19 +416,17 @@ int launch_rows(const T* x, const uint8_t* qx, const uint8_t* ex, const uint8_t*
 template <typename T>
 int linear8(const T* x, const uint8_t* qw, const uint8_t* ew, const void* bias, void* y, int64_t rows, int64_t k, int64_t n, uint8_t* ws, hipStream_t st) {
     const int64_t kb = kblocks(k), kp = kb * 128, kbp = kb4(k), nb = (n + 127) / 128;
-    const bool vec = nvp_vec_width(k, sizeof(T), (uintptr_t)x, 8) == 8;
-    if (rows <= 16) return launch_rows<T, 1, 1, true>(x, nullptr, nullptr, qw, ew, bias, y, rows, k, n, vec ? 1 : 0, st);
+    if (rows <= 16) return launch_rows<T, 1, 1, true>(x, nullptr, nullptr, qw, ew, bias, y, rows, k, n, st);
     uint8_t* qx = ws;
     uint8_t* ex = qx + rows * kp;
     uint8_t* ewp = ex + rows * kbp;                                                          // rows * kbp is a multiple of 4
     const int64_t groups = (rows * kb + 15) / 16, tail = (nb * kbp + 255) / 256;
     if (groups + tail > 0x7fffffff) return NVP_ERR_UNSUPPORTED;
-    if (vec) hipLaunchKernelGGL((quant_rows_kernel<T, true>), dim3((unsigned)(groups + tail)), dim3(256), 0, st, x, qx, ex, rows, k, groups, ew, ewp, nb * kbp);
-    else hipLaunchKernelGGL((quant_rows_kernel<T, false>), dim3((unsigned)(groups + tail)), dim3(256), 0, st, x, qx, ex, rows, k, groups, ew, ewp, nb * kbp);
+    hipLaunchKernelGGL((quant_rows_kernel<T>), dim3((unsigned)(groups + tail)), dim3(256), 0, st, x, qx, ex, rows, k, groups, ew, ewp, nb * kbp);
     NVP_LAUNCH_CHECK();
     const int64_t big = ((rows + 255) / 256) * ((n + 255) / 256);
     if (big >= 128) return launch_tile<T, 256, 256, 2, 4>(qx, ex, qw, ewp, bias, y, rows, k, n, st);
-    if (rows <= 512) return launch_rows<T, 4, 2, false>(x, qx, ex, qw, ewp, bias, y, rows, k, n, 0, st);
+    if (rows <= 512) return launch_rows<T, 4, 2, false>(x, qx, ex, qw, ewp, bias, y, rows, k, n, st);
     return launch_tile<T, 128, 128, 2, 2>(qx, ex, qw, ewp, bias, y, rows, k, n, st);
 }
 

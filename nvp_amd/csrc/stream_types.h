@@ -6,11 +6,17 @@
 typedef _Float16 nvp_f16;
 typedef __bf16 nvp_bf16;
 
-template <typename T, int V> struct alignas(sizeof(T) * V) nvp_vec { T v[V]; };
+template <typename T, int V> struct nvp_vec { T v[V]; };
 
-// V consecutive elements, widened.  `p` must be aligned to V elements.
+// V consecutive elements at any element address.  Global memory takes 16-byte accesses at unaligned addresses (amdhsa runs in unaligned access mode, which the
+// compiler assumes: one global_load_dwordx4 / global_store_dwordx4), so rows of odd widths need no path of their own.
+template <typename T, int V> __device__ __forceinline__ nvp_vec<T, V> nvp_load_raw(const T* __restrict__ p) {
+    nvp_vec<T, V> t;
+    __builtin_memcpy(&t, p, sizeof(t));
+    return t;
+}
 template <typename T, int V> __device__ __forceinline__ void nvp_load(const T* __restrict__ p, float (&f)[V]) {
-    const nvp_vec<T, V> t = *reinterpret_cast<const nvp_vec<T, V>*>(p);
+    const nvp_vec<T, V> t = nvp_load_raw<T, V>(p);
 #pragma unroll
     for (int e = 0; e < V; ++e) f[e] = (float)t.v[e];
 }
@@ -18,14 +24,7 @@ template <typename T, int V> __device__ __forceinline__ void nvp_store(T* __rest
     nvp_vec<T, V> t;
 #pragma unroll
     for (int e = 0; e < V; ++e) t.v[e] = (T)f[e];
-    *reinterpret_cast<nvp_vec<T, V>*>(p) = t;
+    __builtin_memcpy(p, &t, sizeof(t));
 }
 
 __host__ inline int nvp_type_size(int32_t type) { return type == NVP_F32 ? 4 : type == NVP_BF16 || type == NVP_F16 ? 2 : 0; }
-
-// widest vector (in elements, <= limit) that divides d and keeps every pointer of `ored` (OR of the base addresses) aligned
-__host__ inline int nvp_vec_width(int64_t d, int size, uintptr_t ored, int limit) {
-    int v = limit;
-    while (v > 1 && (d % v || ored % ((uintptr_t)v * size))) v >>= 1;
-    return v;
-}

@@ -7,14 +7,12 @@
 // c1 needs E and so c2; written out it is s [sum q (dy + r2 dv) - r2 c2 sum q v] / D with q = a p n: three sums that need neither, so both means come from
 // ONE reduction per row instead of two in sequence.  r1, r2 are kept from forward (8 bytes per row); n, a, y, v are computed again from x, h, g.
 // All arithmetic and every sum is fp32; each result is rounded once to its type.  Bound by memory: 4-5 streams forward, 8-9 backward, each touched once.
-// One row is held in registers by a team of TEAM lanes, 8 values each (16-byte accesses: V = 8 of 16 bits, 4 of 32; V = 1 for widths or addresses that
-// do not allow it).
+// One row is held in registers by a team of TEAM lanes, 8 values each (16 above 4096), in 16-byte accesses: V = 8 of 16 bits, 4 of 32.
 #include "stream_types.h"
 
 namespace {
 
 enum { kBoth = 0, kFirst = 1, kLast = 2 };
-constexpr int kVals = 8;
 
 // sum over a team of `TEAM` consecutive lanes; every lane gets the result, bit-identical in every lane (butterfly; across waves: same order everywhere)
 template <int TEAM, int N> __device__ __forceinline__ void team_sum(float (&s)[N], float* red, int& flip) {
@@ -40,28 +38,56 @@ template <int TEAM, int N> __device__ __forceinline__ void team_sum(float (&s)[N
     }
 }
 
-// column of value j of this lane: vectors of V, team-strided, so that a wave's access is contiguous
-template <int TEAM, int V> __device__ __forceinline__ int col_of(int lane, int j) { return (j / V * TEAM + lane) * V + j % V; }
-
-template <typename T, int TEAM, int V> __device__ __forceinline__ void load_row(const T* __restrict__ p, int lane, int dim, float (&f)[kVals]) {
-#pragma unroll
-    for (int q = 0; q < kVals / V; ++q) {
-        const int c = (q * TEAM + lane) * V;
-        float t[V];
-        if (c < dim) nvp_load<T, V>(p + c, t);
-#pragma unroll
-        for (int e = 0; e < V; ++e) f[q * V + e] = c < dim ? t[e] : 0.f;
-    }
+// number of this thread's team in its workgroup: a scalar wherever a wave belongs to one team, so that row addresses are scalars too
+template <int TEAM, int TEAMS> __device__ __forceinline__ int team_index() {
+    if (TEAMS == 1) return 0;
+    const int t = threadIdx.x / TEAM;
+    return TEAM >= 64 ? __builtin_amdgcn_readfirstlane(t) : t;
 }
-template <typename T, int TEAM, int V> __device__ __forceinline__ void store_row(T* __restrict__ p, int lane, int dim, const float (&f)[kVals]) {
-#pragma unroll
-    for (int q = 0; q < kVals / V; ++q) {
-        const int c = (q * TEAM + lane) * V;
-        float t[V];
-#pragma unroll
-        for (int e = 0; e < V; ++e) t[e] = f[q * V + e];
-        if (c < dim) nvp_store<T, V>(p + c, t);
+
+// A row as a team holds it: vectors of V, team-strided, so that a wave's access is contiguous.  Value j = k * V + e of a lane is column col(k) + e.
+// Where V divides the width (ODD false) a lane behind the last column reads column 0 and holds zeros.  Where it does not (ODD), the vectors that reach behind the
+// end are moved back to end there: some columns are then held twice, with the same values and so the same results (they are stored twice), and only sums
+// across the row have to drop the second copy (keep()).  Loads are unconditional: no branch separates the loads of several rows, and nothing waits for them
+// before they are converted.
+template <typename T, int TEAM, int V, int VALS, bool ODD> struct row_of {
+    nvp_vec<T, V> q[VALS / V];
+    static __device__ __forceinline__ int col(int k, int lane, int dim) {
+        const int c = (k * TEAM + lane) * V;
+        return ODD ? min(c, dim - V) : c < dim ? c : 0;
     }
+    static __device__ __forceinline__ bool inside(int k, int lane, int dim) { return (k * TEAM + lane) * V < dim; }
+    static __device__ __forceinline__ bool keep(int j, int lane, int dim) { return !ODD || col(j / V, lane, dim) + j % V >= (j / V * TEAM + lane) * V; }
+    __device__ __forceinline__ void load(const T* __restrict__ p, int lane, int dim) {
+#pragma unroll
+        for (int k = 0; k < VALS / V; ++k) q[k] = nvp_load_raw<T, V>(p + col(k, lane, dim));
+    }
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int k = 0; k < VALS / V; ++k)
+#pragma unroll
+            for (int e = 0; e < V; ++e) q[k].v[e] = (T)0.f;
+    }
+    __device__ __forceinline__ void get(float (&f)[VALS], int lane, int dim) const {
+#pragma unroll
+        for (int k = 0; k < VALS / V; ++k)
+#pragma unroll
+            for (int e = 0; e < V; ++e) f[k * V + e] = ODD || inside(k, lane, dim) ? (float)q[k].v[e] : 0.f;
+    }
+    static __device__ __forceinline__ void put(T* __restrict__ p, int lane, int dim, const float (&f)[VALS]) {
+#pragma unroll
+        for (int k = 0; k < VALS / V; ++k) {
+            float t[V];
+#pragma unroll
+            for (int e = 0; e < V; ++e) t[e] = f[k * V + e];
+            if (inside(k, lane, dim)) nvp_store<T, V>(p + col(k, lane, dim), t);
+        }
+    }
+};
+template <typename T, int TEAM, int V, int VALS, bool ODD> __device__ __forceinline__ void load_row(const T* __restrict__ p, int lane, int dim, float (&f)[VALS]) {
+    row_of<T, TEAM, V, VALS, ODD> r;
+    r.load(p, lane, dim);
+    r.get(f, lane, dim);
 }
 
 __device__ __forceinline__ float sigmoid(float g) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504f * g)); }
@@ -73,50 +99,78 @@ struct Rows {
     float scale, eps, inv_dim;
 };
 
-template <typename T, typename W, int FORM, int TEAM, int V>
-__global__ __launch_bounds__(TEAM > 256 ? TEAM : 256) void residual_fwd_kernel(const T* __restrict__ x, const T* __restrict__ h, const T* __restrict__ gate, const W* __restrict__ post,
-                                                                               const W* __restrict__ next, T* __restrict__ y, T* __restrict__ u, float* __restrict__ stats, Rows R) {
-    constexpr int kTeams = TEAM > 256 ? 1 : 256 / TEAM;
+constexpr int threads_of(int team) { return team > 256 ? team : 256; }
+
+template <typename T, typename W, int FORM, int TEAM, int V, int VALS, bool ODD>
+__global__ __launch_bounds__(threads_of(TEAM)) void residual_fwd_kernel(const T* __restrict__ x, const T* __restrict__ h, const T* __restrict__ gate, const W* __restrict__ post,
+                                                                        const W* __restrict__ next, T* __restrict__ y, T* __restrict__ u, float* __restrict__ stats, Rows R) {
+    constexpr int kTeams = threads_of(TEAM) / TEAM;
+    typedef row_of<T, TEAM, V, VALS, ODD> Row;
+    constexpr bool kAhead = VALS == 8;                          // registers for a second row?
     __shared__ float red[TEAM > 64 ? 2 * TEAM / 64 : 1];
     int flip = 0;
-    const int lane = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
-    float p[kVals], w[kVals];
-    if (FORM != kFirst) load_row<W, TEAM, V>(post, lane, R.dim, p);
-    if (FORM != kLast) load_row<W, TEAM, V>(next, lane, R.dim, w);
-    for (int64_t row = (int64_t)blockIdx.x * kTeams + team; row < R.rows; row += (int64_t)gridDim.x * kTeams) {
-        float yv[kVals], r1 = 0.f, r2 = 0.f;
-        load_row<T, TEAM, V>(x + row * R.dim, lane, R.dim, yv);
+    const int lane = kTeams == 1 ? threadIdx.x : threadIdx.x % TEAM, team = team_index<TEAM, kTeams>();
+    const int64_t step = (int64_t)gridDim.x * kTeams;
+    int64_t row = (int64_t)blockIdx.x * kTeams + team;
+    if (row >= R.rows) return;                                  // whole teams; a team that spans waves is a workgroup
+    Row rx, rh, rg;                                             // the next row's, one row ahead
+    if (FORM != kFirst) rg.zero();
+    const auto fetch = [&](int64_t r) {
+        rx.load(x + r * R.dim, lane, R.dim);
         if (FORM != kFirst) {
-            float hv[kVals], gv[kVals], s[1] = {0.f};
-            load_row<T, TEAM, V>(h + row * R.dim, lane, R.dim, hv);
-            if (gate) load_row<T, TEAM, V>(gate + (R.share == 1 ? row : (int64_t)((uint32_t)row / (uint32_t)R.share)) * R.dim, lane, R.dim, gv);
+            rh.load(h + r * R.dim, lane, R.dim);
+            if (gate) rg.load(gate + (R.share == 1 ? r : (int64_t)((uint32_t)r / (uint32_t)R.share)) * R.dim, lane, R.dim);
+        }
+    };
+    if (kAhead) fetch(row);
+    float p[VALS], w[VALS];
+    if (FORM != kFirst) load_row<W, TEAM, V, VALS, ODD>(post, lane, R.dim, p);
+    if (FORM != kLast) load_row<W, TEAM, V, VALS, ODD>(next, lane, R.dim, w);
+#pragma unroll 1
+    for (; row < R.rows; row += step) {
+        float yv[VALS], hv[VALS], a[VALS], r1 = 0.f, r2 = 0.f;
+        if (!kAhead) fetch(row);
+        rx.get(yv, lane, R.dim);
+        if (FORM != kFirst) {
+            rh.get(hv, lane, R.dim);
+            rg.get(a, lane, R.dim);
+        }
+        if (kAhead && row + step < R.rows) fetch(row + step);
+        if (FORM != kFirst) {
+            float s[1] = {0.f};
 #pragma unroll
-            for (int j = 0; j < kVals; ++j) s[0] = __fmaf_rn(hv[j], hv[j], s[0]);
+            for (int j = 0; j < VALS; ++j)
+                if (Row::keep(j, lane, R.dim)) s[0] = __fmaf_rn(hv[j], hv[j], s[0]);
             team_sum<TEAM, 1>(s, red, flip);
             r1 = inv_rms(s[0], R.inv_dim, R.eps);
+            if (!gate) {
 #pragma unroll
-            for (int j = 0; j < kVals; ++j) {
-                const float a = gate ? (R.act ? sigmoid(gv[j]) : gv[j]) : 1.f;
-                yv[j] = __fmaf_rn(R.scale * a * p[j], hv[j] * r1, yv[j]);
+                for (int j = 0; j < VALS; ++j) a[j] = 1.f;
+            } else if (R.act) {
+#pragma unroll
+                for (int j = 0; j < VALS; ++j) a[j] = sigmoid(a[j]);
             }
-            store_row<T, TEAM, V>(y + row * R.dim, lane, R.dim, yv);
+#pragma unroll
+            for (int j = 0; j < VALS; ++j) yv[j] = __fmaf_rn(R.scale * a[j] * p[j], hv[j] * r1, yv[j]);
+            Row::put(y + row * R.dim, lane, R.dim, yv);
         }
         if (FORM != kLast) {
             float s[1] = {0.f};
 #pragma unroll
-            for (int j = 0; j < kVals; ++j) s[0] = __fmaf_rn(yv[j], yv[j], s[0]);      // columns behind the last one hold zeros
+            for (int j = 0; j < VALS; ++j)
+                if (Row::keep(j, lane, R.dim)) s[0] = __fmaf_rn(yv[j], yv[j], s[0]);      // columns behind the last one hold zeros
             team_sum<TEAM, 1>(s, red, flip);
             r2 = inv_rms(s[0], R.inv_dim, R.eps);
 #pragma unroll
-            for (int j = 0; j < kVals; ++j) yv[j] = yv[j] * r2 * w[j];
-            store_row<T, TEAM, V>(u + row * R.dim, lane, R.dim, yv);
+            for (int j = 0; j < VALS; ++j) yv[j] = yv[j] * r2 * w[j];
+            Row::put(u + row * R.dim, lane, R.dim, yv);
         }
         if (stats && lane == 0) *reinterpret_cast<float2*>(stats + 2 * row) = make_float2(r1, r2);
     }
 }
 
-// Rows are cut into units of at most `unit` rows that lie within one gate row's share; a team walks whole units, so a shared gate's gradient is summed in
-// registers (a unit that is only a piece of the share leaves a partial sum).  dp and dw are summed over everything the workgroup has seen, the workgroup's
+// Rows are cut into units of at most `unit` rows that lie within one gate row's share; a team walks whole units, so a shared gate's gradient (SUMMED) is added
+// up in registers (a unit that is only a piece of the share leaves a partial sum).  dp and dw are summed over everything the workgroup has seen, the workgroup's
 // teams are added through LDS, and one partial row per workgroup goes to the workspace.  residual_reduce_kernel adds partial rows in a fixed order: no atomics,
 // results do not vary from run to run.
 struct Units {
@@ -124,117 +178,131 @@ struct Units {
     int64_t share, unit;           // rows per such group, rows per unit
 };
 
-template <typename T, typename W, int FORM, int TEAM, int V>
-__global__ __launch_bounds__(TEAM > 256 ? TEAM : 256) void residual_bwd_kernel(const T* __restrict__ x, const T* __restrict__ h, const T* __restrict__ gate, const W* __restrict__ post,
-                                                                               const W* __restrict__ next, const float* __restrict__ stats, const T* __restrict__ dy,
-                                                                               const T* __restrict__ du, T* __restrict__ dx, T* __restrict__ dh, T* __restrict__ dgate,
-                                                                               float* __restrict__ dgate_part, float* __restrict__ dpost_part, float* __restrict__ dnext_part, Rows R,
-                                                                               Units U) {
-    constexpr int kTeams = TEAM > 256 ? 1 : 256 / TEAM, N = FORM == kBoth ? 3 : 1;
+template <typename T, typename W, int FORM, bool SUMMED, int TEAM, int V, int VALS, bool ODD>
+__global__ __launch_bounds__(threads_of(TEAM)) void residual_bwd_kernel(const T* __restrict__ x, const T* __restrict__ h, const T* __restrict__ gate, const W* __restrict__ post,
+                                                                        const W* __restrict__ next, const float* __restrict__ stats, const T* __restrict__ dy, const T* __restrict__ du,
+                                                                        T* __restrict__ dx, T* __restrict__ dh, T* __restrict__ dgate, float* __restrict__ dgate_part,
+                                                                        float* __restrict__ dpost_part, float* __restrict__ dnext_part, Rows R, Units U) {
+    constexpr int kTeams = threads_of(TEAM) / TEAM, N = FORM == kBoth ? 3 : 1;
+    typedef row_of<T, TEAM, V, VALS, ODD> Row;
+    constexpr bool kAhead = VALS == 8;                          // registers for a second row?
     __shared__ float red[TEAM > 64 ? 2 * N * TEAM / 64 : 1];
-    __shared__ float comb[kTeams > 1 ? kTeams : 1][kTeams > 1 ? TEAM * kVals : 1];
+    __shared__ float comb[kTeams > 1 ? kTeams : 1][kTeams > 1 ? TEAM * VALS : 1];
     int flip = 0;
-    const int lane = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
-    const bool summed = gate && R.share > 1;
-    float p[kVals], w[kVals], sp[kVals], sw[kVals], sg[kVals];
+    const int lane = kTeams == 1 ? threadIdx.x : threadIdx.x % TEAM, team = team_index<TEAM, kTeams>();
+    float p[VALS], w[VALS], sp[VALS], sw[VALS];
 #pragma unroll
-    for (int j = 0; j < kVals; ++j) sp[j] = sw[j] = 0.f;
-    if (FORM != kFirst) load_row<W, TEAM, V>(post, lane, R.dim, p);
-    if (FORM != kLast) load_row<W, TEAM, V>(next, lane, R.dim, w);
+    for (int j = 0; j < VALS; ++j) sp[j] = sw[j] = 0.f;
+    if (FORM != kFirst) load_row<W, TEAM, V, VALS, ODD>(post, lane, R.dim, p);
+    if (FORM != kLast) load_row<W, TEAM, V, VALS, ODD>(next, lane, R.dim, w);
+    Row rx, rh, rg, re, rd;                                     // the next row's, one row ahead
+    float2 rst;
+    rg.zero();
+    re.zero();
+    rd.zero();
+    const auto fetch = [&](int64_t r) {
+        rst = *reinterpret_cast<const float2*>(stats + 2 * r);
+        if (FORM != kLast) rx.load(x + r * R.dim, lane, R.dim);
+        if (FORM != kFirst) rh.load(h + r * R.dim, lane, R.dim);
+        if (FORM != kFirst && !SUMMED && gate) rg.load(gate + r * R.dim, lane, R.dim);
+        if (FORM != kFirst && dy) re.load(dy + r * R.dim, lane, R.dim);
+        if (FORM != kLast && du) rd.load(du + r * R.dim, lane, R.dim);
+    };
+#pragma unroll 1
     for (int64_t un = (int64_t)blockIdx.x * kTeams + team; un < U.units; un += (int64_t)gridDim.x * kTeams) {
         const int64_t grp = un / U.per_share, piece = un - grp * U.per_share;
         const int64_t first = grp * U.share + piece * U.unit, last = min(first + U.unit, (grp + 1) * U.share);
-        float a[kVals], da[kVals];                       // act(g) and its derivative
+        float a[VALS], da[VALS], sg[VALS];                      // act(g), its derivative, the sum of the gate's gradient
+        if (kAhead) fetch(first);
+        if (SUMMED) {
+            load_row<T, TEAM, V, VALS, ODD>(gate + grp * R.dim, lane, R.dim, a);
 #pragma unroll
-        for (int j = 0; j < kVals; ++j) {
-            a[j] = 1.f;
-            da[j] = sg[j] = 0.f;
+            for (int j = 0; j < VALS; ++j) {
+                a[j] = R.act ? sigmoid(a[j]) : a[j];
+                da[j] = R.act ? a[j] * (1.f - a[j]) : 1.f;
+                sg[j] = 0.f;
+            }
         }
+#pragma unroll 1
         for (int64_t row = first; row < last; ++row) {
-            float xv[kVals], n[kVals], e[kVals], dv[kVals];
-            const float2 st = *reinterpret_cast<const float2*>(stats + 2 * row);
-            if (FORM != kLast) load_row<T, TEAM, V>(x + row * R.dim, lane, R.dim, xv);
-            if (FORM != kFirst) load_row<T, TEAM, V>(h + row * R.dim, lane, R.dim, n);
-            if (FORM != kFirst && gate && (!summed || row == first)) {
-                load_row<T, TEAM, V>(gate + (summed ? grp : row) * R.dim, lane, R.dim, a);
+            float xv[VALS], n[VALS], e[VALS], dv[VALS];
+            if (!kAhead) fetch(row);
+            const float2 st = rst;
+            if (FORM != kLast) rx.get(xv, lane, R.dim);
+            if (FORM != kFirst) rh.get(n, lane, R.dim);
+            if (FORM != kFirst && !SUMMED) rg.get(a, lane, R.dim);
+            re.get(e, lane, R.dim);
+            rd.get(dv, lane, R.dim);
+            if (kAhead && row + 1 < last) fetch(row + 1);
+            if (FORM != kFirst && !SUMMED) {
+                if (!gate) {
 #pragma unroll
-                for (int j = 0; j < kVals; ++j) {
-                    da[j] = 1.f;
-                    if (R.act) {
-                        a[j] = sigmoid(a[j]);
-                        da[j] = a[j] * (1.f - a[j]);
-                    }
+                    for (int j = 0; j < VALS; ++j) a[j] = 1.f;
+                } else if (R.act) {
+#pragma unroll
+                    for (int j = 0; j < VALS; ++j) a[j] = sigmoid(a[j]);
                 }
-            }
-            if (FORM != kFirst && dy) {
-                load_row<T, TEAM, V>(dy + row * R.dim, lane, R.dim, e);
-            } else {
-#pragma unroll
-                for (int j = 0; j < kVals; ++j) e[j] = 0.f;
-            }
-            if (FORM != kLast && du) {
-                load_row<T, TEAM, V>(du + row * R.dim, lane, R.dim, dv);
-            } else {
-#pragma unroll
-                for (int j = 0; j < kVals; ++j) dv[j] = 0.f;
             }
             float s[N];
 #pragma unroll
             for (int k = 0; k < N; ++k) s[k] = 0.f;
 #pragma unroll
-            for (int j = 0; j < kVals; ++j) {
+            for (int j = 0; j < VALS; ++j) {
                 float q = 0.f;
                 if (FORM != kFirst) {
                     n[j] *= st.x;
                     q = a[j] * p[j] * n[j];
                 }
+                const bool keep = Row::keep(j, lane, R.dim);
                 if (FORM == kLast) {
-                    s[0] = __fmaf_rn(q, e[j], s[0]);
+                    if (keep) s[0] = __fmaf_rn(q, e[j], s[0]);
                 } else {
                     const float v = (FORM == kBoth ? __fmaf_rn(R.scale, q, xv[j]) : xv[j]) * st.y;
                     xv[j] = v;
                     sw[j] = __fmaf_rn(dv[j], v, sw[j]);
                     dv[j] *= w[j];
-                    s[0] = __fmaf_rn(dv[j], v, s[0]);
+                    if (keep) s[0] = __fmaf_rn(dv[j], v, s[0]);
                     e[j] = __fmaf_rn(st.y, dv[j], e[j]);
                     if constexpr (FORM == kBoth) {
-                        s[N - 2] = __fmaf_rn(q, e[j], s[N - 2]);
-                        s[N - 1] = __fmaf_rn(q, v, s[N - 1]);
+                        if (keep) {
+                            s[N - 2] = __fmaf_rn(q, e[j], s[N - 2]);
+                            s[N - 1] = __fmaf_rn(q, v, s[N - 1]);
+                        }
                     }
                 }
             }
             team_sum<TEAM, N>(s, red, flip);
-            float c1 = 0.f;                                // mean(dn n)
+            float c1 = 0.f;                                     // mean(dn n)
             if (FORM != kLast) {
                 const float c2 = st.y * s[0] * R.inv_dim;
 #pragma unroll
-                for (int j = 0; j < kVals; ++j) e[j] = __fmaf_rn(-c2, xv[j], e[j]);
+                for (int j = 0; j < VALS; ++j) e[j] = __fmaf_rn(-c2, xv[j], e[j]);
                 if constexpr (FORM == kBoth) c1 = R.scale * R.inv_dim * (s[N - 2] - c2 * s[N - 1]);
             } else {
                 c1 = R.scale * R.inv_dim * s[0];
             }
-            if (dx) store_row<T, TEAM, V>(dx + row * R.dim, lane, R.dim, e);
+            if (dx) Row::put(dx + row * R.dim, lane, R.dim, e);
             if (FORM != kFirst) {
-                float t[kVals];
+                float t[VALS];
 #pragma unroll
-                for (int j = 0; j < kVals; ++j) {
+                for (int j = 0; j < VALS; ++j) {
                     const float en = R.scale * e[j] * n[j];
                     sp[j] = __fmaf_rn(a[j], en, sp[j]);
-                    t[j] = en * p[j] * da[j];
+                    t[j] = en * p[j] * (SUMMED ? da[j] : R.act ? a[j] * (1.f - a[j]) : 1.f);
                     n[j] = st.x * __fmaf_rn(-c1, n[j], R.scale * a[j] * p[j] * e[j]);
                 }
-                if (dh) store_row<T, TEAM, V>(dh + row * R.dim, lane, R.dim, n);
-                if (summed) {
+                if (dh) Row::put(dh + row * R.dim, lane, R.dim, n);
+                if (SUMMED) {
 #pragma unroll
-                    for (int j = 0; j < kVals; ++j) sg[j] += t[j];
+                    for (int j = 0; j < VALS; ++j) sg[j] += t[j];
                 } else if (dgate) {
-                    store_row<T, TEAM, V>(dgate + row * R.dim, lane, R.dim, t);
+                    Row::put(dgate + row * R.dim, lane, R.dim, t);
                 }
             }
         }
-        if (FORM != kFirst && summed && dgate) {
-            if (U.per_share == 1) store_row<T, TEAM, V>(dgate + grp * R.dim, lane, R.dim, sg);
-            else store_row<float, TEAM, V>(dgate_part + un * R.dim, lane, R.dim, sg);
+        if (SUMMED && dgate) {
+            if (U.per_share == 1) Row::put(dgate + grp * R.dim, lane, R.dim, sg);
+            else row_of<float, TEAM, V, VALS, ODD>::put(dgate_part + un * R.dim, lane, R.dim, sg);
         }
     }
     // one partial row per workgroup for each weight
@@ -245,7 +313,8 @@ __global__ __launch_bounds__(TEAM > 256 ? TEAM : 256) void residual_bwd_kernel(c
         if (kTeams > 1) {
             __syncthreads();
 #pragma unroll
-            for (int j = 0; j < kVals; ++j) comb[team][col_of<TEAM, V>(lane, j)] = which ? sw[j] : sp[j];
+            for (int j = 0; j < VALS; ++j)
+                if (Row::inside(j / V, lane, R.dim)) comb[team][Row::col(j / V, lane, R.dim) + j % V] = which ? sw[j] : sp[j];
             __syncthreads();
             for (int c = threadIdx.x; c < R.dim; c += 256) {
                 float t = 0.f;
@@ -254,7 +323,7 @@ __global__ __launch_bounds__(TEAM > 256 ? TEAM : 256) void residual_bwd_kernel(c
                 out[(int64_t)blockIdx.x * R.dim + c] = t;
             }
         } else {
-            store_row<float, TEAM, V>(out + (int64_t)blockIdx.x * R.dim, lane, R.dim, which ? sw : sp);
+            row_of<float, TEAM, V, VALS, ODD>::put(out + (int64_t)blockIdx.x * R.dim, lane, R.dim, which ? sw : sp);
         }
     }
 }
@@ -271,8 +340,17 @@ __global__ __launch_bounds__(1024) void residual_reduce_kernel(const float* __re
     if ((job == 0 && !dpost) || (job == 1 && !dnext)) return;                  // uniform over the workgroup
     const int64_t rows = job < 2 ? groups : pieces;
     float s = 0.f;
-    if (c < dim)
-        for (int64_t r = r0; r < rows; r += 32) s += src[r * dim + c];
+    if (c < dim) {
+        int64_t r = r0;
+        for (; r + 7 * 32 < rows; r += 8 * 32) {                               // eight loads in flight, added in order
+            float t[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) t[k] = src[(r + k * 32) * dim + c];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) s += t[k];
+        }
+        for (; r < rows; r += 32) s += src[r * dim + c];
+    }
     part[r0][threadIdx.x & 31] = s;
     __syncthreads();
     if (r0 == 0 && c < dim) {
@@ -286,7 +364,7 @@ __global__ __launch_bounds__(1024) void residual_reduce_kernel(const float* __re
 }
 
 constexpr int kMaxDim = 8192;
-int team_of(int dim) { return dim <= 128 ? 16 : dim <= 512 ? 64 : dim <= 2048 ? 256 : dim <= 4096 ? 512 : 1024; }
+int team_of(int dim) { return dim <= 128 ? 16 : dim <= 512 ? 64 : dim <= 2048 ? 256 : 512; }      // 8 values per lane; 16 above 4096
 
 struct Plan {
     Units U;
@@ -300,15 +378,16 @@ Plan plan_of(const nvp_residual* a) {
     const bool shared = a->gate && a->gate_rows < a->rows;
     P.gate_rows = shared ? a->gate_rows : 0;
     P.U.share = shared ? a->rows / a->gate_rows : a->rows;
-    // enough workgroups to fill the chip (256 CUs, 1024 lanes of work each), few enough that their partial rows stay a small part of the traffic
-    const int64_t want = (int64_t)(team >= 512 ? 512 : 1024) * teams;
+    // as many workgroups as the chip holds at once (2 of 256 threads per CU at the kernel's registers, 1 of 512): more would leave a second, partly filled
+    // round and more partial rows to add up
+    const int64_t want = (int64_t)(team >= 512 ? 256 : 512) * teams;
     const int64_t rows_per = (a->rows + want - 1) / want;
     P.U.unit = rows_per < P.U.share ? rows_per : P.U.share;
     P.U.per_share = (P.U.share + P.U.unit - 1) / P.U.unit;
     P.U.units = (shared ? a->gate_rows : 1) * P.U.per_share;
     P.parts = shared && P.U.per_share > 1;
     const int64_t g = (P.U.units + teams - 1) / teams;
-    P.groups = g < 1024 ? g : 1024;
+    P.groups = g < 512 ? g : 512;
     return P;
 }
 
@@ -333,20 +412,27 @@ struct Call {
     hipStream_t st;
 };
 
-template <typename T, typename W, int FORM, int TEAM, int V> int launch(const Call& c) {
+template <typename T, typename W, int FORM, int TEAM, int V, int VALS, bool ODD> int launch(const Call& c) {
     const nvp_residual* a = c.a;
-    constexpr int kTeams = TEAM > 256 ? 1 : 256 / TEAM, kThreads = TEAM > 256 ? TEAM : 256;
+    constexpr int kThreads = threads_of(TEAM), kTeams = kThreads / TEAM;
     const Rows R{a->rows, a->gate ? a->rows / a->gate_rows : 1, a->dim, a->gate_act, a->scale, a->eps, 1.f / (float)a->dim};
     if (!c.backward) {
         const int64_t need = (a->rows + kTeams - 1) / kTeams, cap = 256 * (2048 / kThreads);
-        hipLaunchKernelGGL((residual_fwd_kernel<T, W, FORM, TEAM, V>), dim3((unsigned)(need < cap ? need : cap)), dim3(kThreads), 0, c.st, (const T*)a->x, (const T*)a->h, (const T*)a->gate,
-                           (const W*)a->post, (const W*)a->next, (T*)c.y, (T*)c.u, c.stats, R);
+        hipLaunchKernelGGL((residual_fwd_kernel<T, W, FORM, TEAM, V, VALS, ODD>), dim3((unsigned)(need < cap ? need : cap)), dim3(kThreads), 0, c.st, (const T*)a->x, (const T*)a->h,
+                           (const T*)a->gate, (const W*)a->post, (const W*)a->next, (T*)c.y, (T*)c.u, c.stats, R);
         NVP_LAUNCH_CHECK();
         return 0;
     }
-    hipLaunchKernelGGL((residual_bwd_kernel<T, W, FORM, TEAM, V>), dim3((unsigned)c.P.groups), dim3(kThreads), 0, c.st, (const T*)a->x, (const T*)a->h, (const T*)a->gate, (const W*)a->post,
-                       (const W*)a->next, c.stats, (const T*)c.dy, (const T*)c.du, (T*)c.dx, (T*)c.dh, (T*)c.dgate, c.dgate_part, c.dpost ? c.dpost_part : nullptr,
-                       c.dnext ? c.dnext_part : nullptr, R, c.P.U);
+    const auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)c.P.groups), dim3(kThreads), 0, c.st, (const T*)a->x, (const T*)a->h, (const T*)a->gate, (const W*)a->post, (const W*)a->next, c.stats,
+                           (const T*)c.dy, (const T*)c.du, (T*)c.dx, (T*)c.dh, (T*)c.dgate, c.dgate_part, c.dpost ? c.dpost_part : nullptr, c.dnext ? c.dnext_part : nullptr, R, c.P.U);
+    };
+    if constexpr (FORM != kFirst) {
+        if (R.share > 1) go(residual_bwd_kernel<T, W, FORM, true, TEAM, V, VALS, ODD>);
+        else go(residual_bwd_kernel<T, W, FORM, false, TEAM, V, VALS, ODD>);
+    } else {
+        go(residual_bwd_kernel<T, W, FORM, false, TEAM, V, VALS, ODD>);
+    }
     NVP_LAUNCH_CHECK();
     const bool gsum = c.P.parts && c.dgate;
     if (c.dpost || c.dnext || gsum) {
@@ -357,25 +443,23 @@ template <typename T, typename W, int FORM, int TEAM, int V> int launch(const Ca
     return 0;
 }
 
-template <typename T, typename W, int FORM, int V> int by_team(const Call& c) {
+template <typename T, typename W, int FORM, bool ODD> int by_team(const Call& c) {
+    constexpr int V = 16 / sizeof(T);
     switch (team_of(c.a->dim)) {
-        case 16: return launch<T, W, FORM, 16, V>(c);
-        case 64: return launch<T, W, FORM, 64, V>(c);
-        case 256: return launch<T, W, FORM, 256, V>(c);
-        case 512: return launch<T, W, FORM, 512, V>(c);
-        default: return launch<T, W, FORM, 1024, V>(c);
+        case 16: return launch<T, W, FORM, 16, V, 8, ODD>(c);
+        case 64: return launch<T, W, FORM, 64, V, 8, ODD>(c);
+        case 256: return launch<T, W, FORM, 256, V, 8, ODD>(c);
+        default: return c.a->dim <= 4096 ? launch<T, W, FORM, 512, V, 8, ODD>(c) : launch<T, W, FORM, 512, V, 16, ODD>(c);
     }
 }
-template <typename T, typename W> int by_form(const Call& c) {
+template <typename T, typename W, int FORM> int by_width(const Call& c) {
     constexpr int V = 16 / sizeof(T);
-    const nvp_residual* a = c.a;
-    uintptr_t all = 0;
-    for (const void* p : {a->x, a->h, a->gate, c.dy, c.du, (const void*)c.y, (const void*)c.u, (const void*)c.dx, (const void*)c.dh, (const void*)c.dgate}) all |= (uintptr_t)p;
-    const uintptr_t weights = (uintptr_t)a->post | (uintptr_t)a->next;
-    const bool vec = nvp_vec_width(a->dim, sizeof(T), all, V) == V && nvp_vec_width(a->dim, sizeof(W), weights, V) == V;      // W rows: 16 or 32 bytes
-    if (!a->h) return vec ? by_team<T, W, kFirst, V>(c) : by_team<T, W, kFirst, 1>(c);
-    if (!a->next) return vec ? by_team<T, W, kLast, V>(c) : by_team<T, W, kLast, 1>(c);
-    return vec ? by_team<T, W, kBoth, V>(c) : by_team<T, W, kBoth, 1>(c);
+    if (c.a->dim < V) return launch<T, W, FORM, 16, 1, 8, false>(c);
+    return c.a->dim % V ? by_team<T, W, FORM, true>(c) : by_team<T, W, FORM, false>(c);
+}
+template <typename T, typename W> int by_form(const Call& c) {
+    if (!c.a->h) return by_width<T, W, kFirst>(c);
+    return c.a->next ? by_width<T, W, kBoth>(c) : by_width<T, W, kLast>(c);
 }
 int by_type(const Call& c) {
     const bool wide = c.a->weight_type == NVP_F32;
