@@ -8,13 +8,14 @@
 // list of at most two entries per chunk, which is a sorted list again and goes through the same kernel.  Work per team is P rows however
 // the ids are distributed (one id 10^6 times: three more small levels), the order of every sum is fixed, and the result is the same in every run.
 // Sorting: up to 4096 ids in one workgroup (bitonic, on (id, position) pairs, which are distinct); more: stable radix passes of up to 10 bits.
+#include <type_traits>
 #include "stream_types.h"
 
 namespace {
 
 constexpr unsigned kEmpty = 0xffffffffu, kCarry = 0x80000000u;      // list keys: no entry; the run goes on here, but this entry has no row
 constexpr int kSmall = 4096;                                        // ids sorted in one workgroup
-constexpr int kChunk = 16384, kWaves = 16, kPerWave = kChunk / kWaves;
+constexpr int kChunk = 2048, kWaves = 4, kPerWave = kChunk / kWaves; // ids per workgroup of a radix pass
 constexpr int kMaxBits = 10;
 
 // sort key of an id: the id itself, `codes` (behind every table row) for ids that point nowhere
@@ -51,7 +52,7 @@ __global__ __launch_bounds__(256) void lookup_fwd_kernel(const I* __restrict__ i
 
 // ---- sorting -------------------------------------------------------------------------------------------------------------------------------
 template <typename I>
-__global__ __launch_bounds__(1024) void sort_small_kernel(const I* __restrict__ ids, unsigned* __restrict__ keys, unsigned* __restrict__ order, int n, int64_t codes, int padded) {
+__global__ __launch_bounds__(1024) void sort_small_kernel(const I* __restrict__ ids, uint2* __restrict__ sorted, int n, int64_t codes, int padded) {
     __shared__ unsigned long long s[kSmall];
     for (int i = threadIdx.x; i < padded; i += 1024) s[i] = i < n ? (unsigned long long)key_of(ids, i, codes) << 32 | (unsigned)i : ~0ull;
     for (int size = 2; size <= padded; size <<= 1)
@@ -67,80 +68,147 @@ __global__ __launch_bounds__(1024) void sort_small_kernel(const I* __restrict__ 
             }
         }
     __syncthreads();
-    for (int i = threadIdx.x; i < n; i += 1024) {
-        keys[i] = (unsigned)(s[i] >> 32);
-        order[i] = (unsigned)s[i];
-    }
+    for (int i = threadIdx.x; i < n; i += 1024) sorted[i] = make_uint2((unsigned)(s[i] >> 32), (unsigned)s[i]);
 }
 
-// one radix pass in three launches: counts per (chunk, digit); exclusive prefix in (digit, chunk) order, by one workgroup; stable scatter
+// One radix pass in three launches: counts per (chunk, digit); per digit, the number of its ids in earlier chunks, and its total; stable scatter, where every
+// workgroup adds up the totals of the smaller digits by itself.
 template <typename I, bool FIRST>
-__global__ __launch_bounds__(1024) void radix_count_kernel(const I* __restrict__ ids, const unsigned* __restrict__ keys, unsigned* __restrict__ count, int64_t n, int64_t codes, int shift, int bits) {
+__global__ __launch_bounds__(256) void radix_count_kernel(const I* __restrict__ ids, const uint2* __restrict__ in, unsigned* __restrict__ count, int64_t n, int64_t codes, int shift, int bits) {
     __shared__ unsigned bin[1 << kMaxBits];
     const int bins = 1 << bits;
-    for (int b = threadIdx.x; b < bins; b += 1024) bin[b] = 0u;
+    const int64_t base = (int64_t)blockIdx.x * kChunk + threadIdx.x;
+    unsigned k[kChunk / 256];
+#pragma unroll
+    for (int j = 0; j < kChunk / 256; ++j) k[j] = base + j * 256 < n ? (FIRST ? key_of(ids, base + j * 256, codes) : in[base + j * 256].x) : 0u;
+    for (int b = threadIdx.x; b < bins; b += 256) bin[b] = 0u;
     __syncthreads();
-    const int64_t base = (int64_t)blockIdx.x * kChunk;
-    for (int j = 0; j < kChunk / 1024; ++j) {
-        const int64_t i = base + j * 1024 + threadIdx.x;
-        if (i < n) atomicAdd(&bin[((FIRST ? key_of(ids, i, codes) : keys[i]) >> shift) & (bins - 1)], 1u);
-    }
+#pragma unroll
+    for (int j = 0; j < kChunk / 256; ++j)
+        if (base + j * 256 < n) atomicAdd(&bin[(k[j] >> shift) & (bins - 1)], 1u);
     __syncthreads();
-    for (int b = threadIdx.x; b < bins; b += 1024) count[(int64_t)blockIdx.x * bins + b] = bin[b];
+    for (int b = threadIdx.x; b < bins; b += 256) count[(int64_t)blockIdx.x * bins + b] = bin[b];
 }
 
-__global__ __launch_bounds__(1024) void radix_scan_kernel(unsigned* __restrict__ count, int chunks, int bits) {
-    __shared__ unsigned wsum[16];
-    const int bins = 1 << bits, b = threadIdx.x;
+// count [chunk][digit] -> exclusive prefix over the chunks, total [digit].  A workgroup: 64 digits (lanes) x 16 spans of chunks (waves).
+__global__ __launch_bounds__(1024) void radix_scan_kernel(unsigned* __restrict__ count, unsigned* __restrict__ total, int chunks, int bits) {
+    __shared__ unsigned span[16][64];
+    const int bins = 1 << bits, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, b = blockIdx.x * 64 + lane;
+    const int per = (chunks + 15) / 16, c0 = wave * per, c1 = min(c0 + per, chunks);
     unsigned sum = 0u;
-    if (b < bins)
-        for (int c = 0; c < chunks; ++c) sum += count[(int64_t)c * bins + b];
-    unsigned inc = sum;                                              // inclusive prefix over the digits: within the wave, then over the waves
+    if (b < bins) {
+        int c = c0;
+        for (; c + 8 <= c1; c += 8) {
+            unsigned t[8];
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const unsigned up = __shfl_up(inc, o);
-        if ((threadIdx.x & 63) >= o) inc += up;
-    }
-    if ((threadIdx.x & 63) == 63) wsum[threadIdx.x >> 6] = inc;
-    __syncthreads();
-    unsigned run = inc - sum;
-    for (int w = 0; w < (int)(threadIdx.x >> 6); ++w) run += wsum[w];
-    if (b < bins)
-        for (int c = 0; c < chunks; ++c) {
-            const unsigned v = count[(int64_t)c * bins + b];
-            count[(int64_t)c * bins + b] = run;
-            run += v;
+            for (int k = 0; k < 8; ++k) t[k] = count[(int64_t)(c + k) * bins + b];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) sum += t[k];
         }
+        for (; c < c1; ++c) sum += count[(int64_t)c * bins + b];
+    }
+    span[wave][lane] = sum;
+    __syncthreads();
+    unsigned run = 0u;
+    for (int w = 0; w < wave; ++w) run += span[w][lane];
+    if (b >= bins) return;
+    if (wave == 15) total[b] = run + sum;
+    int c = c0;
+    for (; c + 8 <= c1; c += 8) {
+        unsigned t[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) t[k] = count[(int64_t)(c + k) * bins + b];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            count[(int64_t)(c + k) * bins + b] = run;
+            run += t[k];
+        }
+    }
+    for (; c < c1; ++c) {
+        const unsigned v = count[(int64_t)c * bins + b];
+        count[(int64_t)c * bins + b] = run;
+        run += v;
+    }
 }
 
 template <typename I, bool FIRST>
-__global__ __launch_bounds__(1024) void radix_scatter_kernel(const I* __restrict__ ids, const unsigned* __restrict__ keys, const unsigned* __restrict__ pos, const unsigned* __restrict__ count,
-                                                             unsigned* __restrict__ keys_out, unsigned* __restrict__ pos_out, int64_t n, int64_t codes, int shift, int bits) {
-    extern __shared__ unsigned cursor[];                             // [16 waves][bins]
+__global__ __launch_bounds__(256) void radix_scatter_kernel(const I* __restrict__ ids, const uint2* __restrict__ in, const unsigned* __restrict__ count,
+                                                            const unsigned* __restrict__ total, uint2* __restrict__ sorted, int64_t n, int64_t codes, int shift, int bits) {
+    __shared__ unsigned cursor[kWaves][1 << kMaxBits];                           // where the wave's next id of a digit goes in `list`
+    __shared__ unsigned shift_to[1 << kMaxBits];                                 // place in the output - place in `list`, per digit
+    __shared__ uint2 list[kChunk];
+    __shared__ unsigned wsum[2][kWaves];
     const int bins = 1 << bits, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int b = threadIdx.x; b < kWaves * bins; b += 1024) cursor[b] = 0u;
-    __syncthreads();
     const int64_t base = (int64_t)blockIdx.x * kChunk + (int64_t)wave * kPerWave;      // a wave's ids are consecutive: waves in order, rounds in order, lanes in order
-    unsigned k[kPerWave / 64];
+    constexpr int kRounds = kPerWave / 64, kPer = (1 << kMaxBits) / 256;
+    unsigned k[kRounds], p[kRounds];
 #pragma unroll
-    for (int j = 0; j < kPerWave / 64; ++j) {
+    for (int j = 0; j < kRounds; ++j) {
         const int64_t i = base + j * 64 + lane;
-        k[j] = i < n ? (FIRST ? key_of(ids, i, codes) : keys[i]) : 0u;
-        if (i < n) atomicAdd(&cursor[wave * bins + ((k[j] >> shift) & (bins - 1))], 1u);
+        if (FIRST) {
+            k[j] = i < n ? key_of(ids, i, codes) : 0u;
+            p[j] = (unsigned)i;
+        } else {
+            const uint2 t = i < n ? in[i] : make_uint2(0u, 0u);
+            k[j] = t.x;
+            p[j] = t.y;
+        }
+    }
+    for (int b = threadIdx.x; b < kWaves << kMaxBits; b += 256) (&cursor[0][0])[b] = 0u;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kRounds; ++j)
+        if (base + j * 64 + lane < n) atomicAdd(&cursor[wave][(k[j] >> shift) & (bins - 1)], 1u);
+    __syncthreads();
+    // a thread's digits: where they start in the output (the totals of all smaller digits + the chunk's place among the chunks) and in this chunk
+    unsigned all[kPer], mine[kPer], sum[2] = {0u, 0u};
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+        const int b = threadIdx.x * kPer + e;
+        all[e] = b < bins ? total[b] : 0u;
+        mine[e] = 0u;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) mine[e] += cursor[w][b];
+        sum[0] += all[e];
+        sum[1] += mine[e];
+    }
+    unsigned inc[2] = {sum[0], sum[1]};
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            const unsigned up = __shfl_up(inc[q], o);
+            if (lane >= o) inc[q] += up;
+        }
+    if (lane == 63) {
+        wsum[0][wave] = inc[0];
+        wsum[1][wave] = inc[1];
     }
     __syncthreads();
-    for (int b = threadIdx.x; b < bins; b += 1024) {
-        unsigned run = count[(int64_t)blockIdx.x * bins + b];
+    unsigned out = inc[0] - sum[0], here = inc[1] - sum[1];
+    for (int w = 0; w < wave; ++w) {
+        out += wsum[0][w];
+        here += wsum[1][w];
+    }
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+        const int b = threadIdx.x * kPer + e;
+        if (b >= bins) break;
+        shift_to[b] = out + count[(int64_t)blockIdx.x * bins + b] - here;
+        unsigned run = here;
+#pragma unroll
         for (int w = 0; w < kWaves; ++w) {
-            const unsigned v = cursor[w * bins + b];
-            cursor[w * bins + b] = run;
+            const unsigned v = cursor[w][b];
+            cursor[w][b] = run;
             run += v;
         }
+        out += all[e];
+        here += mine[e];
     }
     __syncthreads();
     const unsigned long long below = lane == 0 ? 0ull : ~0ull >> (64 - lane);
 #pragma unroll
-    for (int j = 0; j < kPerWave / 64; ++j) {
+    for (int j = 0; j < kRounds; ++j) {
         const int64_t i = base + j * 64 + lane;
         const unsigned d = (k[j] >> shift) & (bins - 1);
         unsigned long long same = __ballot(i < n);
@@ -149,24 +217,31 @@ __global__ __launch_bounds__(1024) void radix_scatter_kernel(const I* __restrict
             same &= ((d >> b) & 1u) ? m : ~m;
         }
         if (i < n) {
-            const unsigned at = cursor[wave * bins + d] + (unsigned)__popcll(same & below);
-            keys_out[at] = k[j];
-            pos_out[at] = FIRST ? (unsigned)i : pos[i];
-            if ((same >> lane) == 1ull) cursor[wave * bins + d] = at + 1u;       // the last of the equals moves the cursor; every lane has read it (one wave, in order)
+            const unsigned at = cursor[wave][d] + (unsigned)__popcll(same & below);
+            list[at] = make_uint2(k[j], p[j]);
+            if ((same >> lane) == 1ull) cursor[wave][d] = at + 1u;               // the last of the equals moves the cursor; every lane has read it (one wave, in order)
         }
         __builtin_amdgcn_wave_barrier();
+    }
+    __syncthreads();
+    // equal digits lie side by side now: their places in the output do too, and neighbouring lanes write them together
+    const int len = (int)min((int64_t)kChunk, n - (int64_t)blockIdx.x * kChunk);
+    for (int t = threadIdx.x; t < len; t += 256) {
+        const uint2 v = list[t];
+        sorted[t + shift_to[(v.x >> shift) & (bins - 1)]] = v;
     }
 }
 
 // ---- sums over the sorted list ----------------------------------------------------------------------------------------------------------------
-// Entry i of a list: keys[i] (kEmpty: none; | kCarry: no row) and a row of D values: dout row order[i] (first level) or partial row i.
+// Entry i of a list: a key (kEmpty: none; | kCarry: no row) and a row of D values.  First level: sorted (id, position) pairs, the row is dout row `position`;
+// later: keys[i], partial row i.
 // blocks < sum_blocks: a team of TEAM lanes adds P entries over TEAM * V columns (blockIdx.y: which columns).  The other blocks (first level only): zeros into
 // the table rows no id points to, 64 rows per wave: every lane looks its row up in the sorted keys (binary search), the wave then writes the empty ones.
-template <typename S, typename T, bool FIRST, int TEAM, int V, int BATCH>
-__global__ __launch_bounds__(256) void sum_runs_kernel(const unsigned* __restrict__ keys, const unsigned* __restrict__ order, const S* __restrict__ rows, T* __restrict__ dtable,
+template <typename S, typename T, bool FIRST, int TEAM, int V>
+__global__ __launch_bounds__(256) void sum_runs_kernel(const uint2* __restrict__ sorted, const unsigned* __restrict__ keys, const S* __restrict__ rows, T* __restrict__ dtable,
                                                        unsigned* __restrict__ next_keys, float* __restrict__ next_rows, int64_t m, int per_chunk, int64_t chunks, int64_t sum_blocks, int64_t codes,
                                                        int dim, float scale) {
-    constexpr int kTeams = 256 / TEAM;
+    constexpr int kTeams = 256 / TEAM, kBatch = V > 4 ? 8 : 16;      // rows in flight per team: 64 registers
     if (FIRST && (int64_t)blockIdx.x >= sum_blocks) {
         const int lane = threadIdx.x & 63;
         const int64_t r0 = (((int64_t)blockIdx.x - sum_blocks) * 4 + (threadIdx.x >> 6)) * 64;
@@ -176,10 +251,10 @@ __global__ __launch_bounds__(256) void sum_runs_kernel(const unsigned* __restric
             int64_t lo = 0, hi = m;
             while (lo < hi) {
                 const int64_t mid = (lo + hi) >> 1;
-                if (keys[mid] < (unsigned)row) lo = mid + 1;
+                if (sorted[mid].x < (unsigned)row) lo = mid + 1;
                 else hi = mid;
             }
-            empty = lo >= m || keys[lo] != (unsigned)row;
+            empty = lo >= m || sorted[lo].x != (unsigned)row;
         }
         unsigned long long todo = __ballot(empty);
         const float zero[V] = {};
@@ -196,8 +271,24 @@ __global__ __launch_bounds__(256) void sum_runs_kernel(const unsigned* __restric
     if (ch >= chunks) return;
     const bool live = (blockIdx.y * TEAM + lane) * V < dim;
     const int c = min((int)(blockIdx.y * TEAM + lane) * V, dim - V);      // the last vector of an odd width is moved back: its first columns are summed and written twice, alike
-    const int64_t lo = ch * per_chunk, hi = min(lo + per_chunk, m);
-    const unsigned before = lo > 0 ? keys[lo - 1] : kEmpty, after = hi < m ? keys[hi] : kEmpty;
+    const int64_t lo = ch * per_chunk;
+    const int len = (int)min((int64_t)per_chunk, m - lo);
+    const auto key_at = [&](int64_t i) { return FIRST ? sorted[i].x : keys[i]; };
+    const unsigned before = lo > 0 ? key_at(lo - 1) : kEmpty, after = lo + len < m ? key_at(lo + len) : kEmpty;
+    // the team's lanes hold the keys and positions of a batch (kHeld each) and hand them around; the next batch's are on their way meanwhile
+    constexpr int kHeld = kBatch > TEAM ? kBatch / TEAM : 1;
+    unsigned hk[kHeld], ho[kHeld];
+    const auto hold = [&](int i0) {
+#pragma unroll
+        for (int q = 0; q < kHeld; ++q) {
+            const int i = i0 + q * TEAM + lane;
+            const bool in = i < len && q * TEAM + lane < kBatch;
+            const uint2 t = !in ? make_uint2(kEmpty, 0u) : FIRST ? sorted[lo + i] : make_uint2(keys[lo + i], 0u);
+            hk[q] = t.x;
+            ho[q] = t.y;
+        }
+    };
+    hold(0);
     unsigned cur = kEmpty, head_key = kEmpty, tail_key = kEmpty;
     bool from_left = false;
     float acc[V];
@@ -220,37 +311,37 @@ __global__ __launch_bounds__(256) void sum_runs_kernel(const unsigned* __restric
             if (from_left && to_right) tail_key = cur | kCarry;       // the whole chunk is inside one run: one row, and a key that keeps the run together
         }
     };
-    for (int64_t i0 = lo; i0 < hi; i0 += BATCH) {
-        unsigned k[BATCH];
-        float f[BATCH][V];
+#pragma unroll 1
+    for (int i0 = 0; i0 < len; i0 += kBatch) {                       // whole teams; the shuffles stay within a team
+        unsigned k[kBatch];
+        nvp_vec<S, V> f[kBatch];
 #pragma unroll
-        for (int b = 0; b < BATCH; ++b) {
-            const int64_t i = i0 + b;
-            k[b] = i < hi ? keys[i] : kEmpty;
+        for (int b = 0; b < kBatch; ++b) {
+            const auto from = [&](const unsigned (&v)[kHeld]) {
+                return TEAM == 64 ? (unsigned)__builtin_amdgcn_readlane((int)v[b / TEAM], b % TEAM) : (unsigned)__shfl((int)v[b / TEAM], b % TEAM, TEAM);
+            };
+            k[b] = from(hk);
             if (FIRST && k[b] >= (unsigned)codes) k[b] = kEmpty;
+            const unsigned o = FIRST ? from(ho) : 0u;
+            // first level: an entry without a row reads row 0 and drops it, so that no branch stands between the loads; later lists are mostly empty
+            if (FIRST) f[b] = nvp_load_raw<S, V>(rows + (int64_t)o * dim + c);
+            else if (k[b] != kEmpty && !(k[b] & kCarry)) f[b] = nvp_load_raw<S, V>(rows + (lo + i0 + b) * dim + c);
         }
+        if (i0 + kBatch < len) hold(i0 + kBatch);
 #pragma unroll
-        for (int b = 0; b < BATCH; ++b) {
-            const int64_t i = i0 + b;
-            const bool has = live && k[b] != kEmpty && !(k[b] & kCarry);
-            const int64_t src = has ? (FIRST ? (int64_t)order[i] : i) : 0;
-            if (has) nvp_load<S, V>(rows + src * dim + c, f[b]);
-#pragma unroll
-            for (int e = 0; e < V; ++e) f[b][e] = has ? f[b][e] : 0.f;
-        }
-#pragma unroll
-        for (int b = 0; b < BATCH; ++b) {
+        for (int b = 0; b < kBatch; ++b) {
             if (k[b] == kEmpty) continue;
             const unsigned key = k[b] & ~kCarry;
             if (key != cur) {
                 flush(false);
-                from_left = i0 + b == lo && same_run(before, key);
+                from_left = i0 + b == 0 && same_run(before, key);
                 cur = key;
 #pragma unroll
                 for (int e = 0; e < V; ++e) acc[e] = 0.f;
             }
+            if (!(k[b] & kCarry))
 #pragma unroll
-            for (int e = 0; e < V; ++e) acc[e] += f[b][e];
+                for (int e = 0; e < V; ++e) acc[e] += (float)f[b].v[e];
         }
     }
     flush(same_run(cur, after));
@@ -260,18 +351,70 @@ __global__ __launch_bounds__(256) void sum_runs_kernel(const unsigned* __restric
     }
 }
 
+// A list of at most kLast entries: one workgroup per entry; the entry that begins a run adds the whole run, its teams every kTeams-th entry, the teams in order.
+constexpr int last_threads(int team) { return team >= 32 ? 512 : 256; }      // 16 teams of whole waves; with smaller teams the sum over the teams would take over
+template <typename T, int TEAM, int V>
+__global__ __launch_bounds__(last_threads(TEAM)) void sum_last_kernel(const unsigned* __restrict__ keys, const float* __restrict__ rows, T* __restrict__ dtable, int m, int dim, float scale) {
+    constexpr int kTeams = last_threads(TEAM) / TEAM, kBatch = 16;
+    const int i = blockIdx.x;
+    const unsigned key = keys[i];
+    if (key == kEmpty || (key & kCarry) || (i > 0 && ((keys[i - 1] ^ key) & ~kCarry) == 0u)) return;      // a run begins with an entry that has a row
+    __shared__ float part[kTeams][TEAM * V];
+    const int lane = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
+    const bool live = (blockIdx.y * TEAM + lane) * V < dim;
+    const int c = min((int)(blockIdx.y * TEAM + lane) * V, dim - V);
+    float acc[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) acc[e] = 0.f;
+    bool more = true;
+    for (int e0 = i + team; more; e0 += kTeams * kBatch) {
+        nvp_vec<float, V> f[kBatch];
+        unsigned k[kBatch];
+        bool has[kBatch];
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) k[b] = keys[min(e0 + b * kTeams, m - 1)];
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) {
+            const int at = e0 + b * kTeams;
+            more = at < m && k[b] != kEmpty && ((k[b] ^ key) & ~kCarry) == 0u;      // entries of a run are side by side: the last one looked at tells whether there may be more
+            has[b] = more && !(k[b] & kCarry);
+            f[b] = nvp_load_raw<float, V>(rows + (int64_t)(has[b] ? at : i) * dim + c);      // (no branch between the loads: an entry without a row reads the first one's)
+        }
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b)
+            if (has[b])
+#pragma unroll
+                for (int e = 0; e < V; ++e) acc[e] += f[b].v[e];
+    }
+#pragma unroll
+    for (int e = 0; e < V; ++e) part[team][lane * V + e] = acc[e];
+    __syncthreads();
+    if (team == 0 && live) {
+        float t[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            float s = 0.f;
+#pragma unroll
+            for (int k = 0; k < kTeams; ++k) s += part[k][lane * V + e];
+            t[e] = s * scale;
+        }
+        nvp_store<T, V>(dtable + (int64_t)key * dim + c, t);
+    }
+}
+
 // ---- host ---------------------------------------------------------------------------------------------------------------------------------------
 int64_t up256(int64_t b) { return (b + 255) / 256 * 256; }
-constexpr int kPerChunk1 = 32, kPerChunk2 = 64;
+constexpr int kPerChunk2 = 32, kLast = 2560;
 
 struct Plan {
     bool small;
     int passes, bits;
     int64_t radix_chunks;
     int per_chunk;                  // first level
-    int levels;
-    int64_t m[12], chunks[12];      // entries and chunks of each level
-    int64_t off_key[2], off_pos[2], off_count, off_lkey[2], off_lrow[2], bytes;
+    int levels;                     // of sum_runs_kernel
+    int64_t m[12], chunks[12];      // entries (and, behind them, those of the list that is left) and chunks of each level
+    int64_t last;                   // entries for sum_last_kernel, 0: nothing left
+    int64_t off_sorted[2], off_count, off_total, off_lkey[2], off_lrow[2], bytes;
 };
 Plan plan_of(int64_t n, int64_t codes, int64_t dim) {
     Plan P{};
@@ -281,28 +424,31 @@ Plan plan_of(int64_t n, int64_t codes, int64_t dim) {
     P.passes = (b + kMaxBits - 1) / kMaxBits;
     P.bits = (b + P.passes - 1) / P.passes;
     P.radix_chunks = (n + kChunk - 1) / kChunk;
-    P.per_chunk = n < 65536 ? 16 : kPerChunk1;                       // short lists: more teams with less to do one after another
+    // entries per team at the first level: enough teams to keep the chip's memory busy (256 CUs x 8 waves), and no fewer entries than that allows, because every
+    // chunk may leave two partial rows behind
+    const int64_t waves = n * ((dim * 4 + 1023) / 1024) * (dim >= 256 ? 64 : dim >= 128 ? 32 : dim >= 64 ? 16 : 8) / 64;
+    P.per_chunk = 16;
+    while (P.per_chunk < 128 && waves / (2 * P.per_chunk) >= 2048) P.per_chunk *= 2;
     int64_t m = n;
-    for (P.levels = 0;;) {
-        const int per = P.levels == 0 ? P.per_chunk : kPerChunk2;
+    for (P.levels = 0, P.last = 0;;) {
         P.m[P.levels] = m;
-        P.chunks[P.levels] = (m + per - 1) / per;
-        const bool done = P.chunks[P.levels] <= 1;
-        m = 2 * P.chunks[P.levels];
-        ++P.levels;
-        if (done) break;
+        P.chunks[P.levels] = (m + (P.levels ? kPerChunk2 : P.per_chunk) - 1) / (P.levels ? kPerChunk2 : P.per_chunk);
+        m = P.chunks[P.levels] <= 1 ? 0 : 2 * P.chunks[P.levels];
+        P.m[++P.levels] = m;
+        if (m <= kLast) break;
     }
+    P.last = m;
     int64_t at = 0;
     for (int i = 0; i < (P.small ? 1 : 2); ++i) {
-        P.off_key[i] = at;
-        at += up256(n * 4);
-        P.off_pos[i] = at;
-        at += up256(n * 4);
+        P.off_sorted[i] = at;
+        at += up256(n * 8);
     }
     P.off_count = at;
     if (!P.small) at += up256(P.radix_chunks * (1ll << P.bits) * 4);
+    P.off_total = at;
+    if (!P.small) at += up256((1ll << P.bits) * 4);
     for (int i = 0; i < 2; ++i) {                                    // level l writes list l & 1: a later list is never longer than the one it replaces
-        const int64_t e = i + 1 < P.levels ? P.m[i + 1] : 0;
+        const int64_t e = i + 1 <= P.levels ? P.m[i + 1] : 0;
         P.off_lkey[i] = at;
         at += up256(e * 4);
         P.off_lrow[i] = at;
@@ -321,90 +467,92 @@ template <typename A, typename B> constexpr int vec_of() { return 16 / (sizeof(A
 
 int team_of(int64_t lanes) { return lanes <= 4 ? 4 : lanes <= 8 ? 8 : lanes <= 16 ? 16 : lanes <= 32 ? 32 : 64; }
 
+// calls `f` with the team's size as a constant
+template <typename F> void with_team(int team, F f) {
+    if (team == 4) f(std::integral_constant<int, 4>());
+    else if (team == 8) f(std::integral_constant<int, 8>());
+    else if (team == 16) f(std::integral_constant<int, 16>());
+    else if (team == 32) f(std::integral_constant<int, 32>());
+    else f(std::integral_constant<int, 64>());
+}
+
 template <typename T, typename O, typename I, int V>
 int fwd(const I* ids, const T* table, O* out, int64_t n, int64_t codes, int dim, float scale, hipStream_t st) {
     const int team = team_of((dim + V - 1) / V);
     const int64_t blocks = (n + 4 * (256 / team) - 1) / (4 * (256 / team));
     if (blocks > 0x7fffffff) return NVP_ERR_UNSUPPORTED;
     const dim3 g((unsigned)blocks), wg(256);
-    const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, g, wg, 0, st, ids, table, out, n, codes, dim, scale); };
-    if (team == 4) go(lookup_fwd_kernel<T, O, I, 4, V>);
-    else if (team == 8) go(lookup_fwd_kernel<T, O, I, 8, V>);
-    else if (team == 16) go(lookup_fwd_kernel<T, O, I, 16, V>);
-    else if (team == 32) go(lookup_fwd_kernel<T, O, I, 32, V>);
-    else go(lookup_fwd_kernel<T, O, I, 64, V>);
+    with_team(team, [&](auto t) { hipLaunchKernelGGL((lookup_fwd_kernel<T, O, I, decltype(t)::value, V>), g, wg, 0, st, ids, table, out, n, codes, dim, scale); });
     NVP_LAUNCH_CHECK();
     return 0;
 }
 
 template <typename S, typename T, bool FIRST, int V>
-int sum_level(const unsigned* keys, const unsigned* order, const S* rows, T* dtable, unsigned* nkeys, float* nrows, int64_t m, int per_chunk, int64_t chunks, int64_t codes, int dim, float scale,
+int sum_level(const uint2* sorted, const unsigned* keys, const S* rows, T* dtable, unsigned* nkeys, float* nrows, int64_t m, int per_chunk, int64_t chunks, int64_t codes, int dim, float scale,
               hipStream_t st) {
     const int team = team_of((dim + V - 1) / V), teams = 256 / team;
     const int64_t sums = (chunks + teams - 1) / teams, fill = FIRST ? (codes + 255) / 256 : 0, cols = (dim + team * V - 1) / (team * V);
     if (sums + fill > 0x7fffffff || cols > 65535) return NVP_ERR_UNSUPPORTED;
-    const dim3 g((unsigned)(sums + fill), (unsigned)cols), wg(256);
-    const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, g, wg, 0, st, keys, order, rows, dtable, nkeys, nrows, m, per_chunk, chunks, sums, codes, dim, scale); };
-    if (team == 4) go(sum_runs_kernel<S, T, FIRST, 4, V, 8>);
-    else if (team == 8) go(sum_runs_kernel<S, T, FIRST, 8, V, 8>);
-    else if (team == 16) go(sum_runs_kernel<S, T, FIRST, 16, V, 8>);
-    else if (team == 32) go(sum_runs_kernel<S, T, FIRST, 32, V, 8>);
-    else go(sum_runs_kernel<S, T, FIRST, 64, V, 8>);
+    with_team(team, [&](auto t) {
+        hipLaunchKernelGGL((sum_runs_kernel<S, T, FIRST, decltype(t)::value, V>), dim3((unsigned)(sums + fill), (unsigned)cols), dim3(256), 0, st, sorted, keys, rows, dtable, nkeys, nrows, m,
+                           per_chunk, chunks, sums, codes, dim, scale);
+    });
     NVP_LAUNCH_CHECK();
     return 0;
 }
 
 template <typename S, typename T, int V, int VF>
-int sums(const Plan& P, const unsigned* keys, const unsigned* order, const S* dout, T* dtable, uint8_t* ws, int64_t codes, int dim, float scale, hipStream_t st) {
+int sums(const Plan& P, const uint2* sorted, const S* dout, T* dtable, uint8_t* ws, int64_t codes, int dim, float scale, hipStream_t st) {
     const auto lkey = [&](int l) { return (unsigned*)(ws + P.off_lkey[l & 1]); };
     const auto lrow = [&](int l) { return (float*)(ws + P.off_lrow[l & 1]); };
-    const bool more = P.levels > 1;
-    int rc = sum_level<S, T, true, V>(keys, order, dout, dtable, more ? lkey(0) : nullptr, more ? lrow(0) : nullptr, P.m[0], P.per_chunk, P.chunks[0], codes, dim, scale, st);
-    for (int l = 1; !rc && l < P.levels; ++l) {
-        const bool next = l + 1 < P.levels;
-        rc = sum_level<float, T, false, VF>(lkey(l - 1), nullptr, lrow(l - 1), dtable, next ? lkey(l) : nullptr, next ? lrow(l) : nullptr, P.m[l], kPerChunk2, P.chunks[l], codes, dim, scale, st);
+    int rc = 0;
+    for (int l = 0; !rc && l < P.levels; ++l) {
+        unsigned* nk = P.m[l + 1] ? lkey(l) : nullptr;
+        float* nr = P.m[l + 1] ? lrow(l) : nullptr;
+        rc = l == 0 ? sum_level<S, T, true, V>(sorted, nullptr, dout, dtable, nk, nr, P.m[0], P.per_chunk, P.chunks[0], codes, dim, scale, st)
+                    : sum_level<float, T, false, VF>(nullptr, lkey(l - 1), lrow(l - 1), dtable, nk, nr, P.m[l], kPerChunk2, P.chunks[l], codes, dim, scale, st);
     }
-    return rc;
+    if (rc || !P.last) return rc;
+    const int team = team_of((dim + VF - 1) / VF);
+    with_team(team, [&](auto t) {
+        hipLaunchKernelGGL((sum_last_kernel<T, decltype(t)::value, VF>), dim3((unsigned)P.last, (unsigned)((dim + team * VF - 1) / (team * VF))), dim3(last_threads(decltype(t)::value)), 0, st, lkey(P.levels - 1),
+                           lrow(P.levels - 1), dtable, (int)P.last, dim, scale);
+    });
+    NVP_LAUNCH_CHECK();
+    return 0;
 }
 
 template <typename I, typename S, typename T>
 int bwd(const I* ids, const S* dout, T* dtable, int64_t n, int64_t codes, int dim, float scale, uint8_t* ws, hipStream_t st) {
     const Plan P = plan_of(n, codes, dim);
-    unsigned *key[2], *pos[2];
-    for (int i = 0; i < 2; ++i) {
-        key[i] = (unsigned*)(ws + P.off_key[P.small ? 0 : i]);
-        pos[i] = (unsigned*)(ws + P.off_pos[P.small ? 0 : i]);
-    }
+    uint2* buf[2] = {(uint2*)(ws + P.off_sorted[0]), (uint2*)(ws + P.off_sorted[P.small ? 0 : 1])};
     int at = 0;
     if (n == 0) {
         // nothing to sort: the sums below only write zeros
     } else if (P.small) {
         int padded = 2;
         while (padded < n) padded <<= 1;
-        hipLaunchKernelGGL((sort_small_kernel<I>), dim3(1), dim3(1024), 0, st, ids, key[0], pos[0], (int)n, codes, padded);
+        hipLaunchKernelGGL((sort_small_kernel<I>), dim3(1), dim3(1024), 0, st, ids, buf[0], (int)n, codes, padded);
         NVP_LAUNCH_CHECK();
     } else {
-        unsigned* count = (unsigned*)(ws + P.off_count);
-        const dim3 g((unsigned)P.radix_chunks), wg(1024);
-        const size_t lds = (size_t)kWaves * (1u << P.bits) * 4;
+        unsigned *count = (unsigned*)(ws + P.off_count), *total = (unsigned*)(ws + P.off_total);
+        const dim3 g((unsigned)P.radix_chunks), wg(256);
         for (int p = 0; p < P.passes; ++p) {
             const int shift = p * P.bits;
-            const unsigned *kin = key[at], *pin = pos[at];
-            unsigned *kout = key[at ^ 1], *pout = pos[at ^ 1];
-            if (p == 0) hipLaunchKernelGGL((radix_count_kernel<I, true>), g, wg, 0, st, ids, kin, count, n, codes, shift, P.bits);
-            else hipLaunchKernelGGL((radix_count_kernel<I, false>), g, wg, 0, st, ids, kin, count, n, codes, shift, P.bits);
+            if (p == 0) hipLaunchKernelGGL((radix_count_kernel<I, true>), g, wg, 0, st, ids, buf[at], count, n, codes, shift, P.bits);
+            else hipLaunchKernelGGL((radix_count_kernel<I, false>), g, wg, 0, st, ids, buf[at], count, n, codes, shift, P.bits);
             NVP_LAUNCH_CHECK();
-            hipLaunchKernelGGL(radix_scan_kernel, dim3(1), wg, 0, st, count, (int)P.radix_chunks, P.bits);
+            hipLaunchKernelGGL(radix_scan_kernel, dim3(((1u << P.bits) + 63) / 64), dim3(1024), 0, st, count, total, (int)P.radix_chunks, P.bits);
             NVP_LAUNCH_CHECK();
-            if (p == 0) hipLaunchKernelGGL((radix_scatter_kernel<I, true>), g, wg, lds, st, ids, kin, pin, count, kout, pout, n, codes, shift, P.bits);
-            else hipLaunchKernelGGL((radix_scatter_kernel<I, false>), g, wg, lds, st, ids, kin, pin, count, kout, pout, n, codes, shift, P.bits);
+            if (p == 0) hipLaunchKernelGGL((radix_scatter_kernel<I, true>), g, wg, 0, st, ids, buf[at], count, total, buf[at ^ 1], n, codes, shift, P.bits);
+            else hipLaunchKernelGGL((radix_scatter_kernel<I, false>), g, wg, 0, st, ids, buf[at], count, total, buf[at ^ 1], n, codes, shift, P.bits);
             NVP_LAUNCH_CHECK();
             at ^= 1;
         }
     }
     constexpr int V = vec_of<S, T>();
-    if (dim >= (V > 4 ? V : 4)) return sums<S, T, V, 4>(P, key[at], pos[at], dout, dtable, ws, codes, dim, scale, st);
-    return sums<S, T, 1, 1>(P, key[at], pos[at], dout, dtable, ws, codes, dim, scale, st);
+    if (dim >= (V > 4 ? V : 4)) return sums<S, T, V, 4>(P, buf[at], dout, dtable, ws, codes, dim, scale, st);
+    return sums<S, T, 1, 1>(P, buf[at], dout, dtable, ws, codes, dim, scale, st);
 }
 
 template <typename T, typename O>
