@@ -85,6 +85,20 @@ __device__ __forceinline__ f32x16 mma(const frag<true>& a, const frag<true>& b, 
     return c;
 }
 
+// two tiles against one operand, their chains interleaved
+template <bool W> __device__ __forceinline__ void mma2(const frag<W>& a0, const frag<W>& a1, const frag<W>& b, f32x4& c0, f32x4& c1) {
+    if constexpr (W) {
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+            c0 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a0.h[p], b.h[p], c0, 0, 0, 0);
+            c1 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a1.h[p], b.h[p], c1, 0, 0, 0);
+        }
+    } else {
+        c0 = mma(a0, b, c0);
+        c1 = mma(a1, b, c1);
+    }
+}
+
 // ---- x -> workspace: 16 lanes per block of 128, 8 values each -----------------------------------------------------------------------------
 // q [rows][128 * KB], scales [rows][KB4] (bytes); the launch's last workgroups copy the weights' scales to dword-padded rows [NB][KB4].
 template <typename T>
@@ -264,6 +278,132 @@ __global__ __launch_bounds__(512) void linear8_rows_kernel(const T* __restrict__
     }
 }
 
+// ---- many rows, few columns: x quantised on the way, weights resident in LDS ---------------------------------------------------------------
+// With up to 256 columns the product is bound by the bytes of x and y, and quantising x in a pass of its own would move a quarter more: here a wave
+// takes 16 rows at a time, block by block: 16-byte loads (four lanes cover 64 contiguous bytes of a row) one block ahead, the block's maximum by two
+// shuffles, and the quantised block is the matrix instruction's operand right away.  The weights (all columns, all of K) stay in LDS, with the bytes of a
+// block in the order in which the lanes hold x's columns and the 16-byte pieces of a row swizzled by the row, so that operand reads are free of bank conflicts.
+// Weights are the first operand: a lane then holds four consecutive columns of one row of y.
+template <int NT> __host__ __device__ constexpr int64_t narrow_lds(int64_t kb) { return 16 * NT * kb * 128 + 2 * kb + 16 * NT * 4; }
+template <typename T, int NT>
+__global__ __launch_bounds__(256, NT <= 8 ? 3 : 2) void linear8_narrow_kernel(const T* __restrict__ x, const uint8_t* __restrict__ qw, const uint8_t* __restrict__ ew, const T* __restrict__ bias, T* __restrict__ y,
+                                                             int64_t rows, int k, int n) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    constexpr bool kWide = sizeof(T) == 4;
+    constexpr int E = 16 / sizeof(T), J = 32 / E;                                           // columns per load, loads per lane and block
+    const int kb = (int)kblocks(k), kp = kb * 128, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
+    float* const sbias = reinterpret_cast<float*>(lds + 16 * NT * kp);
+    uint8_t* const sexp = reinterpret_cast<uint8_t*>(sbias + 16 * NT);
+    // Block b is read from column first(b) on: a last block that is not full is moved back to end with the row (k >= 128), and its first columns, which belong
+    // to the block before, are dropped from x: every load stays inside its row, at full width.
+    const auto first = [&](int b) { return min(b * 128, k - 128); };
+    // byte 4 E j + E g + e of a block (column order) -> byte 32 g + E j + e (lane order); its 16-byte piece p of row r lies at place p ^ (r & 7)
+    for (int t = threadIdx.x; t < 16 * NT * kp / 4; t += 256) {
+        const int r = t / (kp / 4), c = (t - r * (kp / 4)) * 4, b = c >> 7, o = c & 127;
+        const int to = 32 * (o % (4 * E) / E) + E * (o / (4 * E)) + o % E;
+        unsigned v = 0u;
+        if (r < n) __builtin_memcpy(&v, qw + (int64_t)r * kp + first(b) + o, 4);
+        *reinterpret_cast<unsigned*>(lds + r * kp + b * 128 + ((to >> 4) ^ (r & 7)) * 16 + (to & 15)) = v;
+    }
+    for (int t = threadIdx.x; t < 16 * NT; t += 256) sbias[t] = bias && t < n ? (float)bias[t] : 0.f;
+    for (int t = threadIdx.x; t < 2 * kb; t += 256) sexp[t] = t < (n + 127) / 128 * kb ? ew[t] : 127;
+    __syncthreads();
+
+    const int64_t tiles = (rows + 15) / 16, step = (int64_t)gridDim.x * 4;
+    nvp_vec<T, E> raw[J];
+    const auto fetch = [&](int64_t tile, int b) {
+        const T* p = x + min(tile * 16 + i, rows - 1) * k + first(b) + g * E;               // rows behind the last one read the last one: their results are not stored
+#pragma unroll
+        for (int j = 0; j < J; ++j) raw[j] = nvp_load_raw<T, E>(p + j * 4 * E);
+    };
+    int64_t tile = (int64_t)blockIdx.x * 4 + wave;
+    if (tile < tiles) fetch(tile, 0);
+    for (; tile < tiles; tile += step) {
+        f32x4 acc[NT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+        for (int b = 0; b < kb; ++b) {
+            float v[32];
+#pragma unroll
+            for (int j = 0; j < J; ++j)
+#pragma unroll
+                for (int e = 0; e < E; ++e) v[j * E + e] = (float)raw[j].v[e];
+            if (first(b) < b * 128) {
+#pragma unroll
+                for (int j = 0; j < J; ++j)
+#pragma unroll
+                    for (int e = 0; e < E; ++e) v[j * E + e] = first(b) + (j * 4 + g) * E + e < b * 128 ? 0.f : v[j * E + e];
+            }
+            {
+                const bool here = b + 1 < kb;
+                const int64_t then = here ? tile : tile + step;
+                if (then < tiles) fetch(then, here ? b + 1 : 0);
+            }
+            unsigned top = 0u;
+#pragma unroll
+            for (int e = 0; e < 32; ++e) top = max(top, __float_as_uint(v[e]) & 0x7fffffffu);
+            top = max(top, (unsigned)__shfl_xor((int)top, 16));
+            top = max(top, (unsigned)__shfl_xor((int)top, 32));
+            const bool odd = __any(top >= 0x7f800000u);                                     // an infinity or a NaN somewhere in the 16 rows: the careful way
+            if (odd) {
+                top = 0u;
+#pragma unroll
+                for (int e = 0; e < 32; ++e) top = max(top, finite_bits(v[e]));
+                top = max(top, (unsigned)__shfl_xor((int)top, 16));
+                top = max(top, (unsigned)__shfl_xor((int)top, 32));
+            }
+            const unsigned byte = scale_byte(top);
+            const float inv = inv_scale(byte);
+            v8i q;
+            if (odd) {
+#pragma unroll
+                for (int p = 0; p < 8; ++p) q[p] = quant4(&v[4 * p], inv);
+            } else {
+#pragma unroll
+                for (int p = 0; p < 8; ++p) {
+                    int w = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * p] * inv, v[4 * p + 1] * inv, 0, false);
+                    q[p] = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * p + 2] * inv, v[4 * p + 3] * inv, w, true);
+                }
+            }
+            frag<kWide> xf;
+            xf.set(q, (int)byte);
+            const int s0 = sexp[b], s1 = sexp[kb + b];
+            __builtin_amdgcn_sched_barrier(0);                                              // operand reads stay behind the quantisation: its registers are free then
+#pragma unroll
+            for (int t = 0; t < NT; t += 2) {
+                frag<kWide> wf[2];
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const int r = 16 * (t + u) + i;
+                    const uint8_t* w = lds + r * kp + b * 128;
+                    const v4i lo = *reinterpret_cast<const v4i*>(w + ((2 * g) ^ (r & 7)) * 16), hi = *reinterpret_cast<const v4i*>(w + ((2 * g + 1) ^ (r & 7)) * 16);
+                    wf[u].set(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), t < 8 ? s0 : s1);
+                }
+                mma2(wf[0], wf[1], xf, acc[t], acc[t + 1]);
+            }
+        }
+        const int64_t row = tile * 16 + i;
+        // D: row (column of y) 4 (lane >> 4) + r, column (row of y) lane & 15
+        if (row < rows && n % 4 == 0) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const int c = 16 * t + 4 * g;
+                float f[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) f[e] = acc[t][e] + sbias[c + e];
+                if (c < n) nvp_store<T, 4>(y + row * n + c, f);
+            }
+        } else if (row < rows) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (16 * t + 4 * g + e < n) y[row * n + 16 * t + 4 * g + e] = (T)(acc[t][e] + sbias[16 * t + 4 * g + e]);
+        }
+    }
+}
+
 // ---- many rows: BM x BN tiles through LDS --------------------------------------------------------------------------------------------------
 // Two stages of (BM + BN) x 128 bytes, filled by direct-to-LDS loads one block ahead; a wave computes (BM / WM) x (BN / WN) with
 // 32x32x64 instructions.  LDS rows are 128 bytes; the 16-byte piece c of row r lies at place c ^ (r & 7), so the eight lanes that a
@@ -413,10 +553,30 @@ int launch_rows(const T* x, const uint8_t* qx, const uint8_t* ex, const uint8_t*
     return 0;
 }
 
+// columns rounded up to 64, 128 or 256 if that many fit the kernel above with two workgroups per CU, else 0
+int narrow_columns(int64_t rows, int64_t k, int64_t n) {
+    const int nt = n <= 64 ? 4 : n <= 128 ? 8 : n <= 256 ? 16 : 0;
+    return rows >= 2048 && k >= 128 && nt && 16 * nt * kblocks(k) * 128 <= 65536 ? 16 * nt : 0;
+}
+template <typename T, int NT>
+int launch_narrow(const T* x, const uint8_t* qw, const uint8_t* ew, const void* bias, void* y, int64_t rows, int64_t k, int64_t n, hipStream_t st) {
+    const int64_t groups = (rows + 63) / 64;
+    const size_t bytes = (size_t)narrow_lds<NT>(kblocks(k));
+    hipLaunchKernelGGL((linear8_narrow_kernel<T, NT>), dim3((unsigned)(groups < 768 ? groups : 768)), dim3(256), bytes, st, x, qw, ew, (const T*)bias, (T*)y, rows,
+                       (int)k, (int)n);
+    NVP_LAUNCH_CHECK();
+    return 0;
+}
+
 template <typename T>
 int linear8(const T* x, const uint8_t* qw, const uint8_t* ew, const void* bias, void* y, int64_t rows, int64_t k, int64_t n, uint8_t* ws, hipStream_t st) {
     const int64_t kb = kblocks(k), kp = kb * 128, kbp = kb4(k), nb = (n + 127) / 128;
     if (rows <= 16) return launch_rows<T, 1, 1, true>(x, nullptr, nullptr, qw, ew, bias, y, rows, k, n, st);
+    switch (narrow_columns(rows, k, n)) {
+        case 64: return launch_narrow<T, 4>(x, qw, ew, bias, y, rows, k, n, st);
+        case 128: return launch_narrow<T, 8>(x, qw, ew, bias, y, rows, k, n, st);
+        case 256: return launch_narrow<T, 16>(x, qw, ew, bias, y, rows, k, n, st);
+    }
     uint8_t* qx = ws;
     uint8_t* ex = qx + rows * kp;
     uint8_t* ewp = ex + rows * kbp;                                                          // rows * kbp is a multiple of 4
@@ -436,7 +596,7 @@ bool sizes_ok(int64_t rows, int64_t k, int64_t n) { return rows >= 0 && n >= 1 &
 
 extern "C" int64_t nvp_linear8_workspace_bytes(int64_t rows, int64_t k, int64_t n) {
     if (!sizes_ok(rows, k, n)) return NVP_ERR_BADARG;
-    if (rows <= 16) return 0;
+    if (rows <= 16 || narrow_columns(rows, k, n)) return 0;
     return rows * kblocks(k) * 128 + rows * kb4(k) + (n + 127) / 128 * kb4(k);
 }
 

@@ -153,7 +153,8 @@ def test_block_form_at_the_borders():
 
 
 SHAPES = [(1, 1, 1), (1, 128, 16), (2, 130, 17), (16, 4096, 100), (17, 256, 128), (33, 129, 300), (64, 1000, 65), (513, 384, 129), (600, 100, 1000), (700, 640, 4099),
-          (4099, 300, 2050), (1, 1100, 5003), (8, 8192, 256)]
+          (4099, 300, 2050), (1, 1100, 5003), (8, 8192, 256),
+          (2048, 242, 128), (2049, 1, 1), (2100, 127, 61), (3001, 130, 200), (2500, 300, 65), (5000, 128, 256), (2777, 515, 100)]
 
 
 @pytest.mark.gpu
@@ -175,8 +176,8 @@ def test_linear8(m, k, n, dtype):
 def test_linear8_scales_of_every_block_count():
     """Blocks whose scales lie far apart, in x and in the weight: a scale that is taken from a neighbouring row or block shows at once."""
     g = torch.Generator().manual_seed(3)
-    for m in (5, 40, 300, 4100):
-        k, n = 128 * 5 + 3, 2100
+    for m, n in ((5, 2100), (40, 2100), (300, 2100), (4100, 2100), (4100, 70), (2100, 40)):
+        k = 128 * 5 + 3
         x = torch.randn(m, k, generator=g) * torch.exp2(torch.randint(-12, 13, (m, -(-k // 128)), generator=g).float()).repeat_interleave(128, 1)[:, :k]
         up = torch.exp2(torch.randint(-12, 13, (-(-n // 128), -(-k // 128)), generator=g).float())
         w = torch.randn(n, k, generator=g) * up.repeat_interleave(128, 0)[:n].repeat_interleave(128, 1)[:, :k]
@@ -186,10 +187,10 @@ def test_linear8_scales_of_every_block_count():
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("m", [3, 100, 5000])
-def test_linear8_rows_with_non_finite_values_are_nan_and_no_others(m):
+@pytest.mark.parametrize("m,n", [(3, 2060), (100, 2060), (5000, 2060), (5000, 60)])
+def test_linear8_rows_with_non_finite_values_are_nan_and_no_others(m, n):
     g = torch.Generator().manual_seed(m)
-    x, w = torch.randn(m, 200, generator=g), torch.randn(2060, 200, generator=g)
+    x, w = torch.randn(m, 200, generator=g), torch.randn(n, 200, generator=g)
     x[0, 5], x[m - 1, 199] = float("inf"), float("nan")
     q, e = Q.quantize_blocks(w.to(dev()), 128)
     y = Q.linear8(x.to(dev()), q, e).cpu()
