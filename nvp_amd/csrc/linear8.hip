@@ -43,6 +43,37 @@ __device__ __forceinline__ int quant4(const float* v, float inv) {
     return p;
 }
 
+// maximum over 16 neighbouring lanes, in every lane: rotations within the row of 16, no LDS
+__device__ __forceinline__ unsigned max16(unsigned v) {
+    v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x128, 0xf, 0xf, true));    // row_ror:8
+    v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x124, 0xf, 0xf, true));
+    v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x122, 0xf, 0xf, true));
+    return max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x121, 0xf, 0xf, true));
+}
+// one row's block of 128, 8 values in each of 16 neighbouring lanes -> 8 bytes per lane and the block's scale byte
+__device__ __forceinline__ int2 quant8(const float (&v)[8], unsigned& byte) {
+    unsigned top = 0u;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(v[e]) & 0x7fffffffu);
+    top = max16(top);
+    int2 q;
+    if (!__any(top >= 0x7f800000u)) {
+        byte = scale_byte(top);
+        const float inv = inv_scale(byte);
+        q.x = __builtin_amdgcn_cvt_pk_fp8_f32(v[2] * inv, v[3] * inv, __builtin_amdgcn_cvt_pk_fp8_f32(v[0] * inv, v[1] * inv, 0, false), true);
+        q.y = __builtin_amdgcn_cvt_pk_fp8_f32(v[6] * inv, v[7] * inv, __builtin_amdgcn_cvt_pk_fp8_f32(v[4] * inv, v[5] * inv, 0, false), true);
+        return q;
+    }
+    top = 0u;                                                                                // an infinity or a NaN among the wave's blocks: the careful way
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = max(top, finite_bits(v[e]));
+    byte = scale_byte(max16(top));
+    const float inv = inv_scale(byte);
+    q.x = quant4(v, inv);
+    q.y = quant4(v + 4, inv);
+    return q;
+}
+
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
@@ -124,16 +155,8 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const T* __restrict__ x
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = c0 + e < k ? (float)x[row * k + c0 + e] : 0.f;
     }
-    unsigned top = 0u;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) top = max(top, finite_bits(v[e]));
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, o));
-    const unsigned byte = scale_byte(top);
-    const float inv = inv_scale(byte);
-    int2 p;
-    p.x = quant4(v, inv);
-    p.y = quant4(v + 4, inv);
+    unsigned byte;
+    const int2 p = quant8(v, byte);
     *reinterpret_cast<int2*>(q + row * kb * 128 + c0) = p;
     if (lane16 == 0) ex[row * kb_pad + b] = (uint8_t)byte;
 }
@@ -178,25 +201,24 @@ __global__ __launch_bounds__(256) void dequant_blocks_kernel(const uint8_t* __re
     x[i] = (T)(v * s);
 }
 
-// ---- few rows: every wave walks its share of K with operands straight from global memory ----------------------------------------------------
-// One workgroup: 16 MT rows x 16 NT columns; its eight waves take every eighth block of 128 and add their tiles up through LDS, so a single row
-// times 4096 columns is 256 workgroups x 8 waves that read disjoint weights: bound by the bytes of the weights.  FUSED (MT = 1): x is quantised
-// in registers by every wave (a lane group of 4 holds one row's block; its maximum is two shuffles), no workspace and no second launch.
+// ---- few rows: every wave walks its share of K with the weights straight from global memory -------------------------------------------------
+// One workgroup: 16 MT rows x 16 NT columns; its WAVES waves take every WAVES-th block of 128 and add their tiles up through LDS, so a single row
+// times 4096 columns is 256 workgroups x 8 waves that read disjoint weights: bound by the bytes of the weights, which are on their way (kAhead blocks)
+// before anything else happens.  FUSED: the workgroup quantises its rows of x into LDS itself - no workspace, no second launch; each workgroup repeats
+// that, which pays while there are few workgroups or few rows.
 // Operand order: lane (i = lane & 15, g = lane >> 4) holds columns 16 g .. 16 g + 15 and 64 + 16 g .. of its row's block, the same for both
 // operands: which k a register byte stands for cancels in the sum, and each load instruction covers 64 contiguous bytes of a row.
-template <typename T, int MT, int NT, bool FUSED>
-__global__ __launch_bounds__(512) void linear8_rows_kernel(const T* __restrict__ x, const uint8_t* __restrict__ qx, const uint8_t* __restrict__ ex, const uint8_t* __restrict__ qw,
-                                                           const uint8_t* __restrict__ ew, const T* __restrict__ bias, T* __restrict__ y, int64_t rows, int64_t k, int64_t n) {
+constexpr int rows_ahead(int mt, int nt) { return mt * nt >= 4 ? 2 : 4; }
+template <typename T, int MT, int NT, int WAVES, bool FUSED>
+__global__ __launch_bounds__(64 * WAVES) void linear8_rows_kernel(const T* __restrict__ x, const uint8_t* __restrict__ qx, const uint8_t* __restrict__ ex, const uint8_t* __restrict__ qw,
+                                                                  const uint8_t* __restrict__ ew, const T* __restrict__ bias, T* __restrict__ y, int64_t rows, int64_t k, int64_t n) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];                           // FUSED: rows of kp + 16 bytes, then their scale bytes; later the partial tiles
     constexpr bool kWide = sizeof(T) == 4;
-    __shared__ float part[8][MT * 16][NT * 16 + 1];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
+    constexpr int kAhead = rows_ahead(MT, NT);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
     const int64_t kb = kblocks(k), kp = kb * 128, kbp = kb4(k);
     const int64_t n0 = (int64_t)blockIdx.x * (16 * NT), m0 = (int64_t)blockIdx.y * (16 * MT);
-    f32x4 acc[MT][NT];
-#pragma unroll
-    for (int a = 0; a < MT; ++a)
-#pragma unroll
-        for (int b = 0; b < NT; ++b) acc[a][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int mrows = (int)min((int64_t)(16 * MT), rows - m0);
     const uint8_t* wrow[NT];
     const uint8_t* wexp[NT];
 #pragma unroll
@@ -205,74 +227,111 @@ __global__ __launch_bounds__(512) void linear8_rows_kernel(const T* __restrict__
         wrow[b] = qw + nn * kp + 16 * g;
         wexp[b] = ew + nn / 128 * (FUSED ? kb : kbp);
     }
-    const int64_t mrow = m0 + i;
-    for (int64_t b0 = wave; b0 < kb; b0 += 8) {
-        frag<kWide> wf[NT], xf[MT];
+    v8i wr[kAhead][NT];
+    int we[kAhead][NT];
+    const auto fetch = [&](int64_t b0) {                                                     // (blocks behind the last one read the last one again)
 #pragma unroll
-        for (int b = 0; b < NT; ++b) {
-            const v4i lo = *reinterpret_cast<const v4i*>(wrow[b] + b0 * 128), hi = *reinterpret_cast<const v4i*>(wrow[b] + b0 * 128 + 64);
-            wf[b].set(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), wexp[b][b0]);
+        for (int q = 0; q < kAhead; ++q) {
+            const int64_t bq = min(b0 + WAVES * q, kb - 1);
+#pragma unroll
+            for (int b = 0; b < NT; ++b) {
+                const v4i lo = *reinterpret_cast<const v4i*>(wrow[b] + bq * 128), hi = *reinterpret_cast<const v4i*>(wrow[b] + bq * 128 + 64);
+                wr[q][b] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+                we[q][b] = wexp[b][bq];
+            }
         }
-        if (FUSED) {
-            float v[2][16];
+    };
+    fetch(wave);
+    const int64_t xs = kp + 16;                                                              // row stride in LDS: 16 rows x 16 bytes fall on different banks
+    uint8_t* const xe = lds + mrows * xs;
+    if (FUSED) {
+        const int l16 = threadIdx.x & 15, tasks = mrows * (int)kb;
+        constexpr int kTasks = 2;                                                            // blocks per 16 lanes and round, their loads in front
+        for (int t0 = threadIdx.x >> 4; t0 < tasks; t0 += 4 * WAVES * kTasks) {              // 16 lanes per block of 128, 8 values each
+            nvp_vec<T, 8> raw[kTasks];
+            int at[kTasks];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int64_t c = b0 * 128 + 64 * h + 16 * g;
-                if (mrow < rows && c + 16 <= k) {
-#pragma unroll
-                    for (int p = 0; p < 2; ++p) {
-                        float t[8];
-                        nvp_load<T, 8>(x + mrow * k + c + 8 * p, t);
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) v[h][8 * p + e] = t[e];
-                    }
+            for (int u = 0; u < kTasks; ++u) {
+                const int t = min(t0 + u * 4 * WAVES, tasks - 1), r = t / (int)kb, b = t - r * (int)kb;
+                const int c0 = b * 128 + l16 * 8;
+                at[u] = r * (int)xs + c0;
+                const T* p = x + (m0 + r) * k + c0;
+                if (c0 + 8 <= k) {
+                    raw[u] = nvp_load_raw<T, 8>(p);
                 } else {
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) v[h][e] = mrow < rows && c + e < k ? (float)x[mrow * k + c + e] : 0.f;
+                    for (int e = 0; e < 8; ++e) raw[u].v[e] = c0 + e < k ? p[e] : (T)0.f;
                 }
             }
-            unsigned top = 0u;
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+            for (int u = 0; u < kTasks; ++u) {
+                float v[8];
 #pragma unroll
-                for (int e = 0; e < 16; ++e) top = max(top, finite_bits(v[h][e]));
-            top = max(top, (unsigned)__shfl_xor((int)top, 16));
-            top = max(top, (unsigned)__shfl_xor((int)top, 32));
-            const unsigned byte = scale_byte(top);
-            const float inv = inv_scale(byte);
-            v8i raw;
+                for (int e = 0; e < 8; ++e) v[e] = (float)raw[u].v[e];
+                unsigned byte;
+                const int2 q = quant8(v, byte);
+                const int t = t0 + u * 4 * WAVES;
+                if (t < tasks) {
+                    *reinterpret_cast<int2*>(lds + at[u]) = q;
+                    if (l16 == 0) xe[t] = (uint8_t)byte;
+                }
+            }
+        }
+        __syncthreads();
+    }
+    f32x4 acc[MT][NT];
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+    for (int a = 0; a < MT; ++a)
 #pragma unroll
-                for (int p = 0; p < 4; ++p) raw[4 * h + p] = quant4(&v[h][4 * p], inv);
-            xf[0].set(raw, (int)byte);
-        } else {
+        for (int b = 0; b < NT; ++b) acc[a][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int64_t b0 = wave; b0 < kb; b0 += WAVES * kAhead) {
+        v8i xr[kAhead][MT];
+        int xb[kAhead][MT];
+#pragma unroll
+        for (int q = 0; q < kAhead; ++q) {
+            const int64_t bq = min(b0 + WAVES * q, kb - 1);
 #pragma unroll
             for (int a = 0; a < MT; ++a) {
-                const int64_t mm = min(mrow + 16 * a, rows - 1);
-                const uint8_t* p = qx + mm * kp + b0 * 128 + 16 * g;
+                const int64_t r = min(16 * a + i, mrows - 1);
+                const uint8_t* p = (FUSED ? lds + r * xs : qx + (m0 + r) * kp) + bq * 128 + 16 * g;
                 const v4i lo = *reinterpret_cast<const v4i*>(p), hi = *reinterpret_cast<const v4i*>(p + 64);
-                xf[a].set(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), ex[mm * kbp + b0]);
+                xr[q][a] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+                xb[q][a] = FUSED ? xe[r * kb + bq] : ex[(m0 + r) * kbp + bq];
             }
         }
 #pragma unroll
-        for (int a = 0; a < MT; ++a)
+        for (int q = 0; q < kAhead; ++q) {
+            if (b0 + WAVES * q >= kb) break;
+            frag<kWide> wf[NT];
 #pragma unroll
-            for (int b = 0; b < NT; ++b) acc[a][b] = mma(xf[a], wf[b], acc[a][b]);
+            for (int b = 0; b < NT; ++b) wf[b].set(wr[q][b], we[q][b]);
+#pragma unroll
+            for (int a = 0; a < MT; ++a) {
+                frag<kWide> xf;
+                xf.set(xr[q][a], xb[q][a]);
+#pragma unroll
+                for (int b = 0; b < NT; ++b) acc[a][b] = mma(xf, wf[b], acc[a][b]);
+            }
+        }
+        if (b0 + WAVES * kAhead < kb) fetch(b0 + WAVES * kAhead);
     }
+    // D: row 4 (lane >> 4) + r, column lane & 15
+    constexpr int kStride = NT * 16 + 1;
+    float* const part = reinterpret_cast<float*>(lds);
+    if (FUSED) __syncthreads();                                                              // every wave has read its x
 #pragma unroll
     for (int a = 0; a < MT; ++a)
 #pragma unroll
         for (int b = 0; b < NT; ++b)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) part[wave][16 * a + 4 * g + r][16 * b + i] = acc[a][b][r];      // D: row 4 (lane >> 4) + r, column lane & 15
+            for (int r = 0; r < 4; ++r) part[(wave * MT * 16 + 16 * a + 4 * g + r) * kStride + 16 * b + i] = acc[a][b][r];
     __syncthreads();
-    for (int t = threadIdx.x; t < MT * 16 * NT * 16; t += 512) {
+    for (int t = threadIdx.x; t < MT * 16 * NT * 16; t += 64 * WAVES) {
         const int r = t / (NT * 16), c = t % (NT * 16);
-        if (m0 + r >= rows || n0 + c >= n) continue;
+        if (r >= mrows || n0 + c >= n) continue;
         float s = 0.f;
 #pragma unroll
-        for (int w = 0; w < 8; ++w) s += part[w][r][c];
+        for (int w = 0; w < WAVES; ++w) s += part[(w * MT * 16 + r) * kStride + c];
         if (bias) s += (float)bias[n0 + c];
         y[(m0 + r) * n + n0 + c] = (T)s;
     }
@@ -544,15 +603,29 @@ int launch_tile(const uint8_t* qx, const uint8_t* ex, const uint8_t* qw, const u
     return 0;
 }
 
-template <typename T, int MT, int NT, bool FUSED>
+int64_t rows_lds(int64_t rows, int64_t k) { return rows * (kblocks(k) * 129 + 16); }
+template <typename T, int MT, int NT, int WAVES, bool FUSED>
 int launch_rows(const T* x, const uint8_t* qx, const uint8_t* ex, const uint8_t* qw, const uint8_t* ew, const void* bias, void* y, int64_t rows, int64_t k, int64_t n, hipStream_t st) {
     const int64_t gx = (n + 16 * NT - 1) / (16 * NT), gy = (rows + 16 * MT - 1) / (16 * MT);
     if (gy > 65535 || gx > 0x7fffffff) return NVP_ERR_UNSUPPORTED;
-    hipLaunchKernelGGL((linear8_rows_kernel<T, MT, NT, FUSED>), dim3((unsigned)gx, (unsigned)gy), dim3(512), 0, st, x, qx, ex, qw, ew, (const T*)bias, (T*)y, rows, k, n);
+    const int64_t xbytes = FUSED ? rows_lds(rows < 16 * MT ? rows : 16 * MT, k) : 0, pbytes = WAVES * MT * 16 * (NT * 16 + 1) * 4;
+    hipLaunchKernelGGL((linear8_rows_kernel<T, MT, NT, WAVES, FUSED>), dim3((unsigned)gx, (unsigned)gy), dim3(64 * WAVES), (size_t)(xbytes > pbytes ? xbytes : pbytes), st, x, qx, ex, qw, ew,
+                       (const T*)bias, (T*)y, rows, k, n);
     NVP_LAUNCH_CHECK();
     return 0;
 }
 
+// The path for (rows, k, n); both the workspace query and the call go by it.
+enum { kFew, kNarrow, kRows, kTiles, kTilesBig };
+int narrow_columns(int64_t rows, int64_t k, int64_t n);
+int path_of(int64_t rows, int64_t k, int64_t n) {
+    // up to 64 blocks of x: two per 16 lanes, one round of loads; beyond that a quantising launch of its own is the shorter way (16 rows x 4096 times 4096
+    // columns: 9.3 us with it, 16.4 us without; 1 row: 7.0 us without)
+    if (rows <= 16 && rows * kblocks(k) <= 64) return kFew;
+    if (narrow_columns(rows, k, n)) return kNarrow;
+    if (((rows + 255) / 256) * ((n + 255) / 256) >= 128) return kTilesBig;
+    return rows <= 512 ? kRows : kTiles;
+}
 // columns rounded up to 64, 128 or 256 if that many fit the kernel above with two workgroups per CU, else 0
 int narrow_columns(int64_t rows, int64_t k, int64_t n) {
     const int nt = n <= 64 ? 4 : n <= 128 ? 8 : n <= 256 ? 16 : 0;
@@ -570,13 +643,17 @@ int launch_narrow(const T* x, const uint8_t* qw, const uint8_t* ew, const void* 
 
 template <typename T>
 int linear8(const T* x, const uint8_t* qw, const uint8_t* ew, const void* bias, void* y, int64_t rows, int64_t k, int64_t n, uint8_t* ws, hipStream_t st) {
-    const int64_t kb = kblocks(k), kp = kb * 128, kbp = kb4(k), nb = (n + 127) / 128;
-    if (rows <= 16) return launch_rows<T, 1, 1, true>(x, nullptr, nullptr, qw, ew, bias, y, rows, k, n, st);
-    switch (narrow_columns(rows, k, n)) {
+    const int path = path_of(rows, k, n);
+    // few columns: twice the waves per workgroup, so that the chip still has enough of them
+    if (path == kFew) {
+        return n <= 2048 ? launch_rows<T, 1, 1, 16, true>(x, nullptr, nullptr, qw, ew, bias, y, rows, k, n, st) : launch_rows<T, 1, 1, 8, true>(x, nullptr, nullptr, qw, ew, bias, y, rows, k, n, st);
+    }
+    switch (path == kNarrow ? narrow_columns(rows, k, n) : 0) {
         case 64: return launch_narrow<T, 4>(x, qw, ew, bias, y, rows, k, n, st);
         case 128: return launch_narrow<T, 8>(x, qw, ew, bias, y, rows, k, n, st);
         case 256: return launch_narrow<T, 16>(x, qw, ew, bias, y, rows, k, n, st);
     }
+    const int64_t kb = kblocks(k), kp = kb * 128, kbp = kb4(k), nb = (n + 127) / 128;
     uint8_t* qx = ws;
     uint8_t* ex = qx + rows * kp;
     uint8_t* ewp = ex + rows * kbp;                                                          // rows * kbp is a multiple of 4
@@ -584,9 +661,12 @@ int linear8(const T* x, const uint8_t* qw, const uint8_t* ew, const void* bias, 
     if (groups + tail > 0x7fffffff) return NVP_ERR_UNSUPPORTED;
     hipLaunchKernelGGL((quant_rows_kernel<T>), dim3((unsigned)(groups + tail)), dim3(256), 0, st, x, qx, ex, rows, k, groups, ew, ewp, nb * kbp);
     NVP_LAUNCH_CHECK();
-    const int64_t big = ((rows + 255) / 256) * ((n + 255) / 256);
-    if (big >= 128) return launch_tile<T, 256, 256, 2, 4>(qx, ex, qw, ewp, bias, y, rows, k, n, st);
-    if (rows <= 512) return launch_rows<T, 4, 2, false>(x, qx, ex, qw, ewp, bias, y, rows, k, n, st);
+    if (path == kTilesBig) return launch_tile<T, 256, 256, 2, 4>(qx, ex, qw, ewp, bias, y, rows, k, n, st);
+    if (path == kRows) {
+        if (rows <= 16) return launch_rows<T, 1, 1, 8, false>(x, qx, ex, qw, ewp, bias, y, rows, k, n, st);
+        if (rows <= 32) return launch_rows<T, 2, 2, 8, false>(x, qx, ex, qw, ewp, bias, y, rows, k, n, st);
+        return launch_rows<T, 4, 2, 8, false>(x, qx, ex, qw, ewp, bias, y, rows, k, n, st);
+    }
     return launch_tile<T, 128, 128, 2, 2>(qx, ex, qw, ewp, bias, y, rows, k, n, st);
 }
 
@@ -596,7 +676,8 @@ bool sizes_ok(int64_t rows, int64_t k, int64_t n) { return rows >= 0 && n >= 1 &
 
 extern "C" int64_t nvp_linear8_workspace_bytes(int64_t rows, int64_t k, int64_t n) {
     if (!sizes_ok(rows, k, n)) return NVP_ERR_BADARG;
-    if (rows <= 16 || narrow_columns(rows, k, n)) return 0;
+    const int path = path_of(rows, k, n);
+    if (path == kFew || path == kNarrow) return 0;
     return rows * kblocks(k) * 128 + rows * kb4(k) + (n + 127) / 128 * kb4(k);
 }
 

@@ -97,17 +97,17 @@ def test_refusals_on_the_host():
 def test_entry_points_refuse_bad_arguments_without_a_device():
     lib, d = L.load(), ctypes.c_void_p(64)                          # never dereferenced
     assert lib.nvp_linear8_workspace_bytes(16, 4096, 4096) == 0
-    assert lib.nvp_linear8_workspace_bytes(100, 300, 130) >= 100 * 384 + 100 * 3 + 2 * 3
+    assert lib.nvp_linear8_workspace_bytes(1000, 300, 1130) >= 1000 * 384 + 1000 * 3 + 9 * 3
     assert lib.nvp_linear8_workspace_bytes(-1, 128, 128) == L.ERR_BADARG and lib.nvp_linear8_workspace_bytes(4, 0, 128) == L.ERR_BADARG
-    need = lib.nvp_linear8_workspace_bytes(100, 128, 128)
+    need = lib.nvp_linear8_workspace_bytes(1000, 128, 1128)
     for args in ((None, d, d, d), (d, None, d, d), (d, d, None, d), (d, d, d, None)):
         x, q, e, y = args
-        assert lib.nvp_linear8(x, 0, q, e, None, y, 100, 128, 128, d, need, None) == L.ERR_BADARG
-        assert lib.nvp_linear8(x, 0, q, e, None, y, 0, 128, 128, d, need, None) == 0
-    assert lib.nvp_linear8(d, 3, d, d, None, d, 100, 128, 128, d, need, None) == L.ERR_BADARG             # no such type
-    assert lib.nvp_linear8(d, 0, ctypes.c_void_p(8), d, None, d, 100, 128, 128, d, need, None) == L.ERR_BADARG      # q not 16-byte aligned
-    assert lib.nvp_linear8(d, 0, d, d, None, d, 100, 128, 128, None, need, None) == L.ERR_BADARG
-    assert lib.nvp_linear8(d, 0, d, d, None, d, 100, 128, 128, d, need - 1, None) == L.ERR_BADARG
+        assert lib.nvp_linear8(x, 0, q, e, None, y, 1000, 128, 1128, d, need, None) == L.ERR_BADARG
+        assert lib.nvp_linear8(x, 0, q, e, None, y, 0, 128, 1128, d, need, None) == 0
+    assert lib.nvp_linear8(d, 3, d, d, None, d, 1000, 128, 1128, d, need, None) == L.ERR_BADARG             # no such type
+    assert lib.nvp_linear8(d, 0, ctypes.c_void_p(8), d, None, d, 1000, 128, 1128, d, need, None) == L.ERR_BADARG      # q not 16-byte aligned
+    assert lib.nvp_linear8(d, 0, d, d, None, d, 1000, 128, 1128, None, need, None) == L.ERR_BADARG
+    assert lib.nvp_linear8(d, 0, d, d, None, d, 1000, 128, 1128, d, need - 1, None) == L.ERR_BADARG
     assert lib.nvp_quantize_blocks(d, 0, d, d, 4, 4, 64, None) == L.ERR_BADARG
     assert lib.nvp_quantize_blocks(None, 0, d, d, 4, 4, 1, None) == L.ERR_BADARG
     assert lib.nvp_dequantize_blocks(d, d, None, 0, 4, 4, 1, None) == L.ERR_BADARG
@@ -153,7 +153,7 @@ def test_block_form_at_the_borders():
 
 
 SHAPES = [(1, 1, 1), (1, 128, 16), (2, 130, 17), (16, 4096, 100), (17, 256, 128), (33, 129, 300), (64, 1000, 65), (513, 384, 129), (600, 100, 1000), (700, 640, 4099),
-          (4099, 300, 2050), (1, 1100, 5003), (8, 8192, 256),
+          (4099, 300, 2050), (1, 1100, 5003), (8, 8192, 256), (16, 9000, 40), (9, 16000, 2100), (32, 3000, 50), (300, 4000, 70), (400, 200, 6000), (77, 1100, 5003), (200, 9000, 300),
           (2048, 242, 128), (2049, 1, 1), (2100, 127, 61), (3001, 130, 200), (2500, 300, 65), (5000, 128, 256), (2777, 515, 100)]
 
 
