@@ -10,6 +10,7 @@
 // lost; normal data: 1.5e-5 of the result's rms, whatever K).  That is an order of magnitude below the rounding of a 16-bit y (bf16 1.7e-3,
 // fp16 2e-4 rms), so 16-bit streams take them.  A 32-bit y would show it: fp32 streams widen both operands to bf16 in registers - exact, the
 // scale goes into the exponent (v_cvt_scalef32_pk_bf16_fp8) - and use the bf16 instructions, whose sums are fp32 throughout (2e-7), at half the rate.
+#include <type_traits>
 #include "stream_types.h"
 
 namespace {
@@ -131,7 +132,11 @@ template <bool W> __device__ __forceinline__ void mma2(const frag<W>& a0, const 
 }
 
 // ---- x -> workspace: 16 lanes per block of 128, 8 values each -----------------------------------------------------------------------------
-// q [rows][128 * KB], scales [rows][KB4] (bytes); the launch's last workgroups copy the weights' scales to dword-padded rows [NB][KB4].
+// q: groups of 8 rows, a block's 8 x 128 bytes in one piece ([rows / 8][KB][8][128]: what one load instruction of the tile kernel fetches, 50 bytes per
+// clock and CU against 40 for 8 pieces of 128 and 30 for 16 of 64); scales [rows][KB4] (bytes); the launch's last workgroups copy the weights' scales to
+// dword-padded rows [NB][KB4].
+__host__ __device__ inline int64_t xq_at(int64_t row, int64_t b, int64_t kb) { return ((row >> 3) * kb + b) * 1024 + (row & 7) * 128; }
+__host__ __device__ inline int64_t xq_bytes(int64_t rows, int64_t kb) { return (rows + 7) / 8 * kb * 1024; }
 template <typename T>
 __global__ __launch_bounds__(256) void quant_rows_kernel(const T* __restrict__ x, uint8_t* __restrict__ q, uint8_t* __restrict__ ex, int64_t rows, int64_t k,
                                                          int64_t x_groups, const uint8_t* __restrict__ ew, uint8_t* __restrict__ ew_pad, int64_t ew_bytes) {
@@ -157,7 +162,7 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const T* __restrict__ x
     }
     unsigned byte;
     const int2 p = quant8(v, byte);
-    *reinterpret_cast<int2*>(q + row * kb * 128 + c0) = p;
+    *reinterpret_cast<int2*>(q + xq_at(row, b, kb) + lane16 * 8) = p;
     if (lane16 == 0) ex[row * kb_pad + b] = (uint8_t)byte;
 }
 
@@ -293,7 +298,7 @@ __global__ __launch_bounds__(64 * WAVES) void linear8_rows_kernel(const T* __res
 #pragma unroll
             for (int a = 0; a < MT; ++a) {
                 const int64_t r = min(16 * a + i, mrows - 1);
-                const uint8_t* p = (FUSED ? lds + r * xs : qx + (m0 + r) * kp) + bq * 128 + 16 * g;
+                const uint8_t* p = (FUSED ? lds + r * xs + bq * 128 : qx + xq_at(m0 + r, bq, kb)) + 16 * g;
                 const v4i lo = *reinterpret_cast<const v4i*>(p), hi = *reinterpret_cast<const v4i*>(p + 64);
                 xr[q][a] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
                 xb[q][a] = FUSED ? xe[r * kb + bq] : ex[(m0 + r) * kbp + bq];
@@ -464,15 +469,33 @@ __global__ __launch_bounds__(256, NT <= 8 ? 3 : 2) void linear8_narrow_kernel(co
 }
 
 // ---- many rows: BM x BN tiles through LDS --------------------------------------------------------------------------------------------------
-// Two stages of (BM + BN) x 128 bytes, filled by direct-to-LDS loads one block ahead; a wave computes (BM / WM) x (BN / WN) with
-// 32x32x64 instructions.  LDS rows are 128 bytes; the 16-byte piece c of row r lies at place c ^ (r & 7), so the eight lanes that a
-// 128-byte LDS cycle serves (eight rows, one piece) fall on different banks; the load swizzles on its global side (LDS writes are linear).
-__device__ __forceinline__ void glds16(const void* ubase, unsigned lane_off, unsigned lds_byte) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(lane_off), "s"(ubase), "s"(lds_byte) : "memory");
+// Two stages of one block (128 columns), (BM + BN) x 128 bytes each, filled by direct-to-LDS loads; a wave computes (BM / WM) x (BN / WN) with 32x32x64
+// instructions, half a block at a time.  While one half is multiplied out of registers the next half's operands are read from LDS, and the loads of the
+// stage that has become free are issued between the products.  One barrier per block, in its middle: behind it this block's stage has been read by
+// everyone and is filled with the block after the next, and the next block's stage, filled since the last barrier, is complete.
+// LDS rows are 128 bytes; the 16-byte piece c of row r lies at place c ^ (r >> 1 & 7): of any 16 rows that one 256-byte LDS cycle serves (0 - 15, or
+// 0-3, 12-15, 20-23, 24-27) no two share a bank (measured: no conflicts; with c ^ (r & 7) a third of the LDS cycles were conflicts).  The loads swizzle on
+// their global side (LDS writes are linear).
+template <int AT> __device__ __forceinline__ void glds16(const void* ubase, unsigned lane_off, unsigned lds_byte) {      // to LDS byte lds_byte + AT + 16 lane
+    asm volatile("s_add_u32 m0, %2, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(lane_off), "s"(ubase), "s"(lds_byte), "n"(AT) : "memory", "scc");
 }
-// the stage's loads have landed and every wave is done with the other stage (its LDS reads have returned: lgkmcnt)
-__device__ __forceinline__ void stage_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+__device__ __forceinline__ void glds4(const void* ubase, unsigned lane_off, unsigned lds_byte) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(lane_off), "s"(ubase), "s"(lds_byte) : "memory");
+}
+// every wave's loads have landed and its LDS reads have returned (that wait by the builtin: the compiler then knows, and waits for them no second time)
+__device__ __forceinline__ void stage_barrier() {
+    __builtin_amdgcn_s_waitcnt(0xc07f);      // lgkmcnt(0)
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
 
+template <int A, int B, typename F> __device__ __forceinline__ void static_for(const F& f) {      // f(A) .. f(B - 1), the argument a constant
+    if constexpr (A < B) {
+        f(std::integral_constant<int, A>());
+        static_for<A + 1, B>(f);
+    }
+}
+
+template <int BM, int BN> constexpr int tile_lds() { return 2 * (BM + BN) * 128 + 2 * BM * 4; }
 template <typename T, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN) void linear8_tile_kernel(const uint8_t* __restrict__ qx, const uint8_t* __restrict__ ex, const uint8_t* __restrict__ qw,
                                                                     const uint8_t* __restrict__ ew, const T* __restrict__ bias, T* __restrict__ y, int64_t rows, int64_t k,
@@ -482,10 +505,11 @@ __global__ __launch_bounds__(64 * WM * WN) void linear8_tile_kernel(const uint8_
     constexpr int kWaves = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32;
     constexpr int kStage = (BM + BN) * 128;
     constexpr int kLoads = (BM + BN) / 8 / kWaves;                                           // one load instruction: 8 rows x 128 bytes
-    static_assert((BM + BN) % (8 * kWaves) == 0 && BN / WN <= 128, "tile shape");
+    static_assert((BM + BN) % (16 * kWaves) == 0 && BN / WN <= 128 && BM % 64 == 0 && BM / 64 <= kWaves && kLoads % 2 == 0, "tile shape");
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wm = wave / WN, wn = wave % WN, i = lane & 31, h = lane >> 5;
+    const int wm = wave / WN, wn = wave % WN, i = lane & 31, hl = lane >> 5;
     const int64_t kb = kblocks(k), kp = kb * 128, kbp = kb4(k);
+    const int blocks = (int)kb, quads = (int)(kbp / 4);
 
     // workgroups go to the eight XCDs in turn: give each XCD a contiguous run of tiles, walked in groups of 8 tile rows, so that the
     // tiles an XCD works on at one time share operand rows in its own L2
@@ -499,82 +523,76 @@ __global__ __launch_bounds__(64 * WM * WN) void linear8_tile_kernel(const uint8_
     const int tm = grp * 8 + in % gm, tn = in / gm;
     const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
 
-    // this lane's source rows: row r of the stage is x row m0 + r (r < BM) or weight row n0 + r - BM; beyond the end the last row is read
-    const int lr = lane >> 3, lp = lane & 7, lc = lp ^ lr;
-    const uint8_t* base[kLoads];
+    // Source rows: row r of a stage is x row m0 + r (r < BM) or weight row n0 + r - BM, in groups of 8; a wave's kLoads groups are all of one kind.  Groups
+    // behind the end read the last one; weight rows behind the last one read that row.  (x rows behind the last one are in the workspace, unwritten: what
+    // comes of them is not stored.)  Addresses: one scalar that moves with the block, one offset per lane and group that does not.
+    static_assert(BM / 8 % kLoads == 0, "a wave loads x or weights");
+    const bool isx = wave * kLoads * 8 < BM;
+    const uint8_t* const src = isx ? qx + (m0 >> 3) * (kb * 1024) : qw + n0 * kp;
+    const int advance = isx ? 1024 : 128;
+    const int lr = lane >> 3;
     unsigned off[kLoads];
 #pragma unroll
     for (int q = 0; q < kLoads; ++q) {
-        const int r = (wave * kLoads + q) * 8;                                               // wave-uniform first row: a group of 8 never straddles BM
-        const bool isx = r < BM;
-        const int64_t first = isx ? min(m0 + r, rows - 1) : min(n0 + r - BM, n - 1);
-        const int64_t row = isx ? min(m0 + r + lr, rows - 1) : min(n0 + r - BM + lr, n - 1);
-        base[q] = (isx ? qx : qw) + first * kp;
-        off[q] = (unsigned)((row - first) * kp) + 16u * lc;                                  // < 8 rows * kp: fits 32 bits for every accepted k
+        const int g = wave * kLoads + q;
+        const int64_t row = isx ? min((m0 >> 3) + g, (rows - 1) >> 3) - (m0 >> 3) : min(n0 + 8 * g - BM + lr, n - 1) - n0;
+        const unsigned piece = 16u * ((lane & 7) ^ (lr >> 1) ^ (4 * (q & 1)));               // (row >> 1) & 7 = 4 (group & 1) + (lr >> 1), kLoads is even
+        off[q] = isx ? (unsigned)(row * kb * 1024) + lr * 128u + piece : (unsigned)(row * kp) + piece;      // < BM * kp: the host sees to it that it fits
     }
     const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
-    auto fill = [&](int64_t b, int stage) {
-#pragma unroll
-        for (int q = 0; q < kLoads; ++q) glds16(base[q] + b * 128, off[q], lds0 + stage * kStage + (wave * kLoads + q) * 1024);
+    const auto fill1 = [&](int b, auto q_) {                                                 // (behind the end the last block is fetched again, into a stage that nobody reads)
+        constexpr int q = decltype(q_)::value;
+        glds16<q * 1024>(src + (int64_t)min(b, blocks - 1) * advance, off[q], lds0 + (b & 1) * kStage + wave * kLoads * 1024);
     };
+    // scale dwords of four blocks: a wave fetches those of 64 rows of x, one group of four blocks ahead; two places in turn
+    const int srow = wave % (BM / 64) * 64;
+    const int64_t sfirst = min(m0 + srow, rows - 1);
+    const uint8_t* const sbase = ex + sfirst * kbp;
+    const unsigned soff = (unsigned)(min((int64_t)lane, rows - 1 - sfirst) * kbp);
+    const auto scales1 = [&](int quad) { glds4(sbase + 4 * min(quad, quads - 1), soff, lds0 + 2 * kStage + (quad & 1) * (BM * 4) + srow * 4); };
+    const uint32_t* const wsrc = reinterpret_cast<const uint32_t*>(ew + min((n0 + wn * (BN / WN)) / 128, (n - 1) / 128) * kbp);      // the wave's columns lie in one weight block row
+
     f32x16 acc[TM][TN];
 #pragma unroll
     for (int a = 0; a < TM; ++a)
 #pragma unroll
         for (int b = 0; b < TN; ++b) acc[a][b] = nvp_zero16();
 
-    const int64_t nbl = (n0 + wn * (BN / WN)) / 128;                                         // the wave's columns lie in one weight block row
-    const uint32_t* xsrc[TM];
-#pragma unroll
-    for (int a = 0; a < TM; ++a) xsrc[a] = reinterpret_cast<const uint32_t*>(ex + min(m0 + wm * (BM / WM) + 32 * a + i, rows - 1) * kbp);
-    const uint32_t* wsrc = reinterpret_cast<const uint32_t*>(ew + min(nbl, (n - 1) / 128) * kbp);
-    // a scale dword holds four blocks' bytes; the next dwords are loaded one block ahead, in front of that block's fill, so that the stage
-    // barrier waits for them and no other wait (which would drain the fill in flight) is needed
-    uint32_t xs[TM], wsc, xs_next[TM], wsc_next;
-#pragma unroll
-    for (int a = 0; a < TM; ++a) xs_next[a] = xsrc[a][0];
-    wsc_next = wsrc[0];
-    fill(0, 0);
-    for (int64_t b = 0; b < kb; ++b) {
+    // operands of a half block: 16-byte pieces 4 half + 2 hl and the one behind it, of row i of a 32-row tile
+    const int sw = i >> 1 & 7, xrow = (wm * (BM / WM) + i) * 128, wrow = (BM + wn * (BN / WN) + i) * 128;
+    const auto operand = [&](int b, int half, int row, int t) {
+        const uint8_t* st = lds + (b & 1) * kStage + row + t * 4096;
+        return __builtin_shufflevector(*reinterpret_cast<const v4i*>(st + 16 * ((4 * half + 2 * hl) ^ sw)), *reinterpret_cast<const v4i*>(st + 16 * ((4 * half + 2 * hl + 1) ^ sw)), 0, 1, 2, 3, 4, 5,
+                                       6, 7);
+    };
+    const auto scale = [&](int b, int a) { return *reinterpret_cast<const uint32_t*>(lds + 2 * kStage + (b >> 2 & 1) * (BM * 4) + (wm * (BM / WM) + 32 * a + i) * 4); };
+    scales1(0);
+    static_for<0, kLoads>([&](auto q) { fill1(0, q); });
+#pragma unroll 1
+    for (int b = 0; b < blocks; ++b) {
         stage_barrier();
-        if ((b & 3) == 0) {
+        const int sh = 8 * (b & 3);
+        const uint32_t ws = wsrc[b >> 2];
+        uint32_t xs[TM];
 #pragma unroll
-            for (int a = 0; a < TM; ++a) {
-                asm volatile("" : "+v"(xs_next[a]));
-                xs[a] = xs_next[a];
-            }
-            asm volatile("" : "+v"(wsc_next));
-            wsc = wsc_next;
-        }
-        if ((b & 3) == 3 && b + 1 < kb) {
-#pragma unroll
-            for (int a = 0; a < TM; ++a) xs_next[a] = xsrc[a][(b + 1) >> 2];
-            wsc_next = wsrc[(b + 1) >> 2];
-        }
-        if (b + 1 < kb) fill(b + 1, (int)((b + 1) & 1));
-        const uint8_t* st = lds + (b & 1) * kStage;
-        const int sh = 8 * (int)(b & 3);
-        const int sw = (int)(wsc >> sh);
-#pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
+        for (int a = 0; a < TM; ++a) xs[a] = scale(b, a);
+        static_for<0, kLoads>([&](auto q) { fill1(b + 1, q); });
+        scales1((b >> 2) + 1);
+        static_for<0, 2>([&](auto half_) {
+            constexpr int half = decltype(half_)::value;
             frag<kWide> wf[TN];
 #pragma unroll
-            for (int t = 0; t < TN; ++t) {
-                const int r = BM + wn * (BN / WN) + 32 * t + i, c = 4 * kk + 2 * h;
-                const v4i lo = *reinterpret_cast<const v4i*>(st + r * 128 + 16 * (c ^ (r & 7))), hi = *reinterpret_cast<const v4i*>(st + r * 128 + 16 * ((c + 1) ^ (r & 7)));
-                wf[t].set(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), sw);
-            }
-#pragma unroll
-            for (int a = 0; a < TM; ++a) {
-                const int r = wm * (BM / WM) + 32 * a + i, c = 4 * kk + 2 * h;
-                const v4i lo = *reinterpret_cast<const v4i*>(st + r * 128 + 16 * (c ^ (r & 7))), hi = *reinterpret_cast<const v4i*>(st + r * 128 + 16 * ((c + 1) ^ (r & 7)));
+            for (int t = 0; t < TN; ++t) wf[t].set(operand(b, half, wrow, t), (int)(ws >> sh));
+            static_for<0, TM>([&](auto a_) {
+                constexpr int a = decltype(a_)::value;
                 frag<kWide> xf;
-                xf.set(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), (int)(xs[a] >> sh));
+                xf.set(operand(b, half, xrow, a), (int)(xs[a] >> sh));
 #pragma unroll
                 for (int t = 0; t < TN; ++t) acc[a][t] = mma(xf, wf[t], acc[a][t]);
-            }
-        }
+            });
+        });
     }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                                         // the last fetches, before this LDS can be another workgroup's
 #pragma unroll
     for (int t = 0; t < TN; ++t) {
         const int64_t col = n0 + wn * (BN / WN) + 32 * t + i;
@@ -584,7 +602,7 @@ __global__ __launch_bounds__(64 * WM * WN) void linear8_tile_kernel(const uint8_
         for (int a = 0; a < TM; ++a)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                const int64_t row = m0 + wm * (BM / WM) + 32 * a + nvp_frag_row(r, h);
+                const int64_t row = m0 + wm * (BM / WM) + 32 * a + nvp_frag_row(r, hl);
                 if (row < rows) y[row * n + col] = (T)(acc[a][t][r] + bv);
             }
     }
@@ -593,8 +611,8 @@ __global__ __launch_bounds__(64 * WM * WN) void linear8_tile_kernel(const uint8_
 template <typename T, int BM, int BN, int WM, int WN>
 int launch_tile(const uint8_t* qx, const uint8_t* ex, const uint8_t* qw, const uint8_t* ew, const void* bias, void* y, int64_t rows, int64_t k, int64_t n, hipStream_t st) {
     const int64_t tm = (rows + BM - 1) / BM, tn = (n + BN - 1) / BN;
-    if (tm * tn > 0x3fffffff) return NVP_ERR_UNSUPPORTED;
-    constexpr size_t lds = 2 * (BM + BN) * 128;
+    if (tm * tn > 0x3fffffff || kblocks(k) * 128 * BM > 0xffffffffll || kblocks(k) * 128 * BN > 0xffffffffll) return NVP_ERR_UNSUPPORTED;      // 32-bit offsets inside a tile
+    constexpr size_t lds = tile_lds<BM, BN>();
     // (HIP on gfx950 takes more than 64 KiB of dynamic LDS with or without the attribute: a refusal must not fail the call)
     static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(linear8_tile_kernel<T, BM, BN, WM, WN>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     if (attr != hipSuccess) (void)hipGetLastError();
@@ -624,7 +642,8 @@ int path_of(int64_t rows, int64_t k, int64_t n) {
     if (rows <= 16 && rows * kblocks(k) <= 64) return kFew;
     if (narrow_columns(rows, k, n)) return kNarrow;
     if (((rows + 255) / 256) * ((n + 255) / 256) >= 128) return kTilesBig;
-    return rows <= 512 ? kRows : kTiles;
+    // a rows workgroup reads 64 + 32 operand rows for 64 x 32 results, a tile 128 + 128 for 128 x 128: the tiles win once there are enough of them
+    return rows <= 256 || (rows + 127) / 128 * ((n + 127) / 128) < 64 ? kRows : kTiles;
 }
 // columns rounded up to 64, 128 or 256 if that many fit the kernel above with two workgroups per CU, else 0
 int narrow_columns(int64_t rows, int64_t k, int64_t n) {
@@ -653,9 +672,9 @@ int linear8(const T* x, const uint8_t* qw, const uint8_t* ew, const void* bias, 
         case 128: return launch_narrow<T, 8>(x, qw, ew, bias, y, rows, k, n, st);
         case 256: return launch_narrow<T, 16>(x, qw, ew, bias, y, rows, k, n, st);
     }
-    const int64_t kb = kblocks(k), kp = kb * 128, kbp = kb4(k), nb = (n + 127) / 128;
+    const int64_t kb = kblocks(k), kbp = kb4(k), nb = (n + 127) / 128;
     uint8_t* qx = ws;
-    uint8_t* ex = qx + rows * kp;
+    uint8_t* ex = qx + xq_bytes(rows, kb);
     uint8_t* ewp = ex + rows * kbp;                                                          // rows * kbp is a multiple of 4
     const int64_t groups = (rows * kb + 15) / 16, tail = (nb * kbp + 255) / 256;
     if (groups + tail > 0x7fffffff) return NVP_ERR_UNSUPPORTED;
@@ -663,9 +682,10 @@ int linear8(const T* x, const uint8_t* qw, const uint8_t* ew, const void* bias, 
     NVP_LAUNCH_CHECK();
     if (path == kTilesBig) return launch_tile<T, 256, 256, 2, 4>(qx, ex, qw, ewp, bias, y, rows, k, n, st);
     if (path == kRows) {
+        const bool narrow = (n + 31) / 32 * ((rows + 63) / 64) < 256;                        // 16 columns per workgroup where 32 would leave CUs without one
         if (rows <= 16) return launch_rows<T, 1, 1, 8, false>(x, qx, ex, qw, ewp, bias, y, rows, k, n, st);
-        if (rows <= 32) return launch_rows<T, 2, 2, 8, false>(x, qx, ex, qw, ewp, bias, y, rows, k, n, st);
-        return launch_rows<T, 4, 2, 8, false>(x, qx, ex, qw, ewp, bias, y, rows, k, n, st);
+        if (rows <= 32) return narrow ? launch_rows<T, 2, 1, 8, false>(x, qx, ex, qw, ewp, bias, y, rows, k, n, st) : launch_rows<T, 2, 2, 8, false>(x, qx, ex, qw, ewp, bias, y, rows, k, n, st);
+        return narrow ? launch_rows<T, 4, 1, 8, false>(x, qx, ex, qw, ewp, bias, y, rows, k, n, st) : launch_rows<T, 4, 2, 8, false>(x, qx, ex, qw, ewp, bias, y, rows, k, n, st);
     }
     return launch_tile<T, 128, 128, 2, 2>(qx, ex, qw, ewp, bias, y, rows, k, n, st);
 }
@@ -678,7 +698,7 @@ extern "C" int64_t nvp_linear8_workspace_bytes(int64_t rows, int64_t k, int64_t 
     if (!sizes_ok(rows, k, n)) return NVP_ERR_BADARG;
     const int path = path_of(rows, k, n);
     if (path == kFew || path == kNarrow) return 0;
-    return rows * kblocks(k) * 128 + rows * kb4(k) + (n + 127) / 128 * kb4(k);
+    return xq_bytes(rows, kblocks(k)) + rows * kb4(k) + (n + 127) / 128 * kb4(k);
 }
 
 extern "C" int nvp_linear8(const void* x, int32_t type, const uint8_t* q, const uint8_t* e, const void* bias, void* y, int64_t rows, int64_t k, int64_t n, void* workspace,
