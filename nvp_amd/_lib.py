@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes as C
+import importlib.util
 import math
 import os
 from typing import Optional, Sequence
@@ -209,6 +210,26 @@ def ptr(t: Optional[torch.Tensor], dtype=torch.float32) -> Optional[int]:
     if not t.is_contiguous():
         raise RuntimeError("expected a contiguous tensor")
     return t.data_ptr()
+
+
+_binding = None
+
+
+def binding():
+    """The torch side of the conditioning operators (csrc/binding.cpp), bound to the loaded library.  Raises RuntimeError if it has not been built."""
+    global _binding
+    if _binding is None:
+        path = os.path.join(_HERE, "csrc", "nvp_binding.so")
+        if not os.path.exists(path):
+            raise RuntimeError(f"{path} not found: the binding is not built. Run nvp_amd/csrc/build.sh "
+                               "(or `python -c 'import __graft_entry__ as g; g.build()'`). There is no other path.")
+        load()
+        spec = importlib.util.spec_from_file_location("nvp_binding", path)
+        mod = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(mod)
+        mod.bind(LIB_PATH)
+        _binding = mod
+    return _binding
 
 
 STREAM_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # NVP_F32 / NVP_BF16 / NVP_F16

@@ -8,35 +8,20 @@ The gradient is dense, like the grids': dtable[v] = scale * the sum of dout over
 gradient, and with NVP_CHECK_IDS=1 the call raises instead (a device synchronisation per call)."""
 from __future__ import annotations
 
-import math
+import os
 
 import torch
 from torch import nn
 
 from . import _lib as L
-from . import functional
-from .functional import CodeLookup
 
-_IDS = (torch.int64, torch.int32)
+CHECK_IDS = os.environ.get("NVP_CHECK_IDS", "0") == "1"
 
 
 def lookup(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0, dtype: torch.dtype | None = None) -> torch.Tensor:
     """ids [...] (int64 / int32), table [codes, dim] (fp32 / bf16 / fp16) -> [..., dim] of `dtype` (default: the table's; an fp32 table may be read
-    as bf16 or fp16).  Differentiable with respect to the table, whose gradient has the table's type."""
-    if ids.dtype not in _IDS:
-        raise RuntimeError(f"lookup: ids must be int64 or int32, got {ids.dtype}")
-    if table.dim() != 2 or table.shape[0] < 1 or table.shape[1] < 1:
-        raise RuntimeError(f"lookup: the table must be [codes, dim] with at least one code, got {tuple(table.shape)}")
-    L.stream_type(table, "lookup")
-    dtype = table.dtype if dtype is None else dtype
-    if dtype not in L.STREAM_TYPES or (table.dtype != torch.float32 and dtype != table.dtype):
-        raise RuntimeError(f"lookup: a {table.dtype} table cannot be read as {dtype}")
-    scale = float(scale)
-    if not math.isfinite(scale):
-        raise RuntimeError(f"lookup: scale must be finite, got {scale}")
-    if functional.CHECK_IDS and ids.is_cuda and ids.numel() and int(ids.max()) >= table.shape[0]:
-        raise IndexError(f"lookup: id {int(ids.max())} in a table of {table.shape[0]} codes")
-    return CodeLookup.apply(ids, table, scale, dtype)
+    as bf16 or fp16).  Differentiable with respect to the table, whose gradient has the table's type; differentiable once."""
+    return L.binding().lookup(ids, table, scale, dtype, CHECK_IDS)
 
 
 class CodeTable(nn.Module):

@@ -53,6 +53,20 @@ build_lib() {
 }
 SRC_HASH=$(cat *.hip *.h ../../include/*.h | sha256sum | cut -c1-16)
 
+# nvp_binding.so: the torch side of the conditioning operators (host code; needs torch's headers), in the background of the kernels
+build_binding() {
+  local out=nvp_binding.so
+  if [ -f "$out" ] && [ "$out" -nt binding.cpp ] && [ "$out" -nt ../../include/nvp_hip.h ] && [ "$out" -nt build.sh ] && [ -z "${NVP_REBUILD:-}" ]; then return 0; fi
+  rm -f "$out"
+  local torch_dir py_inc abi
+  read -r torch_dir py_inc abi < <(python3 -c "import os, sysconfig, torch; print(os.path.dirname(torch.__file__), sysconfig.get_paths()['include'], int(torch._C._GLIBCXX_USE_CXX11_ABI))")
+  g++ -O2 -std=c++17 -fPIC -shared -fvisibility=hidden -D__HIP_PLATFORM_AMD__=1 -DUSE_ROCM=1 -DTORCH_API_INCLUDE_EXTENSION_H -D_GLIBCXX_USE_CXX11_ABI="$abi" \
+    -isystem "$torch_dir/include" -isystem "$torch_dir/include/torch/csrc/api/include" -isystem /opt/rocm/include -isystem "$py_inc" binding.cpp \
+    -L"$torch_dir/lib" -lc10 -lc10_hip -ltorch_cpu -ltorch -ltorch_python -ldl -o "$out"
+  echo "built $(pwd)/$out"
+}
+build_binding & BINDING_PID=$!
+
 build_lib libnvp_hip.so obj "" "$SRCS_PRODUCT"
 if [ -z "${NVP_SKIP_TWIN:-}" ]; then
   build_lib libnvp_hip_fp32mfma.so obj_fp32mfma "-DNVP_FWD_B3=0 -DNVP_BWD_B3=0 -DNVP_DW_B3=0" "$SRCS_PRODUCT"
@@ -60,3 +74,4 @@ fi
 if [ -n "${NVP_BUILD_EXPERIMENTS:-}" ]; then
   build_lib libnvp_hip_experiments.so obj_experiments "-DNVP_EXPERIMENTS=1" "$SRCS_EXPERIMENTS"
 fi
+if ! wait "$BINDING_PID"; then echo "build.sh: nvp_binding.so FAILED" >&2; rm -f nvp_binding.so; exit 1; fi

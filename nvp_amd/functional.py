@@ -726,99 +726,3 @@ class NVPFused(torch.autograd.Function):
         _, grads = _mlp_backward(drgb, steps, zt, saved, mlp, n, d, between=scatter, lm=lm, packed=packed_bwd, sink=sink,
                                  chain=None if chain is None else chain[:2])
         return (None, None, d_xy, d_yt, d_xt, d_emb, None, None, None, None, None, None, None, *grads)
-
-
-# --------------------------------------------------------------------------------------
-# Conditioning operators: learned codes by number, the gated residual step with its norms
-# (nvp_amd/codes.py, nvp_amd/trunk.py are the public entry points)
-# --------------------------------------------------------------------------------------
-# NVP_CHECK_IDS=1: every lookup verifies its ids on the host (a device synchronisation per call: for debugging and tests).  Without it an id >= the
-# number of codes gives a row of NaN and no gradient.
-CHECK_IDS = os.environ.get("NVP_CHECK_IDS", "0") == "1"
-
-
-class CodeLookup(torch.autograd.Function):
-    """out[i] = scale * table[ids[i]] and its dense gradient by sorted ids (nvp_lookup_fwd / nvp_lookup_bwd)."""
-
-    @staticmethod
-    def forward(ctx, ids: torch.Tensor, table: torch.Tensor, scale: float, dtype: torch.dtype) -> torch.Tensor:
-        with L.on_device_of(table, ids):
-            ids, table = ids.contiguous(), table.contiguous()
-            codes, dim = table.shape
-            n = ids.numel()
-            out = torch.empty(ids.shape + (dim,), device=table.device, dtype=dtype)
-            L.check(L.load().nvp_lookup_fwd(L.ptr(ids, ids.dtype), int(ids.dtype == torch.int64), L.ptr(table, table.dtype), L.STREAM_TYPES[table.dtype],
-                                            L.ptr(out, dtype), L.STREAM_TYPES[dtype], n, codes, dim, scale, L.stream_ptr()), "nvp_lookup_fwd")
-        ctx.save_for_backward(ids)
-        ctx.shape, ctx.table_dtype, ctx.scale = (codes, dim), table.dtype, scale
-        return out
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dout: torch.Tensor):
-        (ids,) = ctx.saved_tensors
-        codes, dim = ctx.shape
-        with L.on_device_of(dout, ids):
-            lib = L.load()
-            dout = dout.contiguous()
-            n = ids.numel()
-            need = lib.nvp_lookup_bwd_workspace_bytes(n, codes, dim)
-            if need < 0:
-                L.check(int(need), "nvp_lookup_bwd_workspace_bytes")
-            ws = torch.empty(max(need, 16), device=dout.device, dtype=torch.uint8)
-            dtable = torch.empty((codes, dim), device=dout.device, dtype=ctx.table_dtype)
-            L.check(lib.nvp_lookup_bwd(L.ptr(ids, ids.dtype), int(ids.dtype == torch.int64), L.ptr(dout, dout.dtype), L.STREAM_TYPES[dout.dtype], L.ptr(dtable, dtable.dtype),
-                                       L.STREAM_TYPES[ctx.table_dtype], n, codes, dim, ctx.scale, L.ptr(ws, torch.uint8), ws.numel(), L.stream_ptr()), "nvp_lookup_bwd")
-        return None, dtable, None, None
-
-
-class GatedResidual(torch.autograd.Function):
-    """(y, u) of one gated residual step (nvp_residual_fwd / nvp_residual_bwd); h None: u only (the first norm), next None: y only."""
-
-    @staticmethod
-    def forward(ctx, x, h, gate, post, nxt, gate_rows: int, scale: float, gate_act: int, eps: float, grad_mode: bool):
-        with L.on_device_of(x, h, gate, post, nxt):
-            lib = L.load()
-            x, h, gate, post, nxt = (t if t is None else t.contiguous() for t in (x, h, gate, post, nxt))
-            dim = x.shape[-1]
-            rows = x.numel() // dim
-            weight = post if post is not None else nxt
-            p = lambda t: L.ptr(t, t.dtype) if t is not None else None      # noqa: E731
-            a = L.Residual(p(x), p(h), p(gate), p(post), p(nxt), rows, gate_rows, dim, L.STREAM_TYPES[x.dtype], L.STREAM_TYPES[weight.dtype], gate_act, scale, eps)
-            y = torch.empty_like(x) if h is not None else None
-            u = torch.empty_like(x) if nxt is not None else None
-            keep = bool(grad_mode) and any(ctx.needs_input_grad)
-            stats = torch.empty((rows, 2), device=x.device, dtype=torch.float32) if keep else None
-            if rows:
-                L.check(lib.nvp_residual_fwd(C.byref(a), p(y), p(u), p(stats), L.stream_ptr()), "nvp_residual_fwd")
-        if keep:
-            ctx.save_for_backward(x, h, gate, post, nxt, stats)
-            ctx.args = (gate_rows, scale, gate_act, eps)
-        ctx.set_materialize_grads(False)
-        return y, u
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy, du):
-        x, h, gate, post, nxt, stats = ctx.saved_tensors
-        gate_rows, scale, gate_act, eps = ctx.args
-        if dy is None and du is None:
-            return (None,) * 10
-        with L.on_device_of(x, dy, du):
-            lib = L.load()
-            dim = x.shape[-1]
-            rows = x.numel() // dim
-            weight = post if post is not None else nxt
-            p = lambda t: L.ptr(t, t.dtype) if t is not None else None      # noqa: E731
-            dy, du = (t if t is None else t.contiguous() for t in (dy, du))
-            a = L.Residual(p(x), p(h), p(gate), p(post), p(nxt), rows, gate_rows, dim, L.STREAM_TYPES[x.dtype], L.STREAM_TYPES[weight.dtype], gate_act, scale, eps)
-            new = torch.empty_like if rows else torch.zeros_like
-            outs = [new(t) if t is not None and wanted else None for t, wanted in zip((x, h, gate, post, nxt), ctx.needs_input_grad)]
-            if rows == 0:
-                return (*outs, None, None, None, None, None)
-            need = lib.nvp_residual_bwd_workspace_bytes(C.byref(a))
-            if need < 0:
-                L.check(int(need), "nvp_residual_bwd_workspace_bytes")
-            ws = torch.empty(max(need, 16), device=x.device, dtype=torch.uint8)
-            L.check(lib.nvp_residual_bwd(C.byref(a), p(stats), p(dy), p(du), *(p(t) for t in outs), L.ptr(ws, torch.uint8), ws.numel(), L.stream_ptr()), "nvp_residual_bwd")
-        return (*outs, None, None, None, None, None)

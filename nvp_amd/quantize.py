@@ -117,30 +117,7 @@ def linear8(x: torch.Tensor, q: torch.Tensor, e: torch.Tensor, bias: torch.Tenso
     """x [..., K] (fp32 / bf16 / fp16) -> [..., N] of the same type: the linear layer whose weight [N, K] is (q, e) of
     quantize_blocks(weight, 128), on x quantised row by row in blocks of 128 (inside the call); products in 8 bits, sums in fp32, bias of x's
     type added before the one rounding.  A row with an infinity or a NaN gives a row of NaN.  Inference only."""
-    if x.dim() < 1:
-        raise RuntimeError("linear8 expects x [..., K]")
-    k = x.shape[-1]
-    _check_blocks(q, e, k, BLOCK, "linear8")
-    n = q.shape[0]
-    if n < 1:
-        raise RuntimeError("linear8: the weight has no rows")
-    ty = L.stream_type(x, "linear8")
-    if bias is not None and (bias.dtype != x.dtype or tuple(bias.shape) != (n,)):
-        raise RuntimeError(f"linear8: bias must be {x.dtype} [{n}], got {bias.dtype} {tuple(bias.shape)}")
-    if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
-        raise NotImplementedError("linear8 is an inference-only path: call it under torch.no_grad() or on tensors that need no gradient")
-    with L.on_device_of(x, q, e, bias):
-        lib = L.load()
-        xc = x.contiguous()
-        rows = xc.numel() // k
-        y = torch.empty(x.shape[:-1] + (n,), device=x.device, dtype=x.dtype)
-        need = lib.nvp_linear8_workspace_bytes(rows, k, n)
-        if need < 0:
-            L.check(int(need), "nvp_linear8_workspace_bytes")
-        ws = torch.empty(need, device=x.device, dtype=torch.uint8) if need else None
-        L.check(lib.nvp_linear8(L.ptr(xc, x.dtype), ty, L.ptr(q, q.dtype), L.ptr(e, e.dtype), L.ptr(bias.contiguous(), x.dtype) if bias is not None else None,
-                                L.ptr(y, x.dtype), rows, k, n, L.ptr(ws, torch.uint8), need, L.stream_ptr()), "nvp_linear8")
-    return y
+    return L.binding().linear8(x, q, e, bias)
 
 
 class Linear8(nn.Module):

@@ -15,76 +15,27 @@ import torch
 from torch import nn
 
 from . import _lib as L
-from .functional import GatedResidual
 from .quantize import Linear8
 
 _ACTS = {None: 0, "sigmoid": 1}
 MAX_DIM = 8192
 
 
-def _weight(w: torch.Tensor, x: torch.Tensor, what: str) -> None:
-    if tuple(w.shape) != (x.shape[-1],) or w.dtype not in (torch.float32, x.dtype):
-        raise RuntimeError(f"{what}: expected a weight [{x.shape[-1]}] of float32 or {x.dtype}, got {w.dtype} {tuple(w.shape)}")
-
-
-def _stream(x: torch.Tensor, what: str) -> None:
-    L.stream_type(x, what)
-    if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_DIM:
-        raise RuntimeError(f"{what}: expected [..., D] with 1 <= D <= {MAX_DIM}, got {tuple(x.shape)}")
-
-
-def _eps(eps: float, what: str) -> float:
-    eps = float(eps)
-    if not 0.0 <= eps < float("inf"):
-        raise RuntimeError(f"{what}: eps must be finite and not negative, got {eps}")
-    return eps
-
-
-def _gate_rows(x: torch.Tensor, gate: torch.Tensor) -> int:
-    """How many rows of D the gate has; row r of x uses gate row r // (rows of x // rows of the gate): the gate's leading dimensions are x's up to
-    some point and 1 from there on (dimensions missing on the left count as 1)."""
-    lead, got = list(x.shape[:-1]), list(gate.shape[:-1]) if gate.dim() else None
-    ok = got is not None and gate.dtype == x.dtype and gate.shape[-1] == x.shape[-1] and len(got) <= len(lead)
-    if ok:
-        got = [1] * (len(lead) - len(got)) + got
-        k = len(got)
-        while k and got[k - 1] == 1:
-            k -= 1
-        ok = got[:k] == lead[:k]
-    if not ok:
-        raise RuntimeError(f"gated_residual: a gate for x {tuple(x.shape)} ({x.dtype}) has its type and its shape, or 1 in place of the last leading dimensions, "
-                           f"got {gate.dtype} {tuple(gate.shape)}")
-    return gate.numel() // gate.shape[-1]
-
-
 def pre_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6) -> torch.Tensor:
     """x [..., D] -> x / rms(x) * weight, of x's type."""
-    _stream(x, "pre_norm")
-    _weight(weight, x, "pre_norm")
-    return GatedResidual.apply(x, None, None, None, weight, 1, 1.0, 0, _eps(eps, "pre_norm"), torch.is_grad_enabled())[1]
+    return L.binding().pre_norm(x, weight, eps)
 
 
 def gated_residual(x: torch.Tensor, h: torch.Tensor, gate: torch.Tensor | None, post_weight: torch.Tensor, next_weight: torch.Tensor | None = None, scale: float = 1.0,
                    gate_act: str | None = None, eps: float = 1e-6):
     """x, h [..., D] -> y = x + scale * act(gate) * h / rms(h) * post_weight; with `next_weight` (the norm in front of the next block) the pair
     (y, y / rms(y) * next_weight).  gate: None (1), x's shape, or x's shape with 1 in place of the last leading dimensions (one gate row for all the
-    rows below it: [B, 1, D] for x [B, T, D]); gate_act None or 'sigmoid'.  Differentiable with respect to every tensor."""
-    _stream(x, "gated_residual")
-    if h.shape != x.shape or h.dtype != x.dtype:
-        raise RuntimeError(f"gated_residual: h must be like x ({x.dtype} {tuple(x.shape)}), got {h.dtype} {tuple(h.shape)}")
-    _weight(post_weight, x, "gated_residual")
-    if next_weight is not None:
-        _weight(next_weight, x, "gated_residual")
-        if next_weight.dtype != post_weight.dtype:
-            raise RuntimeError(f"gated_residual: the two weights must be of one type, got {post_weight.dtype} and {next_weight.dtype}")
-    if gate_act not in _ACTS:
+    rows below it: [B, 1, D] for x [B, T, D]); gate_act None or 'sigmoid'.  Differentiable (once) with respect to every tensor."""
+    act = _ACTS.get(gate_act)
+    if act is None:
         raise RuntimeError(f"gated_residual: gate_act must be None or 'sigmoid', got {gate_act!r}")
-    scale = float(scale)
-    if scale != scale or scale in (float("inf"), float("-inf")):
-        raise RuntimeError(f"gated_residual: scale must be finite, got {scale}")
-    gate_rows = _gate_rows(x, gate) if gate is not None else 1
-    y, u = GatedResidual.apply(x, h, gate, post_weight, next_weight, gate_rows, scale, _ACTS[gate_act], _eps(eps, "gated_residual"), torch.is_grad_enabled())
-    return y if next_weight is None else (y, u)
+    out = L.binding().gated_residual(x, h, gate, post_weight, next_weight, scale, act, eps)
+    return out[0] if next_weight is None else (out[0], out[1])
 
 
 class Trunk(nn.Module):

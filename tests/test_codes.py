@@ -9,7 +9,7 @@ import pytest
 import torch
 
 from nvp_amd import _lib as L
-from nvp_amd import codes, functional
+from nvp_amd import codes
 
 F32, B16, F16 = torch.float32, torch.bfloat16, torch.float16
 PAIRS = [(F32, F32), (F32, B16), (F32, F16), (B16, B16), (F16, F16)]
@@ -65,7 +65,7 @@ def check(ids, table, scale, dtype):
 
 
 # ---- on the host -------------------------------------------------------------------------------------------------------------------------------
-def test_refusals_on_the_host(monkeypatch):
+def test_refusals_on_the_host():
     ids, table = torch.zeros(3, dtype=torch.int64), torch.zeros(4, 5)
     with pytest.raises(RuntimeError, match="HIP device"):
         codes.lookup(ids, table)
@@ -191,7 +191,7 @@ def test_lookup_non_finite_values_stay_in_their_rows():
 
 @pytest.mark.gpu
 def test_lookup_verifies_ids_on_request(monkeypatch):
-    monkeypatch.setattr(functional, "CHECK_IDS", True)
+    monkeypatch.setattr(codes, "CHECK_IDS", True)
     table = torch.randn(4, 4, device=dev())
     codes.lookup(torch.tensor([3, -1], device=dev()), table)
     with pytest.raises(IndexError, match="id 4 in a table of 4"):

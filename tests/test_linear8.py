@@ -96,7 +96,7 @@ def test_refusals_on_the_host():
 
 def test_entry_points_refuse_bad_arguments_without_a_device():
     lib, d = L.load(), ctypes.c_void_p(64)                          # never dereferenced
-    assert lib.nvp_linear8_workspace_bytes(16, 4096, 4096) == 0
+    assert lib.nvp_linear8_workspace_bytes(2, 4096, 4096) == 0 and lib.nvp_linear8_workspace_bytes(16, 4096, 4096) > 0
     assert lib.nvp_linear8_workspace_bytes(1000, 300, 1130) >= 1000 * 384 + 1000 * 3 + 9 * 3
     assert lib.nvp_linear8_workspace_bytes(-1, 128, 128) == L.ERR_BADARG and lib.nvp_linear8_workspace_bytes(4, 0, 128) == L.ERR_BADARG
     need = lib.nvp_linear8_workspace_bytes(1000, 128, 1128)

@@ -172,8 +172,9 @@ def test_refusals_on_the_host():
         trunk.gated_residual(x, x, None, w, scale=float("inf"))
     with pytest.raises(ValueError):
         trunk.Trunk(8193, 1)
-    for gate, rows in ((x, 6), (torch.zeros(2, 1, 8), 2), (torch.zeros(1, 1, 8), 1), (torch.zeros(8), 1)):
-        assert trunk._gate_rows(x, gate) == rows
+    for gate in (x, torch.zeros(2, 1, 8), torch.zeros(1, 1, 8), torch.zeros(1, 8), torch.zeros(8)):      # taken: what is refused is the device
+        with pytest.raises(RuntimeError, match="HIP device"):
+            trunk.gated_residual(x, x, gate, w, w)
 
 
 def test_entry_points_refuse_bad_arguments_without_a_device():
