@@ -90,44 +90,45 @@ __global__ __launch_bounds__(256) void radix_count_kernel(const I* __restrict__ 
     for (int b = threadIdx.x; b < bins; b += 256) count[(int64_t)blockIdx.x * bins + b] = bin[b];
 }
 
-// count [chunk][digit] -> exclusive prefix over the chunks, total [digit].  A workgroup: 64 digits (lanes) x 16 spans of chunks (waves).
+// count [chunk][digit] -> exclusive prefix over the chunks, total [digit].  A workgroup: 16 digits (lanes) x 64 spans of chunks: a span of 608 chunks is 10
+// reads long, two waits for memory (64 digits x 16 spans: five, 9.6 against 5 us).
 __global__ __launch_bounds__(1024) void radix_scan_kernel(unsigned* __restrict__ count, unsigned* __restrict__ total, int chunks, int bits) {
-    __shared__ unsigned span[16][64];
-    const int bins = 1 << bits, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, b = blockIdx.x * 64 + lane;
-    const int per = (chunks + 15) / 16, c0 = wave * per, c1 = min(c0 + per, chunks);
+    __shared__ unsigned span[64][16], group[4][16];
+    const int bins = 1 << bits, digit = threadIdx.x & 15, s = threadIdx.x >> 4, b = blockIdx.x * 16 + digit;
+    const int per = (chunks + 63) / 64, c0 = min(s * per, chunks), c1 = min(c0 + per, chunks);
     unsigned sum = 0u;
-    if (b < bins) {
-        int c = c0;
-        for (; c + 8 <= c1; c += 8) {
+    if (b < bins)
+        for (int c = c0; c < c1; c += 8) {
             unsigned t[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) t[k] = count[(int64_t)(c + k) * bins + b];
+            for (int k = 0; k < 8; ++k) t[k] = c + k < c1 ? count[(int64_t)(c + k) * bins + b] : 0u;
 #pragma unroll
             for (int k = 0; k < 8; ++k) sum += t[k];
         }
-        for (; c < c1; ++c) sum += count[(int64_t)c * bins + b];
-    }
-    span[wave][lane] = sum;
+    span[s][digit] = sum;
     __syncthreads();
-    unsigned run = 0u;
-    for (int w = 0; w < wave; ++w) run += span[w][lane];
+    if (s < 4) {
+        unsigned g = 0u;
+#pragma unroll
+        for (int w = 0; w < 16; ++w) g += span[s * 16 + w][digit];
+        group[s][digit] = g;
+    }
+    __syncthreads();
     if (b >= bins) return;
-    if (wave == 15) total[b] = run + sum;
-    int c = c0;
-    for (; c + 8 <= c1; c += 8) {
+    unsigned run = 0u;
+    for (int w = 0; w < s >> 4; ++w) run += group[w][digit];
+    for (int w = s & ~15; w < s; ++w) run += span[w][digit];
+    if (s == 63) total[b] = run + sum;
+    for (int c = c0; c < c1; c += 8) {
         unsigned t[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) t[k] = count[(int64_t)(c + k) * bins + b];
+        for (int k = 0; k < 8; ++k) t[k] = c + k < c1 ? count[(int64_t)(c + k) * bins + b] : 0u;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            count[(int64_t)(c + k) * bins + b] = run;
-            run += t[k];
-        }
-    }
-    for (; c < c1; ++c) {
-        const unsigned v = count[(int64_t)c * bins + b];
-        count[(int64_t)c * bins + b] = run;
-        run += v;
+        for (int k = 0; k < 8; ++k)
+            if (c + k < c1) {
+                count[(int64_t)(c + k) * bins + b] = run;
+                run += t[k];
+            }
     }
 }
 
@@ -154,18 +155,23 @@ __global__ __launch_bounds__(256) void radix_scatter_kernel(const I* __restrict_
             p[j] = t.y;
         }
     }
+    unsigned all[kPer], before[kPer], mine[kPer], sum[2] = {0u, 0u};             // a thread's digits: total, number in earlier chunks, number in this one
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+        const int b = threadIdx.x * kPer + e;
+        all[e] = b < bins ? total[b] : 0u;
+        before[e] = b < bins ? count[(int64_t)blockIdx.x * bins + b] : 0u;
+    }
     for (int b = threadIdx.x; b < kWaves << kMaxBits; b += 256) (&cursor[0][0])[b] = 0u;
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < kRounds; ++j)
         if (base + j * 64 + lane < n) atomicAdd(&cursor[wave][(k[j] >> shift) & (bins - 1)], 1u);
     __syncthreads();
-    // a thread's digits: where they start in the output (the totals of all smaller digits + the chunk's place among the chunks) and in this chunk
-    unsigned all[kPer], mine[kPer], sum[2] = {0u, 0u};
+    // where the digits start in the output (the totals of all smaller digits + the chunk's place among the chunks) and in this chunk
 #pragma unroll
     for (int e = 0; e < kPer; ++e) {
         const int b = threadIdx.x * kPer + e;
-        all[e] = b < bins ? total[b] : 0u;
         mine[e] = 0u;
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) mine[e] += cursor[w][b];
@@ -194,7 +200,7 @@ __global__ __launch_bounds__(256) void radix_scatter_kernel(const I* __restrict_
     for (int e = 0; e < kPer; ++e) {
         const int b = threadIdx.x * kPer + e;
         if (b >= bins) break;
-        shift_to[b] = out + count[(int64_t)blockIdx.x * bins + b] - here;
+        shift_to[b] = out + before[e] - here;
         unsigned run = here;
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) {
@@ -542,7 +548,7 @@ int bwd(const I* ids, const S* dout, T* dtable, int64_t n, int64_t codes, int di
             if (p == 0) hipLaunchKernelGGL((radix_count_kernel<I, true>), g, wg, 0, st, ids, buf[at], count, n, codes, shift, P.bits);
             else hipLaunchKernelGGL((radix_count_kernel<I, false>), g, wg, 0, st, ids, buf[at], count, n, codes, shift, P.bits);
             NVP_LAUNCH_CHECK();
-            hipLaunchKernelGGL(radix_scan_kernel, dim3(((1u << P.bits) + 63) / 64), dim3(1024), 0, st, count, total, (int)P.radix_chunks, P.bits);
+            hipLaunchKernelGGL(radix_scan_kernel, dim3(((1u << P.bits) + 15) / 16), dim3(1024), 0, st, count, total, (int)P.radix_chunks, P.bits);
             NVP_LAUNCH_CHECK();
             if (p == 0) hipLaunchKernelGGL((radix_scatter_kernel<I, true>), g, wg, 0, st, ids, buf[at], count, total, buf[at ^ 1], n, codes, shift, P.bits);
             else hipLaunchKernelGGL((radix_scatter_kernel<I, false>), g, wg, 0, st, ids, buf[at], count, total, buf[at ^ 1], n, codes, shift, P.bits);
