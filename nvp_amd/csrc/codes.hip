@@ -15,7 +15,7 @@ namespace {
 
 constexpr unsigned kEmpty = 0xffffffffu, kCarry = 0x80000000u;      // list keys: no entry; the run goes on here, but this entry has no row
 constexpr int kSmall = 4096;                                        // ids sorted in one workgroup
-constexpr int kChunk = 2048, kWaves = 4, kPerWave = kChunk / kWaves; // ids per workgroup of a radix pass
+constexpr int kChunk = 2048, kWaves = 8, kPerWave = kChunk / kWaves; // ids per workgroup of a radix pass
 constexpr int kMaxBits = 10;
 
 // sort key of an id: the id itself, `codes` (behind every table row) for ids that point nowhere
@@ -133,7 +133,7 @@ __global__ __launch_bounds__(1024) void radix_scan_kernel(unsigned* __restrict__
 }
 
 template <typename I, bool FIRST>
-__global__ __launch_bounds__(256) void radix_scatter_kernel(const I* __restrict__ ids, const uint2* __restrict__ in, const unsigned* __restrict__ count,
+__global__ __launch_bounds__(64 * kWaves) void radix_scatter_kernel(const I* __restrict__ ids, const uint2* __restrict__ in, const unsigned* __restrict__ count,
                                                             const unsigned* __restrict__ total, uint2* __restrict__ sorted, int64_t n, int64_t codes, int shift, int bits) {
     __shared__ unsigned cursor[kWaves][1 << kMaxBits];                           // where the wave's next id of a digit goes in `list`
     __shared__ unsigned shift_to[1 << kMaxBits];                                 // place in the output - place in `list`, per digit
@@ -141,7 +141,7 @@ __global__ __launch_bounds__(256) void radix_scatter_kernel(const I* __restrict_
     __shared__ unsigned wsum[2][kWaves];
     const int bins = 1 << bits, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t base = (int64_t)blockIdx.x * kChunk + (int64_t)wave * kPerWave;      // a wave's ids are consecutive: waves in order, rounds in order, lanes in order
-    constexpr int kRounds = kPerWave / 64, kPer = (1 << kMaxBits) / 256;
+    constexpr int kRounds = kPerWave / 64, kPer = (1 << kMaxBits) / (64 * kWaves);
     unsigned k[kRounds], p[kRounds];
 #pragma unroll
     for (int j = 0; j < kRounds; ++j) {
@@ -162,7 +162,7 @@ __global__ __launch_bounds__(256) void radix_scatter_kernel(const I* __restrict_
         all[e] = b < bins ? total[b] : 0u;
         before[e] = b < bins ? count[(int64_t)blockIdx.x * bins + b] : 0u;
     }
-    for (int b = threadIdx.x; b < kWaves << kMaxBits; b += 256) (&cursor[0][0])[b] = 0u;
+    for (int b = threadIdx.x; b < kWaves << kMaxBits; b += 64 * kWaves) (&cursor[0][0])[b] = 0u;
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < kRounds; ++j)
@@ -232,7 +232,7 @@ __global__ __launch_bounds__(256) void radix_scatter_kernel(const I* __restrict_
     __syncthreads();
     // equal digits lie side by side now: their places in the output do too, and neighbouring lanes write them together
     const int len = (int)min((int64_t)kChunk, n - (int64_t)blockIdx.x * kChunk);
-    for (int t = threadIdx.x; t < len; t += 256) {
+    for (int t = threadIdx.x; t < len; t += 64 * kWaves) {
         const uint2 v = list[t];
         sorted[t + shift_to[(v.x >> shift) & (bins - 1)]] = v;
     }
@@ -542,7 +542,7 @@ int bwd(const I* ids, const S* dout, T* dtable, int64_t n, int64_t codes, int di
         NVP_LAUNCH_CHECK();
     } else {
         unsigned *count = (unsigned*)(ws + P.off_count), *total = (unsigned*)(ws + P.off_total);
-        const dim3 g((unsigned)P.radix_chunks), wg(256);
+        const dim3 g((unsigned)P.radix_chunks), wg(256), wide(64 * kWaves);
         for (int p = 0; p < P.passes; ++p) {
             const int shift = p * P.bits;
             if (p == 0) hipLaunchKernelGGL((radix_count_kernel<I, true>), g, wg, 0, st, ids, buf[at], count, n, codes, shift, P.bits);
@@ -550,8 +550,8 @@ int bwd(const I* ids, const S* dout, T* dtable, int64_t n, int64_t codes, int di
             NVP_LAUNCH_CHECK();
             hipLaunchKernelGGL(radix_scan_kernel, dim3(((1u << P.bits) + 15) / 16), dim3(1024), 0, st, count, total, (int)P.radix_chunks, P.bits);
             NVP_LAUNCH_CHECK();
-            if (p == 0) hipLaunchKernelGGL((radix_scatter_kernel<I, true>), g, wg, 0, st, ids, buf[at], count, total, buf[at ^ 1], n, codes, shift, P.bits);
-            else hipLaunchKernelGGL((radix_scatter_kernel<I, false>), g, wg, 0, st, ids, buf[at], count, total, buf[at ^ 1], n, codes, shift, P.bits);
+            if (p == 0) hipLaunchKernelGGL((radix_scatter_kernel<I, true>), g, wide, 0, st, ids, buf[at], count, total, buf[at ^ 1], n, codes, shift, P.bits);
+            else hipLaunchKernelGGL((radix_scatter_kernel<I, false>), g, wide, 0, st, ids, buf[at], count, total, buf[at ^ 1], n, codes, shift, P.bits);
             NVP_LAUNCH_CHECK();
             at ^= 1;
         }
