@@ -469,10 +469,13 @@ __global__ __launch_bounds__(256, NT <= 8 ? 3 : 2) void linear8_narrow_kernel(co
 }
 
 // ---- many rows: BM x BN tiles through LDS --------------------------------------------------------------------------------------------------
-// Two stages of one block (128 columns), (BM + BN) x 128 bytes each, filled by direct-to-LDS loads; a wave computes (BM / WM) x (BN / WN) with 32x32x64
-// instructions, half a block at a time.  While one half is multiplied out of registers the next half's operands are read from LDS, and the loads of the
-// stage that has become free are issued between the products.  One barrier per block, in its middle: behind it this block's stage has been read by
-// everyone and is filled with the block after the next, and the next block's stage, filled since the last barrier, is complete.
+// A ring of STAGES blocks (128 columns), (BM + BN) x 128 bytes each, filled by direct-to-LDS loads STAGES - 1 blocks ahead; a wave computes
+// (BM / WM) x (BN / WN) with 32x32x64 instructions.  One barrier per block, at its start: behind it the block has landed for everyone (every wave waits for
+// its own loads, counted: those of later blocks stay in flight) and the stage of the block before has been read, so that its refill is issued at once.
+// The scales come through LDS too: a load into registers would be waited for together with all fills before it.
+// Measured, with the quantising launch: 8192 x 8192 x 8192 bf16 489 us, 2.25 PFLOP/s (the 256 x 256 tile; the matrix units are busy 57 - 60 % of the cycles of a
+// clock that their power holds at 1.8 - 2.0 GHz of 2.4: finer interleaving of loads, reads and products, in 4 or 8 waves, was not faster); 256 x 4096 x 4096
+// 15.3 us (the 64 x 64 tile, bound by the bytes through LDS: 128 MB; splitting a tile's blocks over two or four teams of waves was not faster).
 // LDS rows are 128 bytes; the 16-byte piece c of row r lies at place c ^ (r >> 1 & 7): of any 16 rows that one 256-byte LDS cycle serves (0 - 15, or
 // 0-3, 12-15, 20-23, 24-27) no two share a bank (measured: no conflicts; with c ^ (r & 7) a third of the LDS cycles were conflicts).  The loads swizzle on
 // their global side (LDS writes are linear).
@@ -483,9 +486,10 @@ __device__ __forceinline__ void glds4(const void* ubase, unsigned lane_off, unsi
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(lane_off), "s"(ubase), "s"(lds_byte) : "memory");
 }
 // every wave's loads have landed and its LDS reads have returned (that wait by the builtin: the compiler then knows, and waits for them no second time)
-__device__ __forceinline__ void stage_barrier() {
+template <int LATER> __device__ __forceinline__ void stage_barrier() {
+    static_assert(LATER < 64, "vmcnt");
     __builtin_amdgcn_s_waitcnt(0xc07f);      // lgkmcnt(0)
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LATER) : "memory");
 }
 
 template <int A, int B, typename F> __device__ __forceinline__ void static_for(const F& f) {      // f(A) .. f(B - 1), the argument a constant
@@ -495,21 +499,21 @@ template <int A, int B, typename F> __device__ __forceinline__ void static_for(c
     }
 }
 
-template <int BM, int BN> constexpr int tile_lds() { return 2 * (BM + BN) * 128 + 2 * BM * 4; }
-template <typename T, int BM, int BN, int WM, int WN>
+template <int BM, int BN, int STAGES> constexpr int tile_lds() { return STAGES * (BM + BN) * 128 + (STAGES > 2 ? 4 : 2) * BM * 4; }
+template <typename T, int BM, int BN, int WM, int WN, int STAGES>
 __global__ __launch_bounds__(64 * WM * WN) void linear8_tile_kernel(const uint8_t* __restrict__ qx, const uint8_t* __restrict__ ex, const uint8_t* __restrict__ qw,
                                                                     const uint8_t* __restrict__ ew, const T* __restrict__ bias, T* __restrict__ y, int64_t rows, int64_t k,
                                                                     int64_t n, int tiles_m, int tiles_n) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     constexpr bool kWide = sizeof(T) == 4;
     constexpr int kWaves = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32;
-    constexpr int kStage = (BM + BN) * 128;
+    constexpr int kStage = (BM + BN) * 128, kPlaces = STAGES > 2 ? 4 : 2;
     constexpr int kLoads = (BM + BN) / 8 / kWaves;                                           // one load instruction: 8 rows x 128 bytes
-    static_assert((BM + BN) % (16 * kWaves) == 0 && BN / WN <= 128 && BM % 64 == 0 && BM / 64 <= kWaves && kLoads % 2 == 0, "tile shape");
+    static_assert(STAGES <= 5 && (BM + BN) % (16 * kWaves) == 0 && BN / WN <= 128 && BM % 64 == 0 && BM / 64 <= kWaves && kLoads % 2 == 0, "tile shape");
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WN, wn = wave % WN, i = lane & 31, hl = lane >> 5;
     const int64_t kb = kblocks(k), kp = kb * 128, kbp = kb4(k);
-    const int blocks = (int)kb, quads = (int)(kbp / 4);
+    const int blocks = (int)kb;
 
     // workgroups go to the eight XCDs in turn: give each XCD a contiguous run of tiles, walked in groups of 8 tile rows, so that the
     // tiles an XCD works on at one time share operand rows in its own L2
@@ -520,7 +524,7 @@ __global__ __launch_bounds__(64 * WM * WN) void linear8_tile_kernel(const uint8_
         id = xcd * per + min(xcd, more) + at;
     }
     const int gsz = 8 * tiles_n, grp = id / gsz, in = id - grp * gsz, gm = min(8, tiles_m - grp * 8);
-    const int tm = grp * 8 + in % gm, tn = in / gm;
+    const int tm = __builtin_amdgcn_readfirstlane(grp * 8 + in % gm), tn = __builtin_amdgcn_readfirstlane(in / gm);
     const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
 
     // Source rows: row r of a stage is x row m0 + r (r < BM) or weight row n0 + r - BM, in groups of 8; a wave's kLoads groups are all of one kind.  Groups
@@ -539,17 +543,19 @@ __global__ __launch_bounds__(64 * WM * WN) void linear8_tile_kernel(const uint8_
         const unsigned piece = 16u * ((lane & 7) ^ (lr >> 1) ^ (4 * (q & 1)));               // (row >> 1) & 7 = 4 (group & 1) + (lr >> 1), kLoads is even
         off[q] = isx ? (unsigned)(row * kb * 1024) + lr * 128u + piece : (unsigned)(row * kp) + piece;      // < BM * kp: the host sees to it that it fits
     }
-    const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
+    const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;      // STAGES x operands, kPlaces x scales
     const auto fill1 = [&](int b, auto q_) {                                                 // (behind the end the last block is fetched again, into a stage that nobody reads)
         constexpr int q = decltype(q_)::value;
-        glds16<q * 1024>(src + (int64_t)min(b, blocks - 1) * advance, off[q], lds0 + (b & 1) * kStage + wave * kLoads * 1024);
+        glds16<q * 1024>(src + (int64_t)min(b, blocks - 1) * advance, off[q], lds0 + (unsigned)b % STAGES * kStage + wave * kLoads * 1024);
     };
-    // scale dwords of four blocks: a wave fetches those of 64 rows of x, one group of four blocks ahead; two places in turn
+    // Scale dwords of four blocks: with block j a wave fetches group (j + 3) / 4 for 64 rows of x, so that the fetches in flight can be counted and a group's first
+    // fetch is four blocks old when it is read (the block's own group: 8192 x 8192 x 8192 3 % slower).  Block b reads group b / 4; fetches on their way are for
+    // groups up to (b + STAGES + 2) / 4: one behind it with two stages, two with up to five.
     const int srow = wave % (BM / 64) * 64;
     const int64_t sfirst = min(m0 + srow, rows - 1);
     const uint8_t* const sbase = ex + sfirst * kbp;
     const unsigned soff = (unsigned)(min((int64_t)lane, rows - 1 - sfirst) * kbp);
-    const auto scales1 = [&](int quad) { glds4(sbase + 4 * min(quad, quads - 1), soff, lds0 + 2 * kStage + (quad & 1) * (BM * 4) + srow * 4); };
+    const auto scales1 = [&](int b) { glds4(sbase + 4 * min((b + 3) >> 2, (blocks - 1) >> 2), soff, lds0 + STAGES * kStage + ((b + 3) >> 2) % kPlaces * (BM * 4) + srow * 4); };
     const uint32_t* const wsrc = reinterpret_cast<const uint32_t*>(ew + min((n0 + wn * (BN / WN)) / 128, (n - 1) / 128) * kbp);      // the wave's columns lie in one weight block row
 
     f32x16 acc[TM][TN];
@@ -561,23 +567,26 @@ __global__ __launch_bounds__(64 * WM * WN) void linear8_tile_kernel(const uint8_
     // operands of a half block: 16-byte pieces 4 half + 2 hl and the one behind it, of row i of a 32-row tile
     const int sw = i >> 1 & 7, xrow = (wm * (BM / WM) + i) * 128, wrow = (BM + wn * (BN / WN) + i) * 128;
     const auto operand = [&](int b, int half, int row, int t) {
-        const uint8_t* st = lds + (b & 1) * kStage + row + t * 4096;
+        const uint8_t* st = lds + (unsigned)b % STAGES * kStage + row + t * 4096;
         return __builtin_shufflevector(*reinterpret_cast<const v4i*>(st + 16 * ((4 * half + 2 * hl) ^ sw)), *reinterpret_cast<const v4i*>(st + 16 * ((4 * half + 2 * hl + 1) ^ sw)), 0, 1, 2, 3, 4, 5,
                                        6, 7);
     };
-    const auto scale = [&](int b, int a) { return *reinterpret_cast<const uint32_t*>(lds + 2 * kStage + (b >> 2 & 1) * (BM * 4) + (wm * (BM / WM) + 32 * a + i) * 4); };
-    scales1(0);
-    static_for<0, kLoads>([&](auto q) { fill1(0, q); });
+    const auto scale = [&](int b, int a) { return *reinterpret_cast<const uint32_t*>(lds + STAGES * kStage + (b >> 2) % kPlaces * (BM * 4) + (wm * (BM / WM) + 32 * a + i) * 4); };
+    static_for<0, STAGES - 1>([&](auto b) {
+        static_for<0, kLoads>([&](auto q) { fill1(b, q); });
+        scales1(b);
+    });
 #pragma unroll 1
     for (int b = 0; b < blocks; ++b) {
-        stage_barrier();
+        stage_barrier<(STAGES - 2) * (kLoads + 1)>();
         const int sh = 8 * (b & 3);
         const uint32_t ws = wsrc[b >> 2];
         uint32_t xs[TM];
 #pragma unroll
         for (int a = 0; a < TM; ++a) xs[a] = scale(b, a);
-        static_for<0, kLoads>([&](auto q) { fill1(b + 1, q); });
-        scales1((b >> 2) + 1);
+        static_for<0, kLoads>([&](auto q) { fill1(b + STAGES - 1, q); });
+        scales1(b + STAGES - 1);
+        __builtin_amdgcn_sched_barrier(0);                                                   // nothing waits for the scales before all loads are on their way
         static_for<0, 2>([&](auto half_) {
             constexpr int half = decltype(half_)::value;
             frag<kWide> wf[TN];
@@ -608,15 +617,15 @@ __global__ __launch_bounds__(64 * WM * WN) void linear8_tile_kernel(const uint8_
     }
 }
 
-template <typename T, int BM, int BN, int WM, int WN>
+template <typename T, int BM, int BN, int WM, int WN, int STAGES>
 int launch_tile(const uint8_t* qx, const uint8_t* ex, const uint8_t* qw, const uint8_t* ew, const void* bias, void* y, int64_t rows, int64_t k, int64_t n, hipStream_t st) {
     const int64_t tm = (rows + BM - 1) / BM, tn = (n + BN - 1) / BN;
     if (tm * tn > 0x3fffffff || kblocks(k) * 128 * BM > 0xffffffffll || kblocks(k) * 128 * BN > 0xffffffffll) return NVP_ERR_UNSUPPORTED;      // 32-bit offsets inside a tile
-    constexpr size_t lds = tile_lds<BM, BN>();
+    constexpr size_t lds = tile_lds<BM, BN, STAGES>();
     // (HIP on gfx950 takes more than 64 KiB of dynamic LDS with or without the attribute: a refusal must not fail the call)
-    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(linear8_tile_kernel<T, BM, BN, WM, WN>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(linear8_tile_kernel<T, BM, BN, WM, WN, STAGES>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     if (attr != hipSuccess) (void)hipGetLastError();
-    hipLaunchKernelGGL((linear8_tile_kernel<T, BM, BN, WM, WN>), dim3((unsigned)(tm * tn)), dim3(64 * WM * WN), lds, st, qx, ex, qw, ew, (const T*)bias, (T*)y, rows, k, n, (int)tm, (int)tn);
+    hipLaunchKernelGGL((linear8_tile_kernel<T, BM, BN, WM, WN, STAGES>), dim3((unsigned)(tm * tn)), dim3(64 * WM * WN), lds, st, qx, ex, qw, ew, (const T*)bias, (T*)y, rows, k, n, (int)tm, (int)tn);
     NVP_LAUNCH_CHECK();
     return 0;
 }
@@ -634,16 +643,22 @@ int launch_rows(const T* x, const uint8_t* qx, const uint8_t* ex, const uint8_t*
 }
 
 // The path for (rows, k, n); both the workspace query and the call go by it.
-enum { kFew, kNarrow, kRows, kTiles, kTilesBig };
+enum { kFew, kNarrow, kRows, kTiles64, kTiles128, kTiles128x2, kTiles256 };
 int narrow_columns(int64_t rows, int64_t k, int64_t n);
 int path_of(int64_t rows, int64_t k, int64_t n) {
     // up to 64 blocks of x: two per 16 lanes, one round of loads; beyond that a quantising launch of its own is the shorter way (16 rows x 4096 times 4096
     // columns: 9.3 us with it, 16.4 us without; 1 row: 7.0 us without)
     if (rows <= 16 && rows * kblocks(k) <= 64) return kFew;
     if (narrow_columns(rows, k, n)) return kNarrow;
-    if (((rows + 255) / 256) * ((n + 255) / 256) >= 128) return kTilesBig;
-    // a rows workgroup reads 64 + 32 operand rows for 64 x 32 results, a tile 128 + 128 for 128 x 128: the tiles win once there are enough of them
-    return rows <= 256 || (rows + 127) / 128 * ((n + 127) / 128) < 64 ? kRows : kTiles;
+    // bf16, 4096 x 4096 weights, us with the quantising launch, for the rows kernel / 64 x 64 tiles / 128 x 128 tiles one per CU / two per CU / 256 x 256:
+    // 32 rows 12.3 / 13 / 21 / 25 / 48;  64 rows 18 / 13.5 / 21 / 26 / 48;  512 rows - / 26 / 26 / 32 / 54;  1024 rows - / 44 / 30 / 35 / 56;
+    // 2048 rows - / 79 / 56 / 46 / 60;  4096 rows - / 146 / 103 / 87 / 76: the smallest tile that still runs in one round of the chip (two
+    // workgroups per CU where their LDS allows it), and the largest, which reads the least, for what takes more rounds than that
+    if (rows <= 32) return kRows;
+    const auto tiles = [&](int64_t b) { return ((rows + b - 1) / b) * ((n + b - 1) / b); };
+    if (tiles(64) <= 512) return kTiles64;
+    if (tiles(128) <= 256) return kTiles128;
+    return tiles(128) <= 512 ? kTiles128x2 : kTiles256;
 }
 // columns rounded up to 64, 128 or 256 if that many fit the kernel above with two workgroups per CU, else 0
 int narrow_columns(int64_t rows, int64_t k, int64_t n) {
@@ -680,14 +695,17 @@ int linear8(const T* x, const uint8_t* qw, const uint8_t* ew, const void* bias, 
     if (groups + tail > 0x7fffffff) return NVP_ERR_UNSUPPORTED;
     hipLaunchKernelGGL((quant_rows_kernel<T>), dim3((unsigned)(groups + tail)), dim3(256), 0, st, x, qx, ex, rows, k, groups, ew, ewp, nb * kbp);
     NVP_LAUNCH_CHECK();
-    if (path == kTilesBig) return launch_tile<T, 256, 256, 2, 4>(qx, ex, qw, ewp, bias, y, rows, k, n, st);
-    if (path == kRows) {
-        const bool narrow = (n + 31) / 32 * ((rows + 63) / 64) < 256;                        // 16 columns per workgroup where 32 would leave CUs without one
-        if (rows <= 16) return launch_rows<T, 1, 1, 8, false>(x, qx, ex, qw, ewp, bias, y, rows, k, n, st);
-        if (rows <= 32) return narrow ? launch_rows<T, 2, 1, 8, false>(x, qx, ex, qw, ewp, bias, y, rows, k, n, st) : launch_rows<T, 2, 2, 8, false>(x, qx, ex, qw, ewp, bias, y, rows, k, n, st);
-        return narrow ? launch_rows<T, 4, 1, 8, false>(x, qx, ex, qw, ewp, bias, y, rows, k, n, st) : launch_rows<T, 4, 2, 8, false>(x, qx, ex, qw, ewp, bias, y, rows, k, n, st);
+    switch (path) {
+        case kRows: {
+            const bool narrow = (n + 31) / 32 < 256;                                         // 16 columns per workgroup where 32 would leave CUs without one
+            if (rows <= 16) return launch_rows<T, 1, 1, 8, false>(x, qx, ex, qw, ewp, bias, y, rows, k, n, st);
+            return narrow ? launch_rows<T, 2, 1, 8, false>(x, qx, ex, qw, ewp, bias, y, rows, k, n, st) : launch_rows<T, 2, 2, 8, false>(x, qx, ex, qw, ewp, bias, y, rows, k, n, st);
+        }
+        case kTiles64: return launch_tile<T, 64, 64, 2, 2, 4>(qx, ex, qw, ewp, bias, y, rows, k, n, st);
+        case kTiles128: return launch_tile<T, 128, 128, 4, 2, 4>(qx, ex, qw, ewp, bias, y, rows, k, n, st);
+        case kTiles128x2: return launch_tile<T, 128, 128, 2, 2, 2>(qx, ex, qw, ewp, bias, y, rows, k, n, st);
+        default: return launch_tile<T, 256, 256, 2, 4, 2>(qx, ex, qw, ewp, bias, y, rows, k, n, st);
     }
-    return launch_tile<T, 128, 128, 2, 2>(qx, ex, qw, ewp, bias, y, rows, k, n, st);
 }
 
 bool sizes_ok(int64_t rows, int64_t k, int64_t n) { return rows >= 0 && n >= 1 && k >= 1 && rows <= (1ll << 31) - 1 && n <= (1ll << 31) - 1 && k <= (1ll << 24); }
