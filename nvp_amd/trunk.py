@@ -59,8 +59,8 @@ class Trunk(nn.Module):
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         u = pre_norm(x, self.norms[0], self.eps)
         for k in range(self.depth):
-            h = self.downs[k](self.act(self.ups[k](u)))
-            x, u = gated_residual(x, h, self.gates[k](u), self.posts[k], self.norms[k + 1], self.scale, "sigmoid", self.eps)
+            h = self.downs[k](self.act(self.ups[k](u))).to(x.dtype)                   # (under autocast the linear layers answer in its type)
+            x, u = gated_residual(x, h, self.gates[k](u).to(x.dtype), self.posts[k], self.norms[k + 1], self.scale, "sigmoid", self.eps)
         return u
 
     @torch.no_grad()

@@ -258,3 +258,58 @@ def test_code_table_trains_with_the_one_launch_optimizer():
     opt.step()
     moved = (m.codes.detach() - before).abs().amax(1)
     assert bool((moved[:20] > 0).all()) and bool((moved[20:] <= 1e-2 * 1e-2 * 1e-4 * 1.01).all())   # rows no id points to only decay
+
+
+@pytest.mark.gpu
+def test_lookup_is_differentiable_once_and_guards_what_it_saved():
+    table = torch.randn(9, 5, device=dev(), requires_grad=True)
+    ids = torch.tensor([1, 1, 8, -1], device=dev())
+    out = codes.lookup(ids, table)
+    dout = torch.ones_like(out, requires_grad=True)
+    g, = torch.autograd.grad(out, table, dout, create_graph=True)
+    assert torch.equal(g.detach()[1], torch.full((5,), 2.0, device=dev()))
+    with pytest.raises(RuntimeError, match="once"):
+        g.sum().backward()
+    out = codes.lookup(ids, table)
+    first, = torch.autograd.grad(out.sum(), table, retain_graph=True)
+    second, = torch.autograd.grad(out.sum(), table)
+    assert torch.equal(first, second)
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(out.sum(), table)
+    out = codes.lookup(ids, table)
+    ids.fill_(0)                                                    # the ids belong to the recorded call
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        torch.autograd.grad(out.sum(), table)
+    with torch.inference_mode():
+        assert not codes.lookup(ids, table).requires_grad
+    with pytest.raises(RuntimeError, match="HIP device"):
+        codes.lookup(ids.cpu(), table)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,n_codes", [(4097, 3), (10000, 1), (20000, 1 << 20), (300000, 600)])
+def test_lookup_gradient_bits_of_the_sort(n, n_codes):
+    """Integers: sums are exact whatever their order, so every row has to come out right to the bit - one digit, two and three of them."""
+    g = torch.Generator().manual_seed(n)
+    ids = torch.randint(-1, n_codes, (n,), generator=g).to(dev())
+    dout = torch.randint(-8, 9, (n, 8), generator=g).float().to(dev())
+    t = torch.zeros(n_codes, 8, device=dev(), requires_grad=True)
+    got, = torch.autograd.grad(codes.lookup(ids, t), t, dout)
+    want, _, _ = plain_grad(ids, dout, n_codes, 1.0)
+    assert torch.equal(got.cpu().double(), want)
+
+
+@pytest.mark.gpu
+def test_lookup_offsets_past_32_bits():
+    """2.2e9 values out and back: integers below 2^24 in 32-bit sums, so the gradient is exact before its one rounding."""
+    n, n_codes, dim = 2_200_000, 300, 1000
+    ids = torch.randint(0, n_codes, (n,), device=dev())
+    table = torch.randn(n_codes, dim, device=dev(), dtype=B16, requires_grad=True)
+    out = codes.lookup(ids, table)
+    assert all(torch.equal(out[a:a + 1000], table.detach()[ids[a:a + 1000]]) for a in (0, 2_147_400, n - 1000))
+    dout = torch.randn(n, dim, device=dev(), dtype=B16).round_()
+    got, = torch.autograd.grad(out, table, dout)
+    want = torch.zeros(n_codes, dim, device=dev(), dtype=torch.float64)
+    for a in range(0, n, 200_000):
+        want.index_add_(0, ids[a:a + 200_000], dout[a:a + 200_000].double())
+    assert torch.equal(got, want.to(B16))

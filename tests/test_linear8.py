@@ -269,3 +269,43 @@ def test_linear8_two_streams_at_once():
                 got.append((i, Q.linear8(x[i], q, e)))
     torch.cuda.synchronize()
     assert all(torch.equal(y, want[i]) for i, y in got)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,k,n", [(20, 300, 8200), (33, 640, 70), (65, 129, 8191), (511, 1300, 4100), (1500, 700, 4100), (4200, 1300, 2300)])
+def test_linear8_every_tile(m, k, n, dtype):
+    """32 columns a workgroup; 64 x 64 tiles, full and ragged; 128 x 128 with one and with two tiles per CU; 256 x 256 with more blocks than stages."""
+    test_linear8(m, k, n, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n", [(40, 500), (511, 4100), (1500, 4100), (20, 8200)])
+def test_linear8_captured_tiles(m, n):
+    k = 1300
+    x, w = torch.randn(m, k, device=dev()), torch.randn(n, k, device=dev())
+    q, e = Q.quantize_blocks(w, 128)
+    Q.linear8(x, q, e)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = Q.linear8(x, q, e)
+    for _ in range(3):
+        x.copy_(torch.randn(m, k, device=dev()))
+        graph.replay()
+        want = Q.linear8(x, q, e)
+        torch.cuda.synchronize()
+        assert torch.equal(y, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,k,n", [(1_100_000, 2048, 300), (9_000_000, 256, 250)])
+def test_linear8_offsets_past_32_bits(m, k, n):
+    x = torch.randn(m, k, device=dev(), dtype=torch.bfloat16)
+    w = torch.randn(n, k) * k ** -0.5
+    q, e = Q.quantize_blocks(w.to(dev()), 128)
+    y = Q.linear8(x, q, e)
+    for a in (0, 2 ** 31 // k - 20, 2 ** 31 // n - 20, m - 40):
+        a = min(a, m - 40)
+        want, s = plain_linear(x[a:a + 40].cpu(), w, None)
+        within(y[a:a + 40], want, s, k, torch.bfloat16)

@@ -456,3 +456,72 @@ def test_trunk_in_eight_bits():
     other.load_state_dict(eight.state_dict())
     with torch.no_grad():
         assert torch.equal(other(x), eight(x))
+
+
+@pytest.mark.gpu
+def test_residual_is_differentiable_once_and_guards_what_it_saved():
+    leaf, seeds = make((6, 40), F32, F32, "both", (6, 40), 3)
+    mine = {k: v.requires_grad_(True) for k, v in leaf.items()}
+    y, u = call(mine, 0.5, "sigmoid", 1e-6)
+    g, = torch.autograd.grad((y, u), mine["x"], seeds, create_graph=True)
+    with pytest.raises(RuntimeError, match="once"):
+        g.sum().backward()
+    y, u = call(mine, 0.5, "sigmoid", 1e-6)
+    a = torch.autograd.grad((y, u), mine["h"], seeds, retain_graph=True)
+    assert torch.equal(a[0], torch.autograd.grad((y, u), mine["h"], seeds)[0])
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad((y, u), mine["h"], seeds)
+    h = mine["h"].detach().clone()
+    y, u = trunk.gated_residual(mine["x"], h, None, mine["post"], mine["next"])
+    h.zero_()
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        torch.autograd.grad((y, u), mine["x"], seeds)
+    with pytest.raises(RuntimeError, match="HIP device"):
+        trunk.gated_residual(mine["x"], mine["h"], None, mine["post"].cpu())
+
+
+@pytest.mark.gpu
+def test_residual_with_one_tensor_in_several_places():
+    """x as its own block output and gate, one weight for both norms: the gradients of the places add up."""
+    g = torch.Generator().manual_seed(5)
+    x, w = torch.randn(33, 260, generator=g), 1 + 0.2 * torch.randn(260, generator=g)
+    seeds = [torch.randn(33, 260, generator=g) for _ in range(2)]
+    mx, mw = x.to(dev()).requires_grad_(True), w.to(dev()).requires_grad_(True)
+    got = torch.autograd.grad(trunk.gated_residual(mx, mx, mx, mw, mw, 0.5, "sigmoid"), (mx, mw), [s.to(dev()) for s in seeds])
+    one = [x.to(dev()).clone().requires_grad_(True) for _ in range(3)] + [w.to(dev()).clone().requires_grad_(True) for _ in range(2)]
+    parts = torch.autograd.grad(trunk.gated_residual(*one, 0.5, "sigmoid"), one, [s.to(dev()) for s in seeds])
+    for a, b in ((got[0], parts[:3]), (got[1], parts[3:])):
+        s = sum(p.abs() for p in b)
+        assert bool(((a - sum(b)).abs() <= 3 * E * 2 * s).all())           # at most two additions, in one order or another
+
+
+@pytest.mark.gpu
+def test_residual_offsets_past_32_bits():
+    rows, d = 540_000, 4096
+    r = lambda: torch.randn(rows, d, device=dev(), dtype=B16)      # noqa: E731
+    leaf = {"x": r(), "h": r(), "gate": r(), "post": torch.rand(d, device=dev()) + 0.5, "next": torch.rand(d, device=dev()) + 0.5}
+    seeds = [r(), r()]
+    names = ("x", "h", "gate")
+
+    def run(a, b):
+        mine = {k: (v[a:b] if k in names else v).detach().requires_grad_(True) for k, v in leaf.items()}
+        outs = call(mine, 0.5, "sigmoid", 1e-6)
+        return [o.detach() for o in outs] + list(torch.autograd.grad(outs, [mine[k] for k in names], [s[a:b] for s in seeds]))
+    full = run(0, rows)
+    for a in (0, 524_250, rows - 70):                               # 524 288 rows: 2^31 values
+        assert all(torch.equal(f[a:a + 70], p) for f, p in zip(full, run(a, a + 70)))
+
+
+@pytest.mark.gpu
+def test_trunk_under_autocast_keeps_the_stream_in_32_bits():
+    torch.manual_seed(0)
+    m = trunk.Trunk(64, 2).to(dev())
+    x = torch.randn(30, 64, device=dev())
+    want = m(x)
+    with torch.autocast("cuda", dtype=B16):
+        got = m(x)
+    assert got.dtype == F32
+    # two blocks of three products whose operands are rounded to bf16 (2^-9 each, relative): a few 2^-9 of the latent's size, which is 1
+    assert float((got - want).square().mean().sqrt()) <= 2 ** -9 * 16
+    got.sum().backward()
+    assert all(p.grad is not None and bool(p.grad.isfinite().all()) for p in m.parameters())
