@@ -25,7 +25,9 @@ template <typename I> __device__ __forceinline__ unsigned key_of(const I* __rest
 }
 
 // ---- forward -------------------------------------------------------------------------------------------------------------------------------
-// A team of TEAM lanes per row, V values per lane and step; 4 rows per team so that four row reads are in flight.
+// A team of TEAM lanes per row, V values per lane and step; 4 rows per team so that four row reads are in flight.  Bound by the writes of the output:
+// 1 245 184 rows of 32 fp32 out of 600 take 29 us (169 MB written and read: 5.8 TB/s), 200 003 of 512 bf16 out of 50 000 55 us (256 MB, 4.65 TB/s;
+// a large copy reaches 4.8 TB/s here, a fill 6.75).
 template <typename T, typename O, typename I, int TEAM, int V>
 __global__ __launch_bounds__(256) void lookup_fwd_kernel(const I* __restrict__ ids, const T* __restrict__ table, O* __restrict__ out, int64_t n, int64_t codes, int dim, float scale) {
     constexpr int kTeams = 256 / TEAM, kRows = 4;
@@ -72,7 +74,8 @@ __global__ __launch_bounds__(1024) void sort_small_kernel(const I* __restrict__ 
 }
 
 // One radix pass in three launches: counts per (chunk, digit); per digit, the number of its ids in earlier chunks, and its total; stable scatter, where every
-// workgroup adds up the totals of the smaller digits by itself.
+// workgroup adds up the totals of the smaller digits by itself.  A chunk is 2048 ids: its scatter goes through LDS, so that equal digits leave it side by side.
+// Bound by latency, not bytes: a pass over 16 384 ids takes 3 + 3.5 + 7 us, over 1 245 184 ids 5 + 6 + 14.5 us.
 template <typename I, bool FIRST>
 __global__ __launch_bounds__(256) void radix_count_kernel(const I* __restrict__ ids, const uint2* __restrict__ in, unsigned* __restrict__ count, int64_t n, int64_t codes, int shift, int bits) {
     __shared__ unsigned bin[1 << kMaxBits];
@@ -241,6 +244,8 @@ __global__ __launch_bounds__(64 * kWaves) void radix_scatter_kernel(const I* __r
 // ---- sums over the sorted list ----------------------------------------------------------------------------------------------------------------
 // Entry i of a list: a key (kEmpty: none; | kCarry: no row) and a row of D values.  First level: sorted (id, position) pairs, the row is dout row `position`;
 // later: keys[i], partial row i.
+// Bound by the bytes of dout, read in rows at the sorted positions, and of the table: 1 245 184 rows of 32 fp32 into 600 take 48 us (159 MB in pieces of 128 bytes,
+// 3.3 TB/s), 200 003 of 512 bf16 into 50 000 73 us (256 MB, 3.5 TB/s), 16 384 of 1024 bf16 into 65 536 fp32 rows 46 - 66 us (302 MB, of which 268 written).
 // blocks < sum_blocks: a team of TEAM lanes adds P entries over TEAM * V columns (blockIdx.y: which columns).  The other blocks (first level only): zeros into
 // the table rows no id points to, 64 rows per wave: every lane looks its row up in the sorted keys (binary search), the wave then writes the empty ones.
 template <typename S, typename T, bool FIRST, int TEAM, int V>

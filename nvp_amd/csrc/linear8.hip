@@ -210,7 +210,8 @@ __global__ __launch_bounds__(256) void dequant_blocks_kernel(const uint8_t* __re
 // One workgroup: 16 MT rows x 16 NT columns; its WAVES waves take every WAVES-th block of 128 and add their tiles up through LDS, so a single row
 // times 4096 columns is 256 workgroups x 8 waves that read disjoint weights: bound by the bytes of the weights, which are on their way (kAhead blocks)
 // before anything else happens.  FUSED: the workgroup quantises its rows of x into LDS itself - no workspace, no second launch; each workgroup repeats
-// that, which pays while there are few workgroups or few rows.
+// that, which pays while there are few workgroups or few rows.  1 x 4096 x 4096 bf16: 5.6 us (16.8 MB, 3 TB/s: one round of loads, whose latency is most of
+// it); 32 x 4096 x 4096: 12.3 us with the quantising launch.
 // Operand order: lane (i = lane & 15, g = lane >> 4) holds columns 16 g .. 16 g + 15 and 64 + 16 g .. of its row's block, the same for both
 // operands: which k a register byte stands for cancels in the sum, and each load instruction covers 64 contiguous bytes of a row.
 constexpr int rows_ahead(int mt, int nt) { return mt * nt >= 4 ? 2 : 4; }
@@ -348,6 +349,7 @@ __global__ __launch_bounds__(64 * WAVES) void linear8_rows_kernel(const T* __res
 // shuffles, and the quantised block is the matrix instruction's operand right away.  The weights (all columns, all of K) stay in LDS, with the bytes of a
 // block in the order in which the lanes hold x's columns and the 16-byte pieces of a row swizzled by the row, so that operand reads are free of bank conflicts.
 // Weights are the first operand: a lane then holds four consecutive columns of one row of y.
+// 1 245 184 x 242 -> 128 columns, fp32: 380 - 394 us (1.84 GB, 4.7 - 4.85 TB/s: the rate of a large copy).
 template <int NT> __host__ __device__ constexpr int64_t narrow_lds(int64_t kb) { return 16 * NT * kb * 128 + 2 * kb + 16 * NT * 4; }
 template <typename T, int NT>
 __global__ __launch_bounds__(256, NT <= 8 ? 3 : 2) void linear8_narrow_kernel(const T* __restrict__ x, const uint8_t* __restrict__ qw, const uint8_t* __restrict__ ew, const T* __restrict__ bias, T* __restrict__ y,
@@ -473,7 +475,7 @@ __global__ __launch_bounds__(256, NT <= 8 ? 3 : 2) void linear8_narrow_kernel(co
 // (BM / WM) x (BN / WN) with 32x32x64 instructions.  One barrier per block, at its start: behind it the block has landed for everyone (every wave waits for
 // its own loads, counted: those of later blocks stay in flight) and the stage of the block before has been read, so that its refill is issued at once.
 // The scales come through LDS too: a load into registers would be waited for together with all fills before it.
-// Measured, with the quantising launch: 8192 x 8192 x 8192 bf16 489 us, 2.25 PFLOP/s (the 256 x 256 tile; the matrix units are busy 57 - 60 % of the cycles of a
+// Measured, with the quantising launch: 8192 x 8192 x 8192 bf16 490 us, 2.24 PFLOP/s (the 256 x 256 tile; the matrix units are busy 57 - 60 % of the cycles of a
 // clock that their power holds at 1.8 - 2.0 GHz of 2.4: finer interleaving of loads, reads and products, in 4 or 8 waves, was not faster); 256 x 4096 x 4096
 // 15.3 us (the 64 x 64 tile, bound by the bytes through LDS: 128 MB; splitting a tile's blocks over two or four teams of waves was not faster).
 // LDS rows are 128 bytes; the 16-byte piece c of row r lies at place c ^ (r >> 1 & 7): of any 16 rows that one 256-byte LDS cycle serves (0 - 15, or
@@ -485,7 +487,7 @@ template <int AT> __device__ __forceinline__ void glds16(const void* ubase, unsi
 __device__ __forceinline__ void glds4(const void* ubase, unsigned lane_off, unsigned lds_byte) {
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(lane_off), "s"(ubase), "s"(lds_byte) : "memory");
 }
-// every wave's loads have landed and its LDS reads have returned (that wait by the builtin: the compiler then knows, and waits for them no second time)
+// every wave's loads but the LATER newest have landed and its LDS reads have returned (that wait by the builtin: the compiler then knows, and waits for them no second time)
 template <int LATER> __device__ __forceinline__ void stage_barrier() {
     static_assert(LATER < 64, "vmcnt");
     __builtin_amdgcn_s_waitcnt(0xc07f);      // lgkmcnt(0)
@@ -660,10 +662,15 @@ int path_of(int64_t rows, int64_t k, int64_t n) {
     if (tiles(128) <= 256) return kTiles128;
     return tiles(128) <= 512 ? kTiles128x2 : kTiles256;
 }
-// columns rounded up to 64, 128 or 256 if that many fit the kernel above with two workgroups per CU, else 0
+// Columns rounded up to 64, 128 or 256 where the narrow kernel is the faster one, else 0: the weights leave room for two workgroups per CU, there is a whole
+// block to read (k >= 128: the kernel moves a row's last block back to end with the row), and the rows are worth the time it takes every workgroup to lay
+// the weights out (12 us for 32 KB, 21 us for 64 KB).  bf16, us, tiles / narrow: 242 -> 128 columns (32 KB) 8192 rows 8.1 / 13.0, 32768 rows 16 / 14, 131072 rows
+// 52 / 31, 524288 rows 199 / 109;  130 -> 64 (16 KB) 65536 rows 22 / 12;  1000 -> 64 (64 KB) 65536 rows 49 / 64, 131072 rows 121 / 94;  512 -> 128 (64 KB) 131072
+// rows 68 / 70, 524288 rows 277 / 198;  228 -> 256 (64 KB) 131072 rows 54 / 71 (fp32 83 / 82), 524288 rows 226 / 174.
 int narrow_columns(int64_t rows, int64_t k, int64_t n) {
     const int nt = n <= 64 ? 4 : n <= 128 ? 8 : n <= 256 ? 16 : 0;
-    return rows >= 2048 && k >= 128 && nt && 16 * nt * kblocks(k) * 128 <= 65536 ? 16 * nt : 0;
+    const int64_t bytes = 16 * nt * kblocks(k) * 128;
+    return k >= 128 && nt && bytes <= 65536 && rows >= 2 * bytes ? 16 * nt : 0;
 }
 template <typename T, int NT>
 int launch_narrow(const T* x, const uint8_t* qw, const uint8_t* ew, const void* bias, void* y, int64_t rows, int64_t k, int64_t n, hipStream_t st) {

@@ -309,3 +309,36 @@ def test_linear8_offsets_past_32_bits(m, k, n):
         a = min(a, m - 40)
         want, s = plain_linear(x[a:a + 40].cpu(), w, None)
         within(y[a:a + 40], want, s, k, torch.bfloat16)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,k,n", [(8200, 128, 1), (33003, 130, 61), (32769, 129, 64), (66001, 242, 128), (49999, 300, 50), (65601, 128, 250), (33000, 128, 65), (131073, 515, 33)])
+def test_linear8_few_columns(m, k, n, dtype):
+    test_linear8(m, k, n, dtype)
+
+
+@pytest.mark.gpu
+def test_linear8_few_columns_scales_non_finite_values_and_replays():
+    g = torch.Generator().manual_seed(4)
+    m, k, n = 50001, 259, 40
+    x = torch.randn(m, k, generator=g) * torch.exp2(torch.randint(-12, 13, (m, 3), generator=g).float()).repeat_interleave(128, 1)[:, :k]
+    w = torch.randn(n, k, generator=g) * torch.exp2(torch.randint(-12, 13, (1, 3), generator=g).float()).repeat_interleave(128, 1)[:, :k]
+    q, e = Q.quantize_blocks(w.to(dev()), 128)
+    want, s = plain_linear(x, w, None)
+    mine = x.to(dev())
+    y = Q.linear8(mine, q, e)
+    within(y, want, s, k, torch.float32)
+    bad = mine.clone()
+    bad[0, 5], bad[m - 1, 258] = float("inf"), float("nan")
+    z = Q.linear8(bad, q, e)
+    assert bool(z[0].isnan().all()) and bool(z[m - 1].isnan().all()) and torch.equal(z[1:m - 1], y[1:m - 1])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = Q.linear8(mine, q, e)
+    for _ in range(3):
+        mine.copy_(mine.roll(1, 0))
+        graph.replay()
+        want = Q.linear8(mine, q, e)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
