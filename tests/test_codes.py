@@ -313,3 +313,17 @@ def test_lookup_offsets_past_32_bits():
     for a in range(0, n, 200_000):
         want.index_add_(0, ids[a:a + 200_000], dout[a:a + 200_000].double())
     assert torch.equal(got, want.to(B16))
+
+
+@pytest.mark.gpu
+def test_lookup_in_a_table_past_32_bits():
+    n_codes, dim = 70_000, 40_001                                   # 2.8e9 values, rows that are not 16-byte aligned
+    table = torch.randn(n_codes, dim, device=dev(), dtype=B16, requires_grad=True)
+    ids = torch.tensor([n_codes - 1, 0, 53_700, n_codes - 1, -1], device=dev())
+    out = codes.lookup(ids, table)
+    assert torch.equal(out[:4], table.detach()[ids[:4]]) and not out[4].any()
+    dout = torch.randint(-8, 9, (5, dim), device=dev()).to(B16)
+    got, = torch.autograd.grad(out, table, dout)
+    assert torch.equal(got[n_codes - 1], dout[0] + dout[3]) and torch.equal(got[0], dout[1]) and torch.equal(got[53_700], dout[2])
+    rows = torch.cat([got[a:a + 10_000].ne(0).any(1) for a in range(0, n_codes, 10_000)]).nonzero().flatten()
+    assert rows.tolist() == [0, 53_700, n_codes - 1]
