@@ -363,10 +363,12 @@ __global__ __launch_bounds__(256) void sum_runs_kernel(const uint2* __restrict__
 }
 
 // A list of at most kLast entries: one workgroup per entry; the entry that begins a run adds the whole run, its teams every kTeams-th entry, the teams in order.
-constexpr int last_threads(int team) { return team >= 32 ? 512 : 256; }      // 16 teams of whole waves; with smaller teams the sum over the teams would take over
+// Most of the workgroups find no run that begins at their entry, so a workgroup is small: 256 threads (2048 entries of 1024 columns: 10.0 us, 512 threads 10.9, 1024
+// 22.8 - what the launch of the waves takes).
+constexpr int kLastThreads = 256;
 template <typename T, int TEAM, int V>
-__global__ __launch_bounds__(last_threads(TEAM)) void sum_last_kernel(const unsigned* __restrict__ keys, const float* __restrict__ rows, T* __restrict__ dtable, int m, int dim, float scale) {
-    constexpr int kTeams = last_threads(TEAM) / TEAM, kBatch = 16;
+__global__ __launch_bounds__(kLastThreads) void sum_last_kernel(const unsigned* __restrict__ keys, const float* __restrict__ rows, T* __restrict__ dtable, int m, int dim, float scale) {
+    constexpr int kTeams = kLastThreads / TEAM, kBatch = 16;
     const int i = blockIdx.x;
     const unsigned key = keys[i];
     if (key == kEmpty || (key & kCarry) || (i > 0 && ((keys[i - 1] ^ key) & ~kCarry) == 0u)) return;      // a run begins with an entry that has a row
@@ -526,7 +528,7 @@ int sums(const Plan& P, const uint2* sorted, const S* dout, T* dtable, uint8_t* 
     if (rc || !P.last) return rc;
     const int team = team_of((dim + VF - 1) / VF);
     with_team(team, [&](auto t) {
-        hipLaunchKernelGGL((sum_last_kernel<T, decltype(t)::value, VF>), dim3((unsigned)P.last, (unsigned)((dim + team * VF - 1) / (team * VF))), dim3(last_threads(decltype(t)::value)), 0, st, lkey(P.levels - 1),
+        hipLaunchKernelGGL((sum_last_kernel<T, decltype(t)::value, VF>), dim3((unsigned)P.last, (unsigned)((dim + team * VF - 1) / (team * VF))), dim3(kLastThreads), 0, st, lkey(P.levels - 1),
                            lrow(P.levels - 1), dtable, (int)P.last, dim, scale);
     });
     NVP_LAUNCH_CHECK();
