@@ -7,14 +7,15 @@
 // is handed to the next level: a run of equal ids that lies inside one chunk is finished there, a run that reaches over an edge leaves a partial row in a
 // list of at most two entries per chunk, which is a sorted list again and goes through the same kernel.  Work per team is P rows however
 // the ids are distributed (one id 10^6 times: three more small levels), the order of every sum is fixed, and the result is the same in every run.
-// Sorting: up to 4096 ids in one workgroup (bitonic, on (id, position) pairs, which are distinct); more: stable radix passes of up to 10 bits.
+// Sorting: up to 1024 ids in one workgroup (bitonic, on (id, position) pairs, which are distinct); more: stable radix passes of up to 10 bits.  Where codes are
+// few and rows are narrow the batch is not sorted as a whole but chunk by chunk (further down).
 #include <type_traits>
 #include "stream_types.h"
 
 namespace {
 
 constexpr unsigned kEmpty = 0xffffffffu, kCarry = 0x80000000u;      // list keys: no entry; the run goes on here, but this entry has no row
-constexpr int kSmall = 4096;                                        // ids sorted in one workgroup
+constexpr int kSmall = 1024;                                        // ids sorted in one workgroup (1000 ids, us, so / by radix passes: 23 / 20 for one pass, 24 / 30 for two; 4096: 45 / 21, 49 / 34)
 constexpr int kChunk = 2048, kWaves = 8, kPerWave = kChunk / kWaves; // ids per workgroup of a radix pass
 constexpr int kMaxBits = 10;
 
@@ -75,7 +76,7 @@ __global__ __launch_bounds__(1024) void sort_small_kernel(const I* __restrict__ 
 
 // One radix pass in three launches: counts per (chunk, digit); per digit, the number of its ids in earlier chunks, and its total; stable scatter, where every
 // workgroup adds up the totals of the smaller digits by itself.  A chunk is 2048 ids: its scatter goes through LDS, so that equal digits leave it side by side.
-// Bound by latency, not bytes: a pass over 16 384 ids takes 3 + 3.5 + 7 us, over 1 245 184 ids 5 + 6 + 14.5 us.
+// Bound by latency, not bytes: a pass over 16 384 ids takes 3 + 3.5 + 7 us, over 200 003 ids 4.5 + 4.5 + 7 us.
 template <typename I, bool FIRST>
 __global__ __launch_bounds__(256) void radix_count_kernel(const I* __restrict__ ids, const uint2* __restrict__ in, unsigned* __restrict__ count, int64_t n, int64_t codes, int shift, int bits) {
     __shared__ unsigned bin[1 << kMaxBits];
@@ -93,8 +94,8 @@ __global__ __launch_bounds__(256) void radix_count_kernel(const I* __restrict__ 
     for (int b = threadIdx.x; b < bins; b += 256) count[(int64_t)blockIdx.x * bins + b] = bin[b];
 }
 
-// count [chunk][digit] -> exclusive prefix over the chunks, total [digit].  A workgroup: 16 digits (lanes) x 64 spans of chunks: a span of 608 chunks is 10
-// reads long, two waits for memory (64 digits x 16 spans: five, 9.6 against 5 us).
+// count [chunk][digit] -> exclusive prefix over the chunks, total [digit].  A workgroup: 16 digits (lanes) x 64 spans of chunks: a span of 608 chunks
+// (1.2 million ids) is 10 reads long, two waits for memory (64 digits x 16 spans: five, 9.6 against 5 us).
 __global__ __launch_bounds__(1024) void radix_scan_kernel(unsigned* __restrict__ count, unsigned* __restrict__ total, int chunks, int bits) {
     __shared__ unsigned span[64][16], group[4][16];
     const int bins = 1 << bits, digit = threadIdx.x & 15, s = threadIdx.x >> 4, b = blockIdx.x * 16 + digit;
@@ -132,6 +133,30 @@ __global__ __launch_bounds__(1024) void radix_scan_kernel(unsigned* __restrict__
                 count[(int64_t)(c + k) * bins + b] = run;
                 run += t[k];
             }
+    }
+}
+
+// Stable places by digit for a wave's ids, one round of 64 in turn: an id's place is its digit's cursor plus the number of equal digits in lanes before it, and the
+// last of the equals moves the cursor (every lane has read it: one wave, in order).  `put` gets the round and the place.
+template <int ROUNDS, typename P> __device__ __forceinline__ void place_ids(const unsigned (&d)[ROUNDS], int64_t base, int64_t n, int bits, unsigned* cursor, const P& put) {
+    const int lane = threadIdx.x & 63;
+    const unsigned long long below = lane == 0 ? 0ull : ~0ull >> (64 - lane);
+#pragma unroll
+    for (int j = 0; j < ROUNDS; ++j) {
+        const int64_t i = base + j * 64 + lane;
+        if (base + j * 64 >= n) break;                                           // the wave's ids are over
+        unsigned long long same = __ballot(i < n);
+        for (int b = 0; b < bits; ++b) {
+            const unsigned long long m = __ballot((d[j] >> b) & 1u);
+            same &= ((d[j] >> b) & 1u) ? m : ~m;
+        }
+        if (i < n) {
+            const unsigned at = cursor[d[j]] + (unsigned)__popcll(same & below);
+            put(j, at);
+            if ((same >> lane) == 1ull) cursor[d[j]] = at + 1u;
+        }
+        __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");                   // the next round reads what this one wrote (no instruction: LDS keeps a wave's order)
+        __builtin_amdgcn_wave_barrier();
     }
 }
 
@@ -215,23 +240,10 @@ __global__ __launch_bounds__(64 * kWaves) void radix_scatter_kernel(const I* __r
         here += mine[e];
     }
     __syncthreads();
-    const unsigned long long below = lane == 0 ? 0ull : ~0ull >> (64 - lane);
+    unsigned d[kRounds];
 #pragma unroll
-    for (int j = 0; j < kRounds; ++j) {
-        const int64_t i = base + j * 64 + lane;
-        const unsigned d = (k[j] >> shift) & (bins - 1);
-        unsigned long long same = __ballot(i < n);
-        for (int b = 0; b < bits; ++b) {
-            const unsigned long long m = __ballot((d >> b) & 1u);
-            same &= ((d >> b) & 1u) ? m : ~m;
-        }
-        if (i < n) {
-            const unsigned at = cursor[wave][d] + (unsigned)__popcll(same & below);
-            list[at] = make_uint2(k[j], p[j]);
-            if ((same >> lane) == 1ull) cursor[wave][d] = at + 1u;               // the last of the equals moves the cursor; every lane has read it (one wave, in order)
-        }
-        __builtin_amdgcn_wave_barrier();
-    }
+    for (int j = 0; j < kRounds; ++j) d[j] = (k[j] >> shift) & (bins - 1);
+    place_ids<kRounds>(d, base, n, bits, cursor[wave], [&](int j, unsigned at) { list[at] = make_uint2(k[j], p[j]); });
     __syncthreads();
     // equal digits lie side by side now: their places in the output do too, and neighbouring lanes write them together
     const int len = (int)min((int64_t)kChunk, n - (int64_t)blockIdx.x * kChunk);
@@ -244,8 +256,7 @@ __global__ __launch_bounds__(64 * kWaves) void radix_scatter_kernel(const I* __r
 // ---- sums over the sorted list ----------------------------------------------------------------------------------------------------------------
 // Entry i of a list: a key (kEmpty: none; | kCarry: no row) and a row of D values.  First level: sorted (id, position) pairs, the row is dout row `position`;
 // later: keys[i], partial row i.
-// Bound by the bytes of dout, read in rows at the sorted positions, and of the table: 1 245 184 rows of 32 fp32 into 600 take 48 us (159 MB in pieces of 128 bytes,
-// 3.3 TB/s), 200 003 of 512 bf16 into 50 000 73 us (256 MB, 3.5 TB/s), 16 384 of 1024 bf16 into 65 536 fp32 rows 46 - 66 us (302 MB, of which 268 written).
+// Bound by the bytes of dout, read in rows at the sorted positions, and of the table: 200 003 of 512 bf16 into 50 000 73 us (256 MB, 3.5 TB/s), 16 384 of 1024 bf16 into 65 536 fp32 rows 46 - 66 us (302 MB, of which 268 written).
 // blocks < sum_blocks: a team of TEAM lanes adds P entries over TEAM * V columns (blockIdx.y: which columns).  The other blocks (first level only): zeros into
 // the table rows no id points to, 64 rows per wave: every lane looks its row up in the sorted keys (binary search), the wave then writes the empty ones.
 template <typename S, typename T, bool FIRST, int TEAM, int V>
@@ -415,12 +426,180 @@ __global__ __launch_bounds__(kLastThreads) void sum_last_kernel(const unsigned* 
     }
 }
 
+// ---- few codes: sums of a chunk of rows at a time ------------------------------------------------------------------------------------------------
+// With up to 1023 codes a chunk of 1024 to 8192 consecutive rows (one chunk per CU) holds every code a few times: a workgroup sorts its chunk's ids in LDS (one
+// digit), adds the rows of each run up and leaves one partial row per code that is there; a second launch adds the chunks' rows in order.  dout is read once,
+// chunk by chunk, so the accesses of a workgroup stay within a window of a few thousand rows (sorted over the whole batch, neighbours in the list are pages
+// apart), and nothing is sorted in global memory: two launches.  Teams take equal shares of the sorted list, however the ids are distributed: a run that
+// reaches into the shares behind is finished by the team it begins in, out of the sums (`head`) the others leave in LDS.
+// Bound by the latency of the sort in front (11 - 14 us for few rows) and the bytes of dout behind it: 1 245 184 rows of 32 fp32 into 600 take 43 us (159 MB, 3.7 TB/s).
+constexpr int kLocal = 8192, kLocalWaves = 16, kLocalRounds = kLocal / (64 * kLocalWaves);      // ids of a chunk at most; a chunk has a multiple of 1024
+template <typename I, typename S, int TEAM, int V>
+__global__ __launch_bounds__(64 * kLocalWaves) void sum_local_kernel(const I* __restrict__ ids, const S* __restrict__ rows, float* __restrict__ part, uint8_t* __restrict__ there, int64_t n,
+                                                                int chunk, int codes, int dim, int bits) {
+    constexpr int kTeams = 64 * kLocalWaves / TEAM, kBatch = V > 4 ? 8 : 16, kPer = (1 << kMaxBits) / (64 * kLocalWaves);
+    static_assert(kLocalWaves * (1 << kMaxBits) >= kTeams * TEAM * V, "the teams' sums take the cursors' place");
+    __shared__ unsigned space[kLocalWaves << kMaxBits];                               // cursors of the waves, then the teams' first sums
+    __shared__ unsigned list[kLocal];                                            // sorted: id << 16 | row of the chunk
+    __shared__ unsigned wsum[kLocalWaves], length, through[kTeams];
+    const int lane64 = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int per_wave = chunk / kLocalWaves;
+    const int64_t chunk0 = (int64_t)blockIdx.x * chunk, base = chunk0 + wave * per_wave, end = min(base + per_wave, n);
+    unsigned d[kLocalRounds];
+#pragma unroll
+    for (int j = 0; j < kLocalRounds; ++j) d[j] = base + j * 64 + lane64 < end ? key_of(ids, base + j * 64 + lane64, codes) : 0u;
+    for (int b = threadIdx.x; b < kLocalWaves << kMaxBits; b += 64 * kLocalWaves) space[b] = 0u;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kLocalRounds; ++j)
+        if (base + j * 64 + lane64 < end) atomicAdd(&space[(wave << kMaxBits) + d[j]], 1u);
+    __syncthreads();
+    unsigned mine[kPer], sum = 0u;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+        const int b = threadIdx.x * kPer + e;
+        mine[e] = 0u;
+#pragma unroll
+        for (int w = 0; w < kLocalWaves; ++w) mine[e] += space[(w << kMaxBits) + b];
+        sum += mine[e];
+        if (b < codes) there[(int64_t)blockIdx.x * codes + b] = mine[e] ? 1 : 0;
+    }
+    unsigned inc = sum;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const unsigned up = __shfl_up(inc, o);
+        if (lane64 >= o) inc += up;
+    }
+    if (lane64 == 63) wsum[wave] = inc;
+    __syncthreads();
+    unsigned here = inc - sum;
+    for (int w = 0; w < wave; ++w) here += wsum[w];
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+        const int b = threadIdx.x * kPer + e;
+        if (b == codes) length = here;                                           // what lies behind points nowhere
+        unsigned run = here;
+#pragma unroll
+        for (int w = 0; w < kLocalWaves; ++w) {
+            const unsigned v = space[(w << kMaxBits) + b];
+            space[(w << kMaxBits) + b] = run;
+            run += v;
+        }
+        here += mine[e];
+    }
+    __syncthreads();
+    place_ids<kLocalRounds>(d, base, end, bits, space + (wave << kMaxBits),
+                            [&](int j, unsigned at) { list[at] = d[j] << 16 | (unsigned)(wave * per_wave + j * 64 + lane64); });
+    __syncthreads();
+
+    const int len = (int)length, share = (len + kTeams - 1) / kTeams, team = threadIdx.x / TEAM, lane = threadIdx.x % TEAM;
+    const int lo = team * share, hi = min(lo + share, len);
+    const bool live = lane * V < dim;
+    const int c = min(lane * V, dim - V);                                        // the last vector of an odd width is moved back: its first columns are summed and written twice, alike
+    float* const head = reinterpret_cast<float*>(space) + lane * V;              // [team][TEAM * V]
+    float* const out = part + (int64_t)blockIdx.x * codes * dim + c;
+    const S* const in = rows + chunk0 * dim + c;
+    float acc[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) acc[e] = 0.f;
+    unsigned cur = 0u;
+    bool to_right = false;
+    if (lo < hi) {
+        cur = list[lo] >> 16;
+        bool from_left = lo > 0 && list[lo - 1] >> 16 == cur;                    // the run begins in a share before
+        const auto flush = [&] {
+            if (from_left) {
+#pragma unroll
+                for (int e = 0; e < V; ++e) head[team * (TEAM * V) + e] = acc[e];
+            } else if (live) {
+                nvp_store<float, V>(out + (int64_t)cur * dim, acc);
+            }
+        };
+        for (int i0 = lo; i0 < hi; i0 += kBatch) {
+            nvp_vec<S, V> f[kBatch];
+            unsigned k[kBatch];
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b) {
+                const unsigned t = list[min(i0 + b, hi - 1)];
+                k[b] = t >> 16;
+                f[b] = nvp_load_raw<S, V>(in + (int64_t)(t & 0xffffu) * dim);
+            }
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b)
+                if (i0 + b < hi) {
+                    if (k[b] != cur) {
+                        flush();
+                        from_left = false;
+                        cur = k[b];
+#pragma unroll
+                        for (int e = 0; e < V; ++e) acc[e] = 0.f;
+                    }
+#pragma unroll
+                    for (int e = 0; e < V; ++e) acc[e] += (float)f[b].v[e];
+                }
+        }
+        to_right = hi < len && list[hi] >> 16 == cur;
+        if (!to_right || from_left) flush();
+        if (lane == 0) through[team] = to_right && from_left;
+        to_right = to_right && !from_left;                                       // the run begins here and goes on
+    }
+    __syncthreads();
+    if (!to_right) return;
+    for (int t = team + 1; t < kTeams; ++t) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) acc[e] += head[t * (TEAM * V) + e];
+        if (!through[t]) break;
+    }
+    if (live) nvp_store<float, V>(out + (int64_t)cur * dim, acc);
+}
+
+// dtable[code] = scale * (the chunks' partial rows of the code, in order); a workgroup per code, its teams every kTeams-th chunk, the teams in order
+template <typename T, int TEAM, int V>
+__global__ __launch_bounds__(256) void sum_chunks_kernel(const float* __restrict__ part, const uint8_t* __restrict__ there, T* __restrict__ dtable, int64_t chunks, int codes, int dim, float scale) {
+    constexpr int kTeams = 256 / TEAM, kBatch = V > 4 ? 8 : 16;
+    __shared__ float sums[kTeams][TEAM * V];
+    const int code = blockIdx.x, lane = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
+    const int c = min(lane * V, dim - V);
+    float acc[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) acc[e] = 0.f;
+    for (int64_t w0 = team; w0 < chunks; w0 += kTeams * kBatch) {
+        nvp_vec<float, V> f[kBatch];
+        bool has[kBatch];
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) {
+            const int64_t w = min(w0 + b * kTeams, chunks - 1);
+            has[b] = w0 + b * kTeams < chunks && there[w * codes + code];
+            f[b] = nvp_load_raw<float, V>(part + (w * codes + code) * dim + c);  // (no branch between the loads; what is not there is dropped)
+        }
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b)
+            if (has[b])
+#pragma unroll
+                for (int e = 0; e < V; ++e) acc[e] += f[b].v[e];
+    }
+#pragma unroll
+    for (int e = 0; e < V; ++e) sums[team][lane * V + e] = acc[e];
+    __syncthreads();
+    if (team == 0 && lane * V < dim) {
+        float t[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            float a = 0.f;
+#pragma unroll
+            for (int k = 0; k < kTeams; ++k) a += sums[k][lane * V + e];
+            t[e] = a * scale;
+        }
+        nvp_store<T, V>(dtable + (int64_t)code * dim + c, t);
+    }
+}
+
 // ---- host ---------------------------------------------------------------------------------------------------------------------------------------
 int64_t up256(int64_t b) { return (b + 255) / 256 * 256; }
 constexpr int kPerChunk2 = 32, kLast = 2560;
 
 struct Plan {
-    bool small;
+    bool small, local;
     int passes, bits;
     int64_t radix_chunks;
     int per_chunk;                  // first level
@@ -431,6 +610,20 @@ struct Plan {
 };
 Plan plan_of(int64_t n, int64_t codes, int64_t dim) {
     Plan P{};
+    // chunk by chunk or sorted as a whole, us of kernels, fp32: 600 codes x 32: 64 rows 11 / 12.5, 4096 rows 14 / 22, 65 536 rows 16 / 32, 1 245 184 rows 43 / 67;
+    // x 64: 1 245 184 rows 90 / 106;  x 114: 65 536 rows 27 / 36, 262 144 rows 51 / 54, 1 245 184 rows 177 / 165;  1000 codes x 256: 16 384 rows 39 / 26, 262 144 rows
+    // 138 / 71 (few teams of many lanes, and a fourth of a chunk's bytes again in partial rows)
+    P.local = n && codes < (1 << kMaxBits) && (dim <= 64 || (dim <= 128 && n <= 1 << 18));
+    if (P.local) {
+        // a chunk per CU, as long as its ids fit; equal chunks where there are more
+        const int64_t rounds = (n + 256 * kLocal - 1) / (256 * kLocal);
+        P.per_chunk = (int)((n + 256 * rounds * 1024 - 1) / (256 * rounds * 1024)) * 1024;
+        P.chunks[0] = (n + P.per_chunk - 1) / P.per_chunk;
+        for (P.bits = 1; (codes >> P.bits) != 0;) ++P.bits;                      // keys 0 .. codes
+        P.off_total = up256(P.chunks[0] * codes * dim * 4);
+        P.bytes = P.off_total + up256(P.chunks[0] * codes);
+        return P;
+    }
     P.small = n <= kSmall;
     int b = 1;
     while (b < 32 && ((codes + 1) - 1) >> b) ++b;                    // keys 0 .. codes
@@ -535,9 +728,28 @@ int sums(const Plan& P, const uint2* sorted, const S* dout, T* dtable, uint8_t* 
     return 0;
 }
 
+template <typename I, typename S, typename T, int V>
+int sums_local(const Plan& P, const I* ids, const S* dout, T* dtable, uint8_t* ws, int64_t n, int64_t codes, int dim, float scale, hipStream_t st) {
+    float* const part = (float*)ws;
+    uint8_t* const there = ws + P.off_total;
+    const int team = team_of((dim + V - 1) / V);
+    if (P.chunks[0] > 0x7fffffff) return NVP_ERR_UNSUPPORTED;
+    with_team(team, [&](auto t) {
+        hipLaunchKernelGGL((sum_local_kernel<I, S, decltype(t)::value, V>), dim3((unsigned)P.chunks[0]), dim3(64 * kLocalWaves), 0, st, ids, dout, part, there, n, P.per_chunk, (int)codes, dim, P.bits);
+    });
+    NVP_LAUNCH_CHECK();
+    with_team(team, [&](auto t) {
+        hipLaunchKernelGGL((sum_chunks_kernel<T, decltype(t)::value, V>), dim3((unsigned)codes), dim3(256), 0, st, part, there, dtable, P.chunks[0], (int)codes, dim, scale);
+    });
+    NVP_LAUNCH_CHECK();
+    return 0;
+}
+
 template <typename I, typename S, typename T>
 int bwd(const I* ids, const S* dout, T* dtable, int64_t n, int64_t codes, int dim, float scale, uint8_t* ws, hipStream_t st) {
     const Plan P = plan_of(n, codes, dim);
+    constexpr int VL = 16 / sizeof(S);
+    if (P.local) return dim >= VL ? sums_local<I, S, T, VL>(P, ids, dout, dtable, ws, n, codes, dim, scale, st) : sums_local<I, S, T, 1>(P, ids, dout, dtable, ws, n, codes, dim, scale, st);
     uint2* buf[2] = {(uint2*)(ws + P.off_sorted[0]), (uint2*)(ws + P.off_sorted[P.small ? 0 : 1])};
     int at = 0;
     if (n == 0) {
