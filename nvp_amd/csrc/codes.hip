@@ -54,9 +54,28 @@ __global__ __launch_bounds__(256) void lookup_fwd_kernel(const I* __restrict__ i
 }
 
 // ---- sorting -------------------------------------------------------------------------------------------------------------------------------
+// A short list of ids keeps few CUs busy: where most rows of the gradient stay empty the other workgroups of the sort's launches write zeros, each launch a part
+// of the table.  Workgroups from `work` on write 64 KB each.
+struct Fill {
+    uint8_t* to;
+    int64_t bytes;
+    unsigned work;
+};
+constexpr int64_t kFillBytes = 65536;
+__device__ __forceinline__ bool fills(const Fill& F) {
+    if (blockIdx.x < F.work) return false;
+    uint8_t* const to = F.to + (int64_t)(blockIdx.x - F.work) * kFillBytes;
+    const int len = (int)min(kFillBytes, F.bytes - (int64_t)(blockIdx.x - F.work) * kFillBytes);
+    const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int i = threadIdx.x * 16; i + 16 <= len; i += blockDim.x * 16) nvp_store<float, 4>(reinterpret_cast<float*>(to + i), zero);
+    for (int i = (len & ~15) + threadIdx.x; i < len; i += blockDim.x) to[i] = 0;
+    return true;
+}
+
 template <typename I>
-__global__ __launch_bounds__(1024) void sort_small_kernel(const I* __restrict__ ids, uint2* __restrict__ sorted, int n, int64_t codes, int padded) {
+__global__ __launch_bounds__(1024) void sort_small_kernel(const I* __restrict__ ids, uint2* __restrict__ sorted, int n, int64_t codes, int padded, Fill fill) {
     __shared__ unsigned long long s[kSmall];
+    if (fills(fill)) return;
     for (int i = threadIdx.x; i < padded; i += 1024) s[i] = i < n ? (unsigned long long)key_of(ids, i, codes) << 32 | (unsigned)i : ~0ull;
     for (int size = 2; size <= padded; size <<= 1)
         for (int step = size >> 1; step > 0; step >>= 1) {
@@ -78,8 +97,10 @@ __global__ __launch_bounds__(1024) void sort_small_kernel(const I* __restrict__ 
 // workgroup adds up the totals of the smaller digits by itself.  A chunk is 2048 ids: its scatter goes through LDS, so that equal digits leave it side by side.
 // Bound by latency, not bytes: a pass over 16 384 ids takes 3 + 3.5 + 7 us, over 200 003 ids 4.5 + 4.5 + 7 us.
 template <typename I, bool FIRST>
-__global__ __launch_bounds__(256) void radix_count_kernel(const I* __restrict__ ids, const uint2* __restrict__ in, unsigned* __restrict__ count, int64_t n, int64_t codes, int shift, int bits) {
+__global__ __launch_bounds__(256) void radix_count_kernel(const I* __restrict__ ids, const uint2* __restrict__ in, unsigned* __restrict__ count, int64_t n, int64_t codes, int shift, int bits,
+                                                          Fill fill) {
     __shared__ unsigned bin[1 << kMaxBits];
+    if (fills(fill)) return;
     const int bins = 1 << bits;
     const int64_t base = (int64_t)blockIdx.x * kChunk + threadIdx.x;
     unsigned k[kChunk / 256];
@@ -96,8 +117,9 @@ __global__ __launch_bounds__(256) void radix_count_kernel(const I* __restrict__ 
 
 // count [chunk][digit] -> exclusive prefix over the chunks, total [digit].  A workgroup: 16 digits (lanes) x 64 spans of chunks: a span of 608 chunks
 // (1.2 million ids) is 10 reads long, two waits for memory (64 digits x 16 spans: five, 9.6 against 5 us).
-__global__ __launch_bounds__(1024) void radix_scan_kernel(unsigned* __restrict__ count, unsigned* __restrict__ total, int chunks, int bits) {
+__global__ __launch_bounds__(1024) void radix_scan_kernel(unsigned* __restrict__ count, unsigned* __restrict__ total, int chunks, int bits, Fill fill) {
     __shared__ unsigned span[64][16], group[4][16];
+    if (fills(fill)) return;
     const int bins = 1 << bits, digit = threadIdx.x & 15, s = threadIdx.x >> 4, b = blockIdx.x * 16 + digit;
     const int per = (chunks + 63) / 64, c0 = min(s * per, chunks), c1 = min(c0 + per, chunks);
     unsigned sum = 0u;
@@ -162,11 +184,13 @@ template <int ROUNDS, typename P> __device__ __forceinline__ void place_ids(cons
 
 template <typename I, bool FIRST>
 __global__ __launch_bounds__(64 * kWaves) void radix_scatter_kernel(const I* __restrict__ ids, const uint2* __restrict__ in, const unsigned* __restrict__ count,
-                                                            const unsigned* __restrict__ total, uint2* __restrict__ sorted, int64_t n, int64_t codes, int shift, int bits) {
+                                                            const unsigned* __restrict__ total, uint2* __restrict__ sorted, int64_t n, int64_t codes, int shift, int bits,
+                                                            Fill fill) {
     __shared__ unsigned cursor[kWaves][1 << kMaxBits];                           // where the wave's next id of a digit goes in `list`
     __shared__ unsigned shift_to[1 << kMaxBits];                                 // place in the output - place in `list`, per digit
     __shared__ uint2 list[kChunk];
     __shared__ unsigned wsum[2][kWaves];
+    if (fills(fill)) return;
     const int bins = 1 << bits, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t base = (int64_t)blockIdx.x * kChunk + (int64_t)wave * kPerWave;      // a wave's ids are consecutive: waves in order, rounds in order, lanes in order
     constexpr int kRounds = kPerWave / 64, kPer = (1 << kMaxBits) / (64 * kWaves);
@@ -695,9 +719,9 @@ int fwd(const I* ids, const T* table, O* out, int64_t n, int64_t codes, int dim,
 
 template <typename S, typename T, bool FIRST, int V>
 int sum_level(const uint2* sorted, const unsigned* keys, const S* rows, T* dtable, unsigned* nkeys, float* nrows, int64_t m, int per_chunk, int64_t chunks, int64_t codes, int dim, float scale,
-              hipStream_t st) {
+              bool filled, hipStream_t st) {
     const int team = team_of((dim + V - 1) / V), teams = 256 / team;
-    const int64_t sums = (chunks + teams - 1) / teams, fill = FIRST ? (codes + 255) / 256 : 0, cols = (dim + team * V - 1) / (team * V);
+    const int64_t sums = (chunks + teams - 1) / teams, fill = FIRST && !filled ? (codes + 255) / 256 : 0, cols = (dim + team * V - 1) / (team * V);
     if (sums + fill > 0x7fffffff || cols > 65535) return NVP_ERR_UNSUPPORTED;
     with_team(team, [&](auto t) {
         hipLaunchKernelGGL((sum_runs_kernel<S, T, FIRST, decltype(t)::value, V>), dim3((unsigned)(sums + fill), (unsigned)cols), dim3(256), 0, st, sorted, keys, rows, dtable, nkeys, nrows, m,
@@ -708,15 +732,15 @@ int sum_level(const uint2* sorted, const unsigned* keys, const S* rows, T* dtabl
 }
 
 template <typename S, typename T, int V, int VF>
-int sums(const Plan& P, const uint2* sorted, const S* dout, T* dtable, uint8_t* ws, int64_t codes, int dim, float scale, hipStream_t st) {
+int sums(const Plan& P, const uint2* sorted, const S* dout, T* dtable, uint8_t* ws, int64_t codes, int dim, float scale, bool filled, hipStream_t st) {
     const auto lkey = [&](int l) { return (unsigned*)(ws + P.off_lkey[l & 1]); };
     const auto lrow = [&](int l) { return (float*)(ws + P.off_lrow[l & 1]); };
     int rc = 0;
     for (int l = 0; !rc && l < P.levels; ++l) {
         unsigned* nk = P.m[l + 1] ? lkey(l) : nullptr;
         float* nr = P.m[l + 1] ? lrow(l) : nullptr;
-        rc = l == 0 ? sum_level<S, T, true, V>(sorted, nullptr, dout, dtable, nk, nr, P.m[0], P.per_chunk, P.chunks[0], codes, dim, scale, st)
-                    : sum_level<float, T, false, VF>(nullptr, lkey(l - 1), lrow(l - 1), dtable, nk, nr, P.m[l], kPerChunk2, P.chunks[l], codes, dim, scale, st);
+        rc = l == 0 ? sum_level<S, T, true, V>(sorted, nullptr, dout, dtable, nk, nr, P.m[0], P.per_chunk, P.chunks[0], codes, dim, scale, filled, st)
+                    : sum_level<float, T, false, VF>(nullptr, lkey(l - 1), lrow(l - 1), dtable, nk, nr, P.m[l], kPerChunk2, P.chunks[l], codes, dim, scale, filled, st);
     }
     if (rc || !P.last) return rc;
     const int team = team_of((dim + VF - 1) / VF);
@@ -751,33 +775,51 @@ int bwd(const I* ids, const S* dout, T* dtable, int64_t n, int64_t codes, int di
     constexpr int VL = 16 / sizeof(S);
     if (P.local) return dim >= VL ? sums_local<I, S, T, VL>(P, ids, dout, dtable, ws, n, codes, dim, scale, st) : sums_local<I, S, T, 1>(P, ids, dout, dtable, ws, n, codes, dim, scale, st);
     uint2* buf[2] = {(uint2*)(ws + P.off_sorted[0]), (uint2*)(ws + P.off_sorted[P.small ? 0 : 1])};
+    // zeros first, beside the sort, where three quarters of the rows stay empty (the others are written twice): us, fp32, zeros behind the sort / beside it,
+    // 65 536 codes x 1024: 512 ids 48 / 40, 16 384 ids 110 / 99;  65 536 codes x 512: 32 768 ids 59 / 63, 65 536 ids 80 / 85
+    const int64_t bytes = codes * (int64_t)dim * (int64_t)sizeof(T), launches = P.small ? 1 : 3 * P.passes;
+    const int64_t slice = ((bytes + launches - 1) / launches + kFillBytes - 1) / kFillBytes * kFillBytes;
+    const bool filled = n && codes >= 4 * n && slice / kFillBytes < 0x3fffffff;
+    int64_t done = 0;
+    const auto next = [&](int64_t work, int64_t& grid) {                         // the launch's grid with its part of the table
+        const int64_t len = filled ? (bytes - done < slice ? bytes - done : slice) : 0;
+        const Fill f{(uint8_t*)dtable + done, len, (unsigned)work};
+        done += len;
+        grid = work + (len + kFillBytes - 1) / kFillBytes;
+        return f;
+    };
     int at = 0;
+    int64_t g;
     if (n == 0) {
         // nothing to sort: the sums below only write zeros
     } else if (P.small) {
         int padded = 2;
         while (padded < n) padded <<= 1;
-        hipLaunchKernelGGL((sort_small_kernel<I>), dim3(1), dim3(1024), 0, st, ids, buf[0], (int)n, codes, padded);
+        const Fill f = next(1, g);
+        hipLaunchKernelGGL((sort_small_kernel<I>), dim3((unsigned)g), dim3(1024), 0, st, ids, buf[0], (int)n, codes, padded, f);
         NVP_LAUNCH_CHECK();
     } else {
         unsigned *count = (unsigned*)(ws + P.off_count), *total = (unsigned*)(ws + P.off_total);
-        const dim3 g((unsigned)P.radix_chunks), wg(256), wide(64 * kWaves);
+        const dim3 wg(256), wide(64 * kWaves);
         for (int p = 0; p < P.passes; ++p) {
             const int shift = p * P.bits;
-            if (p == 0) hipLaunchKernelGGL((radix_count_kernel<I, true>), g, wg, 0, st, ids, buf[at], count, n, codes, shift, P.bits);
-            else hipLaunchKernelGGL((radix_count_kernel<I, false>), g, wg, 0, st, ids, buf[at], count, n, codes, shift, P.bits);
+            Fill f = next(P.radix_chunks, g);
+            if (p == 0) hipLaunchKernelGGL((radix_count_kernel<I, true>), dim3((unsigned)g), wg, 0, st, ids, buf[at], count, n, codes, shift, P.bits, f);
+            else hipLaunchKernelGGL((radix_count_kernel<I, false>), dim3((unsigned)g), wg, 0, st, ids, buf[at], count, n, codes, shift, P.bits, f);
             NVP_LAUNCH_CHECK();
-            hipLaunchKernelGGL(radix_scan_kernel, dim3(((1u << P.bits) + 15) / 16), dim3(1024), 0, st, count, total, (int)P.radix_chunks, P.bits);
+            f = next(((1 << P.bits) + 15) / 16, g);
+            hipLaunchKernelGGL(radix_scan_kernel, dim3((unsigned)g), dim3(1024), 0, st, count, total, (int)P.radix_chunks, P.bits, f);
             NVP_LAUNCH_CHECK();
-            if (p == 0) hipLaunchKernelGGL((radix_scatter_kernel<I, true>), g, wide, 0, st, ids, buf[at], count, total, buf[at ^ 1], n, codes, shift, P.bits);
-            else hipLaunchKernelGGL((radix_scatter_kernel<I, false>), g, wide, 0, st, ids, buf[at], count, total, buf[at ^ 1], n, codes, shift, P.bits);
+            f = next(P.radix_chunks, g);
+            if (p == 0) hipLaunchKernelGGL((radix_scatter_kernel<I, true>), dim3((unsigned)g), wide, 0, st, ids, buf[at], count, total, buf[at ^ 1], n, codes, shift, P.bits, f);
+            else hipLaunchKernelGGL((radix_scatter_kernel<I, false>), dim3((unsigned)g), wide, 0, st, ids, buf[at], count, total, buf[at ^ 1], n, codes, shift, P.bits, f);
             NVP_LAUNCH_CHECK();
             at ^= 1;
         }
     }
     constexpr int V = vec_of<S, T>();
-    if (dim >= (V > 4 ? V : 4)) return sums<S, T, V, 4>(P, buf[at], dout, dtable, ws, codes, dim, scale, st);
-    return sums<S, T, 1, 1>(P, buf[at], dout, dtable, ws, codes, dim, scale, st);
+    if (dim >= (V > 4 ? V : 4)) return sums<S, T, V, 4>(P, buf[at], dout, dtable, ws, codes, dim, scale, filled, st);
+    return sums<S, T, 1, 1>(P, buf[at], dout, dtable, ws, codes, dim, scale, filled, st);
 }
 
 template <typename T, typename O>

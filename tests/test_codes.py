@@ -409,3 +409,14 @@ def test_lookup_distributions_of_many_codes(kind, n):
 def test_lookup_at_the_borders_of_the_two_ways(n, n_codes, dim, table_dtype, dtype):
     g = torch.Generator().manual_seed(n + dim)
     check(torch.randint(-1, n_codes, (n,), generator=g).to(dev()), torch.randn(n_codes, dim, generator=g).to(table_dtype).to(dev()), 1.5, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("table_dtype,dtype", PAIRS)
+@pytest.mark.parametrize("n,n_codes,dim", [(1, 1025, 1), (9, 40, 301), (513, 5000, 333), (1024, 4096, 129), (1025, 4100, 130), (1025, 4099, 130), (3000, 200000, 17), (2049, 1 << 21, 5)])
+def test_lookup_mostly_empty_tables(n, n_codes, dim, table_dtype, dtype):
+    """Zeros written beside the sort (and behind it, just short of that): odd sizes, so that the last bytes are fewer than one access."""
+    g = torch.Generator().manual_seed(n + dim)
+    junk = torch.full((n_codes, dim), float("nan"), device=dev(), dtype=table_dtype)       # the allocator hands this memory out again: what is not written shows
+    del junk
+    check(torch.randint(-1, n_codes, (n,), generator=g).to(dev()), torch.randn(n_codes, dim, generator=g).to(table_dtype).to(dev()), 1.5, dtype)
