@@ -280,7 +280,8 @@ __global__ __launch_bounds__(64 * kWaves) void radix_scatter_kernel(const I* __r
 // ---- sums over the sorted list ----------------------------------------------------------------------------------------------------------------
 // Entry i of a list: a key (kEmpty: none; | kCarry: no row) and a row of D values.  First level: sorted (id, position) pairs, the row is dout row `position`;
 // later: keys[i], partial row i.
-// Bound by the bytes of dout, read in rows at the sorted positions, and of the table: 200 003 of 512 bf16 into 50 000 73 us (256 MB, 3.5 TB/s), 16 384 of 1024 bf16 into 65 536 fp32 rows 46 - 66 us (302 MB, of which 268 written).
+// Bound by the bytes of dout, read in rows at the sorted positions, and of the table: 200 003 of 512 bf16 into 50 000 73 us (256 MB, 3.5 TB/s),
+// 16 384 of 1024 bf16 into 65 536 fp32 rows 16 - 18 us (the empty rows are written beside the sort there, 268 MB in 55 us).
 // blocks < sum_blocks: a team of TEAM lanes adds P entries over TEAM * V columns (blockIdx.y: which columns).  The other blocks (first level only): zeros into
 // the table rows no id points to, 64 rows per wave: every lane looks its row up in the sorted keys (binary search), the wave then writes the empty ones.
 template <typename S, typename T, bool FIRST, int TEAM, int V>
@@ -456,7 +457,8 @@ __global__ __launch_bounds__(kLastThreads) void sum_last_kernel(const unsigned* 
 // chunk by chunk, so the accesses of a workgroup stay within a window of a few thousand rows (sorted over the whole batch, neighbours in the list are pages
 // apart), and nothing is sorted in global memory: two launches.  Teams take equal shares of the sorted list, however the ids are distributed: a run that
 // reaches into the shares behind is finished by the team it begins in, out of the sums (`head`) the others leave in LDS.
-// Bound by the latency of the sort in front (11 - 14 us for few rows) and the bytes of dout behind it: 1 245 184 rows of 32 fp32 into 600 take 43 us (159 MB, 3.7 TB/s).
+// Bound by the latency of the sort in front (11 - 14 us for few rows) and the bytes of dout behind it: 1 245 184 rows of 32 fp32 into 600 take 53 - 55 us and 6.5 for
+// the second launch (159 MB and 19 MB of partial rows there and back, 3.2 TB/s; 43 us in all where dout is still in the memory-side cache).
 constexpr int kLocal = 8192, kLocalWaves = 16, kLocalRounds = kLocal / (64 * kLocalWaves);      // ids of a chunk at most; a chunk has a multiple of 1024
 template <typename I, typename S, int TEAM, int V>
 __global__ __launch_bounds__(64 * kLocalWaves) void sum_local_kernel(const I* __restrict__ ids, const S* __restrict__ rows, float* __restrict__ part, uint8_t* __restrict__ there, int64_t n,
