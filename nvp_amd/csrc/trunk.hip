@@ -7,10 +7,11 @@
 // c1 needs E and so c2; written out it is s [sum q (dy + r2 dv) - r2 c2 sum q v] / D with q = a p n: three sums that need neither, so both means come from
 // ONE reduction per row instead of two in sequence.  r1, r2 are kept from forward (8 bytes per row); n, a, y, v are computed again from x, h, g.
 // All arithmetic and every sum is fp32; each result is rounded once to its type.  Bound by memory: 4-5 streams forward, 8-9 backward, each touched once.
-// One row is held in registers by a team of TEAM lanes, 8 values each (16 above 4096), in 16-byte accesses: V = 8 of 16 bits, 4 of 32.
+// One row is held in registers by a team of TEAM lanes, 8 values each (12 above 4096, 16 above 6144), in 16-byte accesses: V = 8 of 16 bits, 4 of 32.
 // Measured: 16384 x 2048 bf16 with shared gates, forward 55 us (268 MB, 4.9 TB/s), backward 85 us (403 MB, 4.7 TB/s) and 4.5 us for the partial rows; 65536 x 4096
-// forward 530 - 580 us (2.68 GB, 4.6 - 5.1 TB/s): the rate of a large copy.  Above 4096 columns the backward kernel has no registers left to load a row
-// ahead and reaches 2.9 - 4.7 TB/s (teams of 1024 lanes with 8 values each leave 128 registers per lane, spill, and reach 0.6 - 2.6).
+// forward 530 - 580 us (2.68 GB, 4.6 - 5.1 TB/s): the rate of a large copy.  Above 4096 columns the backward kernel runs
+// short of registers: 16384 x 5000 at 4.7 - 4.8 TB/s, 8192 x 8192 at 4.4 - 4.7 (teams of 1024 lanes with 8 values each leave 128 registers per lane, spill, and
+// reach 0.6 - 2.6).
 #include "stream_types.h"
 
 namespace {
@@ -109,7 +110,7 @@ __global__ __launch_bounds__(threads_of(TEAM)) void residual_fwd_kernel(const T*
                                                                         const W* __restrict__ next, T* __restrict__ y, T* __restrict__ u, float* __restrict__ stats, Rows R) {
     constexpr int kTeams = threads_of(TEAM) / TEAM;
     typedef row_of<T, TEAM, V, VALS, ODD> Row;
-    constexpr bool kAhead = VALS == 8;                          // registers for a second row?
+    constexpr bool kAhead = VALS <= 12;                         // registers for a second row?
     __shared__ float red[TEAM > 64 ? 2 * TEAM / 64 : 1];
     int flip = 0;
     const int lane = kTeams == 1 ? threadIdx.x : threadIdx.x % TEAM, team = team_index<TEAM, kTeams>();
@@ -188,7 +189,7 @@ __global__ __launch_bounds__(threads_of(TEAM)) void residual_bwd_kernel(const T*
                                                                         float* __restrict__ dpost_part, float* __restrict__ dnext_part, Rows R, Units U) {
     constexpr int kTeams = threads_of(TEAM) / TEAM, N = FORM == kBoth ? 3 : 1;
     typedef row_of<T, TEAM, V, VALS, ODD> Row;
-    constexpr bool kAhead = VALS == 8;                          // registers for a second row?
+    constexpr bool kAhead = VALS == 8 || (VALS == 12 && sizeof(T) == 2);      // registers for a second row? (12 values, fp32: 434 us without, 444 with, 16384 x 4104)
     __shared__ float red[TEAM > 64 ? 2 * N * TEAM / 64 : 1];
     __shared__ float comb[kTeams > 1 ? kTeams : 1][kTeams > 1 ? TEAM * VALS : 1];
     int flip = 0;
@@ -367,7 +368,7 @@ __global__ __launch_bounds__(1024) void residual_reduce_kernel(const float* __re
 }
 
 constexpr int kMaxDim = 8192;
-int team_of(int dim) { return dim <= 128 ? 16 : dim <= 512 ? 64 : dim <= 2048 ? 256 : 512; }      // 8 values per lane; 16 above 4096
+int team_of(int dim) { return dim <= 128 ? 16 : dim <= 512 ? 64 : dim <= 2048 ? 256 : 512; }      // 8 values per lane; 12 above 4096, 16 above 6144
 
 struct Plan {
     Units U;
@@ -452,7 +453,11 @@ template <typename T, typename W, int FORM, bool ODD> int by_team(const Call& c)
         case 16: return launch<T, W, FORM, 16, V, 8, ODD>(c);
         case 64: return launch<T, W, FORM, 64, V, 8, ODD>(c);
         case 256: return launch<T, W, FORM, 256, V, 8, ODD>(c);
-        default: return c.a->dim <= 4096 ? launch<T, W, FORM, 512, V, 8, ODD>(c) : launch<T, W, FORM, 512, V, 16, ODD>(c);
+        default:
+            if (c.a->dim <= 4096) return launch<T, W, FORM, 512, V, 8, ODD>(c);
+            // 12 values per lane up to 6144, in accesses of four (16384 x 5000, backward: 279 us bf16, 543 us fp32; 16 values: 329, 802), 16 above (fp32 always
+            // as an odd width: 8192 x 8190 in 481 us, 8192 x 8192 by the even way in 530)
+            return c.a->dim <= 6144 ? launch<T, W, FORM, 512, 4, 12, ODD>(c) : launch<T, W, FORM, 512, V, 16, ODD || V == 4>(c);
     }
 }
 template <typename T, typename W, int FORM> int by_width(const Call& c) {

@@ -525,3 +525,28 @@ def test_trunk_under_autocast_keeps_the_stream_in_32_bits():
     assert float((got - want).square().mean().sqrt()) <= 2 ** -9 * 16
     got.sum().backward()
     assert all(p.grad is not None and bool(p.grad.isfinite().all()) for p in m.parameters())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,wdtype", TYPES)
+@pytest.mark.parametrize("rows,d", [(3, 4097), (700, 4100), (5, 5000), (4, 6143), (2, 6144), (601, 6145), (3, 8191)])
+def test_residual_wide_rows(rows, d, dtype, wdtype):
+    for k, (form, gate) in enumerate((("both", (rows, d)), ("both", (1, d)), ("first", None), ("last", (rows, d)))):
+        if rows > 100 and k:
+            break
+        leaf, seeds = make((rows, d), dtype, wdtype, form, gate, rows * 100 + d)
+        check(leaf, seeds, 0.75, "sigmoid" if k % 2 == 0 else None)
+
+
+@pytest.mark.gpu
+def test_residual_wide_rows_do_not_depend_on_their_neighbours():
+    for d in (4104, 5000, 6144, 8192):
+        leaf, seeds = make((1500, d), B16, F32, "both", (1500, d), d)
+        names = ("x", "h", "gate")
+
+        def run(a, b):
+            mine = {k: (v[a:b] if k in names else v).detach().requires_grad_(True) for k, v in leaf.items()}
+            outs = call(mine, 0.5, "sigmoid", 1e-6)
+            return [o.detach() for o in outs] + list(torch.autograd.grad(outs, [mine[k] for k in names], [s[a:b] for s in seeds]))
+        full = run(0, 1500)
+        assert all(torch.equal(f[1490:], p) for f, p in zip(full, run(1490, 1500)))
