@@ -103,7 +103,7 @@ struct Rows {
     float scale, eps, inv_dim;
 };
 
-constexpr int threads_of(int team) { return team > 256 ? team : 256; }
+constexpr int threads_of(int team) { return team > 64 ? team : 256; }      // a team that spans waves is a workgroup
 
 template <typename T, typename W, int FORM, int TEAM, int V, int VALS, bool ODD>
 __global__ __launch_bounds__(threads_of(TEAM)) void residual_fwd_kernel(const T* __restrict__ x, const T* __restrict__ h, const T* __restrict__ gate, const W* __restrict__ post,
@@ -368,7 +368,9 @@ __global__ __launch_bounds__(1024) void residual_reduce_kernel(const float* __re
 }
 
 constexpr int kMaxDim = 8192;
-int team_of(int dim) { return dim <= 128 ? 16 : dim <= 512 ? 64 : dim <= 2048 ? 256 : 512; }      // 8 values per lane; 12 above 4096, 16 above 6144
+// 8 values per lane; 12 above 4096, 16 above 6144.  The smallest team that holds the row (bf16, us, so / with a team of four times
+// the lanes below 512 columns, twice above: 1 245 184 x 32 forward 97 / 169; 262 144 x 228 backward 230 / 238; 131 072 x 640 backward 283 / 512)
+int team_of(int dim) { return dim <= 64 ? 8 : dim <= 128 ? 16 : dim <= 256 ? 32 : dim <= 512 ? 64 : dim <= 1024 ? 128 : dim <= 2048 ? 256 : 512; }
 
 struct Plan {
     Units U;
@@ -378,20 +380,21 @@ struct Plan {
 };
 Plan plan_of(const nvp_residual* a) {
     Plan P;
-    const int team = team_of(a->dim), teams = team > 256 ? 1 : 256 / team;
+    const int team = team_of(a->dim), teams = threads_of(team) / team;
     const bool shared = a->gate && a->gate_rows < a->rows;
     P.gate_rows = shared ? a->gate_rows : 0;
     P.U.share = shared ? a->rows / a->gate_rows : a->rows;
-    // as many workgroups as the chip holds at once (2 of 256 threads per CU at the kernel's registers, 1 of 512): more would leave a second, partly filled
-    // round and more partial rows to add up
-    const int64_t want = (int64_t)(team >= 512 ? 256 : 512) * teams;
+    // as many workgroups as the chip holds at once (8 waves per CU at the kernel's registers): more would leave a second, partly filled round and more partial
+    // rows to add up
+    const int64_t wgs = 256 * 512 / threads_of(team), want = wgs * teams;
     const int64_t rows_per = (a->rows + want - 1) / want;
     P.U.unit = rows_per < P.U.share ? rows_per : P.U.share;
     P.U.per_share = (P.U.share + P.U.unit - 1) / P.U.unit;
     P.U.units = (shared ? a->gate_rows : 1) * P.U.per_share;
     P.parts = shared && P.U.per_share > 1;
     const int64_t g = (P.U.units + teams - 1) / teams;
-    P.groups = g < 512 ? g : 512;
+    const int64_t most = wgs > 512 ? wgs : 512;
+    P.groups = g < most ? g : most;
     return P;
 }
 
@@ -450,8 +453,11 @@ template <typename T, typename W, int FORM, int TEAM, int V, int VALS, bool ODD>
 template <typename T, typename W, int FORM, bool ODD> int by_team(const Call& c) {
     constexpr int V = 16 / sizeof(T);
     switch (team_of(c.a->dim)) {
+        case 8: return launch<T, W, FORM, 8, V, 8, ODD>(c);
         case 16: return launch<T, W, FORM, 16, V, 8, ODD>(c);
+        case 32: return launch<T, W, FORM, 32, V, 8, ODD>(c);
         case 64: return launch<T, W, FORM, 64, V, 8, ODD>(c);
+        case 128: return launch<T, W, FORM, 128, V, 8, ODD>(c);
         case 256: return launch<T, W, FORM, 256, V, 8, ODD>(c);
         default:
             if (c.a->dim <= 4096) return launch<T, W, FORM, 512, V, 8, ODD>(c);
@@ -462,7 +468,7 @@ template <typename T, typename W, int FORM, bool ODD> int by_team(const Call& c)
 }
 template <typename T, typename W, int FORM> int by_width(const Call& c) {
     constexpr int V = 16 / sizeof(T);
-    if (c.a->dim < V) return launch<T, W, FORM, 16, 1, 8, false>(c);
+    if (c.a->dim < V) return launch<T, W, FORM, 8, 1, 8, false>(c);
     return c.a->dim % V ? by_team<T, W, FORM, true>(c) : by_team<T, W, FORM, false>(c);
 }
 template <typename T, typename W> int by_form(const Call& c) {
