@@ -32,6 +32,7 @@ build_lib() {
   for f in $SRCS; do
     [ -f "$f.hip" ] || continue
     local o="$objdir/$f.o"
+    case "$f" in linear8|codes|trunk) o="obj/$f.o";; esac      # no library's flags concern these: compiled once, for the product (built first)
     if [ ! -f "$o" ] || [ "$f.hip" -nt "$o" ] || [ -n "$(find . -maxdepth 1 -name '*.h' -newer "$o" 2>/dev/null)" ] || [ ../../include/nvp_hip.h -nt "$o" ] || [ ../../include/nvp_hip_experiments.h -nt "$o" ] || [ -n "${NVP_REBUILD:-}" ]; then
       local EXTRA=""
       case "$f" in encode|encode_fwd_lds|encode_bwd|harness|optim) EXTRA="-ffp-contract=off";; esac   # separately rounded mul/add (index parity)
@@ -44,7 +45,7 @@ build_lib() {
   done
   local rc=0
   for i in "${!PIDS[@]}"; do
-    if ! wait "${PIDS[$i]}"; then echo "build.sh: compiling ${NAMES[$i]}.hip ($out) FAILED" >&2; rm -f "$objdir/${NAMES[$i]}.o"; rc=1; fi
+    if ! wait "${PIDS[$i]}"; then echo "build.sh: compiling ${NAMES[$i]}.hip ($out) FAILED" >&2; rm -f "$objdir/${NAMES[$i]}.o" "obj/${NAMES[$i]}.o"; rc=1; fi
   done
   if [ $rc -ne 0 ]; then rm -f "$out"; exit 1; fi
   "$HIPCC" --offload-arch=gfx950 -shared -fPIC "${OBJS[@]}" -o "$out"
