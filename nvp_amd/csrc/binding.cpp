@@ -1,7 +1,8 @@
 // The conditioning operators (nvp_amd.codes, nvp_amd.trunk, nvp_amd.quantize.linear8) as torch calls: argument checks, output and workspace allocation,
 // autograd nodes, and the calls of the C ABI (include/nvp_hip.h) on the current stream of the tensors' device.  C++ rather than Python because of what small calls
 // cost: a backward pass runs on autograd's own thread, and a Python backward has to take the interpreter lock there and run its few dozen lines with cold
-// caches - 105 to 200 us for a forward and backward pass whose kernels take 32 us; as C++ nodes the same pass takes 50 to 70 us of host time.
+// caches - 105 to 200 us for a forward and backward pass whose kernels take 10 to 30 us; as C++ nodes 48 us (lookup) to 86 us (residual step with all its
+// gradients), some 45 of them for waking that thread (39 us in all where the engine is told to stay on the caller's).
 // Host code only: no kernel lives here.  The library it calls is the one nvp_amd._lib has loaded (bind()).
 #include <dlfcn.h>
 
