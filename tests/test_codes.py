@@ -420,3 +420,10 @@ def test_lookup_mostly_empty_tables(n, n_codes, dim, table_dtype, dtype):
     junk = torch.full((n_codes, dim), float("nan"), device=dev(), dtype=table_dtype)       # the allocator hands this memory out again: what is not written shows
     del junk
     check(torch.randint(-1, n_codes, (n,), generator=g).to(dev()), torch.randn(n_codes, dim, generator=g).to(table_dtype).to(dev()), 1.5, dtype)
+
+
+def test_a_missing_binding_is_an_error(monkeypatch, tmp_path):
+    monkeypatch.setattr(L, "_binding", None)
+    monkeypatch.setattr(L, "_HERE", str(tmp_path))
+    with pytest.raises(RuntimeError, match="the binding is not built"):
+        codes.lookup(torch.zeros(3, dtype=torch.int64), torch.zeros(4, 5))
