@@ -95,6 +95,14 @@ template <typename T, int TEAM, int V, int VALS, bool ODD> __device__ __forceinl
 }
 
 __device__ __forceinline__ float sigmoid(float g) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504f * g)); }
+// The sigmoid a with what its derivative a (1 - a) needs: t / (1 + t), t = exp(-|g|), is the smaller of a and 1 - a.  A closed gate (g < 0) is kept as a, an open one as
+// -(1 - a): open_of() and slope_of() are then free of cancellation (1 - a from a rounded a is off by 2^-24 / (1 - a) of itself: 1 % at g = 12, all of it from 17 on).
+__device__ __forceinline__ float gate_side(float g) {
+    const float t = __builtin_amdgcn_exp2f(-1.44269504f * fabsf(g));
+    return copysignf(t * __builtin_amdgcn_rcpf(1.f + t), -g);
+}
+__device__ __forceinline__ float open_of(float s, int act) { return act && __float_as_int(s) < 0 ? 1.f + s : s; }      // act 0: s is the gate itself
+__device__ __forceinline__ float slope_of(float s, int act) { return act ? __fmaf_rn(-s, s, fabsf(s)) : 1.f; }
 __device__ __forceinline__ float inv_rms(float sum, float inv_dim, float eps) { return 1.f / sqrtf(sum * inv_dim + eps); }
 
 struct Rows {
@@ -216,14 +224,15 @@ __global__ __launch_bounds__(threads_of(TEAM)) void residual_bwd_kernel(const T*
     for (int64_t un = (int64_t)blockIdx.x * kTeams + team; un < U.units; un += (int64_t)gridDim.x * kTeams) {
         const int64_t grp = un / U.per_share, piece = un - grp * U.per_share;
         const int64_t first = grp * U.share + piece * U.unit, last = min(first + U.unit, (grp + 1) * U.share);
-        float a[VALS], da[VALS], sg[VALS];                      // act(g), its derivative, the sum of the gate's gradient
+        float a[VALS], da[VALS], sg[VALS];                      // act(g) (not SUMMED: gate_side(g)), its derivative, the sum of the gate's gradient
         if (kAhead) fetch(first);
         if (SUMMED) {
             load_row<T, TEAM, V, VALS, ODD>(gate + grp * R.dim, lane, R.dim, a);
 #pragma unroll
             for (int j = 0; j < VALS; ++j) {
-                a[j] = R.act ? sigmoid(a[j]) : a[j];
-                da[j] = R.act ? a[j] * (1.f - a[j]) : 1.f;
+                const float side = R.act ? gate_side(a[j]) : a[j];
+                a[j] = open_of(side, R.act);
+                da[j] = slope_of(side, R.act);
                 sg[j] = 0.f;
             }
         }
@@ -244,9 +253,10 @@ __global__ __launch_bounds__(threads_of(TEAM)) void residual_bwd_kernel(const T*
                     for (int j = 0; j < VALS; ++j) a[j] = 1.f;
                 } else if (R.act) {
 #pragma unroll
-                    for (int j = 0; j < VALS; ++j) a[j] = sigmoid(a[j]);
+                    for (int j = 0; j < VALS; ++j) a[j] = gate_side(a[j]);
                 }
             }
+            const int act = SUMMED || !gate ? 0 : R.act;
             float s[N];
 #pragma unroll
             for (int k = 0; k < N; ++k) s[k] = 0.f;
@@ -255,7 +265,7 @@ __global__ __launch_bounds__(threads_of(TEAM)) void residual_bwd_kernel(const T*
                 float q = 0.f;
                 if (FORM != kFirst) {
                     n[j] *= st.x;
-                    q = a[j] * p[j] * n[j];
+                    q = open_of(a[j], act) * p[j] * n[j];
                 }
                 const bool keep = Row::keep(j, lane, R.dim);
                 if (FORM == kLast) {
@@ -290,10 +300,10 @@ __global__ __launch_bounds__(threads_of(TEAM)) void residual_bwd_kernel(const T*
                 float t[VALS];
 #pragma unroll
                 for (int j = 0; j < VALS; ++j) {
-                    const float en = R.scale * e[j] * n[j];
-                    sp[j] = __fmaf_rn(a[j], en, sp[j]);
-                    t[j] = en * p[j] * (SUMMED ? da[j] : R.act ? a[j] * (1.f - a[j]) : 1.f);
-                    n[j] = st.x * __fmaf_rn(-c1, n[j], R.scale * a[j] * p[j] * e[j]);
+                    const float en = R.scale * e[j] * n[j], open = open_of(a[j], act);
+                    sp[j] = __fmaf_rn(open, en, sp[j]);
+                    t[j] = en * p[j] * (SUMMED ? da[j] : slope_of(a[j], act));
+                    n[j] = st.x * __fmaf_rn(-c1, n[j], R.scale * open * p[j] * e[j]);
                 }
                 if (dh) Row::put(dh + row * R.dim, lane, R.dim, n);
                 if (SUMMED) {

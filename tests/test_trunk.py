@@ -550,3 +550,16 @@ def test_residual_wide_rows_do_not_depend_on_their_neighbours():
             return [o.detach() for o in outs] + list(torch.autograd.grad(outs, [mine[k] for k in names], [s[a:b] for s in seeds]))
         full = run(0, 1500)
         assert all(torch.equal(f[1490:], p) for f, p in zip(full, run(1490, 1500)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,wdtype", TYPES)
+@pytest.mark.parametrize("shape,gate", [((40, 228), (40, 228)), ((9, 115), (9, 115)), ((6, 50, 114), (6, 1, 114)), ((2, 1500, 130), (1, 1, 130)), ((3, 4100), (3, 4100)), ((2, 30, 8190), (2, 1, 8190))])
+def test_residual_gates_far_open_and_far_closed(shape, gate, dtype, wdtype, monkeypatch):
+    """A sigmoid's derivative is a (1 - a) whichever side a is near: every gradient to the tolerance above, of numbers down to 1e-13.  The 64-bit sigmoid is written
+    out here, because autograd differentiates 1 / (1 + exp(-g)) without a difference, while torch.sigmoid's own backward has 1 - a (1e-3 off at 30, in 64 bits)."""
+    monkeypatch.setattr(torch, "sigmoid", lambda g: 1 / (1 + torch.exp(-g)))
+    leaf, seeds = make(shape, dtype, wdtype, "both", gate, sum(shape))
+    g = torch.Generator().manual_seed(1)
+    leaf["gate"] = (torch.rand(gate, generator=g) * 60 - 30).to(dtype).to(dev())
+    check(leaf, seeds, 0.75, "sigmoid")
