@@ -6,11 +6,11 @@
 //     dn = s a p E,  c1 = mean(dn n),  dh = r1 (dn - n c1),  dg = s E n p a'(g),  dp = sum s a E n,  dw = sum du v.
 // c1 needs E and so c2; written out it is s [sum q (dy + r2 dv) - r2 c2 sum q v] / D with q = a p n: three sums that need neither, so both means come from
 // ONE reduction per row instead of two in sequence.  r1, r2 are kept from forward (8 bytes per row); n, a, y, v are computed again from x, h, g.
-// All arithmetic and every sum is fp32; each result is rounded once to its type.  Bound by memory: 4-5 streams forward, 8-9 backward, each touched once.
+// All arithmetic and every sum is fp32; each result is rounded once to its type.  Bound by memory: 4 - 5 streams forward, 6 (shared gate) to 8 backward, each touched once.
 // One row is held in registers by a team of TEAM lanes, 8 values each (12 above 4096, 16 above 6144), in 16-byte accesses: V = 8 of 16 bits, 4 of 32.
 // Measured: 16384 x 2048 bf16 with shared gates, forward 55 us (268 MB, 4.9 TB/s), backward 85 us (403 MB, 4.7 TB/s) and 4.5 us for the partial rows; 65536 x 4096
 // forward 530 - 580 us (2.68 GB, 4.6 - 5.1 TB/s): the rate of a large copy.  Above 4096 columns the backward kernel runs
-// short of registers: 16384 x 5000 at 4.7 - 4.8 TB/s, 8192 x 8192 at 4.4 - 4.7 (teams of 1024 lanes with 8 values each leave 128 registers per lane, spill, and
+// short of registers: 16384 x 5000 at 4.6 - 4.7 TB/s, 8192 x 8192 at 4.3 - 4.6 (teams of 1024 lanes with 8 values each leave 128 registers per lane, spill, and
 // reach 0.6 - 2.6).
 #include "stream_types.h"
 
@@ -94,11 +94,31 @@ template <typename T, int TEAM, int V, int VALS, bool ODD> __device__ __forceinl
     r.get(f, lane, dim);
 }
 
-__device__ __forceinline__ float sigmoid(float g) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504f * g)); }
-// The sigmoid a with what its derivative a (1 - a) needs: t / (1 + t), t = exp(-|g|), is the smaller of a and 1 - a.  A closed gate (g < 0) is kept as a, an open one as
-// -(1 - a): open_of() and slope_of() are then free of cancellation (1 - a from a rounded a is off by 2^-24 / (1 - a) of itself: 1 % at g = 12, all of it from 17 on).
-__device__ __forceinline__ float gate_side(float g) {
-    const float t = __builtin_amdgcn_exp2f(-1.44269504f * fabsf(g));
+// The sigmoid.  exp2(-g log2 e) is off by half an ulp of its argument, |g| / 2 * 2^-24 of the result on top of the rest (40 * 2^-24 at |g| = 80): nothing beside a 16-bit stream's
+// rounding (2^-9, 2^-12 of it), so those stop there.  fp32 streams take exp(-|g|) = e + e (r ln 2 - |g| c'), e = exp2(x), x = -|g| fp32(log2 e) rounded, r what that rounding
+// lost, c' = 1 - ln 2 * fp32(log2 e): two roundings, wherever g is.  Beyond 104 the result is 0; a NaN stays one.
+__device__ __forceinline__ float exp_minus_abs(float g) {
+    float m = fabsf(g);
+    m = m > 104.f ? 104.f : m;
+    const float x = -1.44269504f * m, e = __builtin_amdgcn_exp2f(x), r = __fmaf_rn(-1.44269504f, m, -x);
+    return __fmaf_rn(e, __fmaf_rn(r, 0.693147182f, -1.33497582e-8f * m), e);
+}
+// Its derivative as t a^2, t = exp(-g), and not as a (1 - a), which cancels for open gates (1 - a from a rounded a is off by 2^-24 / (1 - a) of itself: 1 % at g = 12, all of it
+// from 17 on).
+template <typename T> __device__ __forceinline__ float sigmoid(float g, float& slope) {
+    if constexpr (sizeof(T) < 4) {
+        const float t = __builtin_amdgcn_exp2f(-1.44269504f * g), a = __builtin_amdgcn_rcpf(1.f + t);
+        slope = fminf(t, 1e38f) * a * a;                        // (t infinite: a is 0; a NaN is in a)
+        return a;
+    } else {
+        const float t = exp_minus_abs(g), r = __builtin_amdgcn_rcpf(1.f + t), m = t * r;
+        slope = m * r;
+        return g < 0.f ? m : r;
+    }
+}
+// Both in one register, where registers are short: m = t / (1 + t), t = exp(-|g|), is the smaller of a and 1 - a; a closed gate (g < 0) is kept as a, an open one as -(1 - a).
+template <typename T> __device__ __forceinline__ float gate_side(float g) {
+    const float t = sizeof(T) < 4 ? __builtin_amdgcn_exp2f(-1.44269504f * fabsf(g)) : exp_minus_abs(g);
     return copysignf(t * __builtin_amdgcn_rcpf(1.f + t), -g);
 }
 __device__ __forceinline__ float open_of(float s, int act) { return act && __float_as_int(s) < 0 ? 1.f + s : s; }      // act 0: s is the gate itself
@@ -160,7 +180,10 @@ __global__ __launch_bounds__(threads_of(TEAM)) void residual_fwd_kernel(const T*
                 for (int j = 0; j < VALS; ++j) a[j] = 1.f;
             } else if (R.act) {
 #pragma unroll
-                for (int j = 0; j < VALS; ++j) a[j] = sigmoid(a[j]);
+                for (int j = 0; j < VALS; ++j) {
+                    float unused;
+                    a[j] = sigmoid<T>(a[j], unused);
+                }
             }
 #pragma unroll
             for (int j = 0; j < VALS; ++j) yv[j] = __fmaf_rn(R.scale * a[j] * p[j], hv[j] * r1, yv[j]);
@@ -198,6 +221,7 @@ __global__ __launch_bounds__(threads_of(TEAM)) void residual_bwd_kernel(const T*
     constexpr int kTeams = threads_of(TEAM) / TEAM, N = FORM == kBoth ? 3 : 1;
     typedef row_of<T, TEAM, V, VALS, ODD> Row;
     constexpr bool kAhead = VALS == 8 || (VALS == 12 && sizeof(T) == 2);      // registers for a second row? (12 values, fp32: 434 us without, 444 with, 16384 x 4104)
+    constexpr bool kSide = !SUMMED && VALS > 8;                 // (8192 x 8192 fp32: 498 us with one register for gate and slope, 560 with two)
     __shared__ float red[TEAM > 64 ? 2 * N * TEAM / 64 : 1];
     __shared__ float comb[kTeams > 1 ? kTeams : 1][kTeams > 1 ? TEAM * VALS : 1];
     int flip = 0;
@@ -224,15 +248,14 @@ __global__ __launch_bounds__(threads_of(TEAM)) void residual_bwd_kernel(const T*
     for (int64_t un = (int64_t)blockIdx.x * kTeams + team; un < U.units; un += (int64_t)gridDim.x * kTeams) {
         const int64_t grp = un / U.per_share, piece = un - grp * U.per_share;
         const int64_t first = grp * U.share + piece * U.unit, last = min(first + U.unit, (grp + 1) * U.share);
-        float a[VALS], da[VALS], sg[VALS];                      // act(g) (not SUMMED: gate_side(g)), its derivative, the sum of the gate's gradient
+        float a[VALS], da[VALS], sg[VALS];                      // act(g) (kSide: gate_side(g)), its derivative, the sum of the gate's gradient
         if (kAhead) fetch(first);
         if (SUMMED) {
             load_row<T, TEAM, V, VALS, ODD>(gate + grp * R.dim, lane, R.dim, a);
 #pragma unroll
             for (int j = 0; j < VALS; ++j) {
-                const float side = R.act ? gate_side(a[j]) : a[j];
-                a[j] = open_of(side, R.act);
-                da[j] = slope_of(side, R.act);
+                da[j] = 1.f;
+                if (R.act) a[j] = sigmoid<T>(a[j], da[j]);
                 sg[j] = 0.f;
             }
         }
@@ -248,15 +271,17 @@ __global__ __launch_bounds__(threads_of(TEAM)) void residual_bwd_kernel(const T*
             rd.get(dv, lane, R.dim);
             if (kAhead && row + 1 < last) fetch(row + 1);
             if (FORM != kFirst && !SUMMED) {
+#pragma unroll
+                for (int j = 0; j < VALS; ++j) da[j] = 1.f;
                 if (!gate) {
 #pragma unroll
                     for (int j = 0; j < VALS; ++j) a[j] = 1.f;
                 } else if (R.act) {
 #pragma unroll
-                    for (int j = 0; j < VALS; ++j) a[j] = gate_side(a[j]);
+                    for (int j = 0; j < VALS; ++j) a[j] = kSide ? gate_side<T>(a[j]) : sigmoid<T>(a[j], da[j]);
                 }
             }
-            const int act = SUMMED || !gate ? 0 : R.act;
+            const int act = kSide && gate ? R.act : 0;
             float s[N];
 #pragma unroll
             for (int k = 0; k < N; ++k) s[k] = 0.f;
@@ -298,11 +323,14 @@ __global__ __launch_bounds__(threads_of(TEAM)) void residual_bwd_kernel(const T*
             if (dx) Row::put(dx + row * R.dim, lane, R.dim, e);
             if (FORM != kFirst) {
                 float t[VALS];
+                if (kSide)                                      // act(g) is worked out again from gate_side(g): the compiler is not to keep it from above
+#pragma unroll
+                    for (int j = 0; j < VALS; ++j) asm("" : "+v"(a[j]));
 #pragma unroll
                 for (int j = 0; j < VALS; ++j) {
                     const float en = R.scale * e[j] * n[j], open = open_of(a[j], act);
                     sp[j] = __fmaf_rn(open, en, sp[j]);
-                    t[j] = en * p[j] * (SUMMED ? da[j] : slope_of(a[j], act));
+                    t[j] = en * p[j] * (kSide ? slope_of(a[j], act) : da[j]);
                     n[j] = st.x * __fmaf_rn(-c1, n[j], R.scale * open * p[j] * e[j]);
                 }
                 if (dh) Row::put(dh + row * R.dim, lane, R.dim, n);
@@ -471,8 +499,8 @@ template <typename T, typename W, int FORM, bool ODD> int by_team(const Call& c)
         case 256: return launch<T, W, FORM, 256, V, 8, ODD>(c);
         default:
             if (c.a->dim <= 4096) return launch<T, W, FORM, 512, V, 8, ODD>(c);
-            // 12 values per lane up to 6144, in accesses of four (16384 x 5000, backward: 279 us bf16, 543 us fp32; 16 values: 329, 802), 16 above (fp32 always
-            // as an odd width: 8192 x 8190 in 481 us, 8192 x 8192 by the even way in 530)
+            // 12 values per lane up to 6144, in accesses of four (16384 x 5000, backward: 287 us bf16, 555 us fp32; 16 values: 329, 802), 16 above (fp32 always
+            // as an odd width: 8192 x 8192 in 498 us; the even way took 530 where this one took 469)
             return c.a->dim <= 6144 ? launch<T, W, FORM, 512, 4, 12, ODD>(c) : launch<T, W, FORM, 512, V, 16, ODD || V == 4>(c);
     }
 }

@@ -563,3 +563,31 @@ def test_residual_gates_far_open_and_far_closed(shape, gate, dtype, wdtype, monk
     g = torch.Generator().manual_seed(1)
     leaf["gate"] = (torch.rand(gate, generator=g) * 60 - 30).to(dtype).to(dev())
     check(leaf, seeds, 0.75, "sigmoid")
+
+
+@pytest.mark.gpu
+def test_residual_sigmoid_in_32_bits_far_from_zero():
+    """y = scale * sigmoid(g) * n * post with x = 0: a chain of products, so the whole error is relative.  Roundings of 2^-24, counted as half ulps: the norm n < 20 (above) + 1 + 1
+    (its product with h, h's own rounding), the three other products 3, exp(-|g|) with its correction 4 (exp2's own ulp, the constant's and the correction's rounding, the
+    last fma), 1 + t 1, reciprocal 2, t / (1 + t) 1: 33, wherever g is.  Without the correction -80 alone would take 40 more, and the odds that no sample of 40 000 shows it
+    are nil: the sum below is over what a gate near zero (|g| < 1) is off by on the same rows, which holds all but the sigmoid's own part."""
+    g = torch.Generator().manual_seed(2)
+    h = torch.randn(200, 200, generator=g).to(dev())
+    zero, one = torch.zeros_like(h), torch.ones(200, device=dev())
+
+    def off(gate):
+        gate = gate.to(dev())
+        y = trunk.gated_residual(zero, h, gate, one, None, 1.0, "sigmoid", 0.0).double()
+        n = h.double() / torch.sqrt((h.double() ** 2).mean(-1, keepdim=True))
+        want = n / (1 + torch.exp(-gate.double()))
+        return float(((y - want).abs() / want.abs()).max()) / E
+    near, far = off(torch.rand(200, 200, generator=g) * 2 - 1), off(torch.rand(200, 200, generator=g) * 160 - 80)
+    assert far <= 33 and far <= near + 8
+    bad = torch.tensor([float("inf"), -float("inf"), float("nan"), 3e38, -3e38, 104.0, -104.0, 0.0]).repeat(200, 25).to(dev())
+    mine = {"gate": bad.requires_grad_(True), "h": h.clone().requires_grad_(True)}
+    y = trunk.gated_residual(zero, mine["h"], mine["gate"], one, None, 1.0, "sigmoid")
+    n = trunk.gated_residual(zero, h, None, one, None)
+    assert torch.equal(y[:, 0::8], n[:, 0::8]) and torch.equal(y[:, 3::8], n[:, 3::8]) and not y[:, 1::8].any() and not y[:, 4::8].any()
+    assert bool(y[:, 2::8].isnan().all()) and int(y.isnan().sum()) == 200 * 25
+    dgate, = torch.autograd.grad(y, mine["gate"], torch.where(bad.isnan(), 0.0, 1.0).detach())
+    assert not dgate[:, :2].any() and not dgate[:, 3:5].any() and bool(dgate[:, 7].ne(0).all())
