@@ -70,6 +70,11 @@ void one_device(std::initializer_list<const Tensor*> ts) {
         TORCH_CHECK(t->device() == first.device(), "expected every tensor on ", first.device(), ", got one on ", t->device());
     }
 }
+// A kernel call carries no forward-mode tangent along: its output would have none, which is the tangent zero.
+void no_tangents(const char* what, std::initializer_list<const Tensor*> ts) {
+    for (const Tensor* t : ts)
+        TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(), what, " has no forward-mode derivative: call it on tensors without a tangent (torch.autograd.forward_ad.unpack_dual)");
+}
 void ok(int64_t rc, const char* what) {
     if (rc == 0) return;
     TORCH_CHECK(false, what, " failed: ", rc == NVP_ERR_BADARG ? std::string("bad argument") : rc == NVP_ERR_UNSUPPORTED ? std::string("unsupported configuration") : "hipError " + std::to_string(rc));
@@ -127,6 +132,7 @@ struct Lookup : torch::autograd::Function<Lookup> {
         return lookup_run(ids, table, scale, (at::ScalarType)type);
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        no_tangents("the gradient of lookup", {&grads[0]});
         Tensor ids = ctx->get_saved_variables()[0], dout = grads[0].contiguous();
         const int64_t codes = ctx->saved_data["codes"].toInt(), dim = dout.size(-1), n = ids.numel();
         const auto type = (at::ScalarType)ctx->saved_data["type"].toInt();
@@ -146,6 +152,7 @@ Tensor lookup(const Tensor& ids, const Tensor& table, double scale, std::optiona
     const at::ScalarType type = dtype.value_or(table.scalar_type());
     TORCH_CHECK(type_number(type) >= 0 && (table.scalar_type() == at::kFloat || type == table.scalar_type()), "lookup: a ", table.scalar_type(), " table cannot be read as ", type);
     TORCH_CHECK(std::isfinite(scale), "lookup: scale must be finite, got ", scale);
+    no_tangents("lookup", {&table});
     one_device({&table, &ids});
     const c10::DeviceGuard guard(table.device());
     if (verify && ids.numel()) {
@@ -201,6 +208,7 @@ struct Residual : torch::autograd::Function<Residual> {
         variable_list out(9);
         const Tensor dy = s.h.defined() ? dense(grads[0]) : Tensor(), du = s.next.defined() ? dense(grads.back()) : Tensor();
         if (!dy.defined() && !du.defined()) return out;
+        no_tangents("the gradient of gated_residual", {&dy, &du});
         const c10::DeviceGuard guard(s.x.device());
         const Tensor* in[5] = {&s.x, &s.h, &s.gate, &s.post, &s.next};
         const bool empty = s.x.numel() == 0;
@@ -246,6 +254,7 @@ int64_t gate_rows(const Tensor& x, const Tensor& gate) {
 variable_list residual(const Tensor& x, const Tensor& h, const Tensor& gate, const Tensor& post, const Tensor& next, double scale, int64_t act, double eps, const char* what) {
     TORCH_CHECK(eps >= 0 && std::isfinite(eps), what, ": eps must be finite and not negative, got ", eps);
     const int64_t grows = gate.defined() ? gate_rows(x, gate) : 1;
+    no_tangents(what, {&x, &h, &gate, &post, &next});
     one_device({&x, &h, &gate, &post, &next});
     const c10::DeviceGuard guard(x.device());
     const Tensor xc = dense(x), hc = dense(h), gc = dense(gate), pc = dense(post), nc = dense(next);
@@ -286,6 +295,7 @@ Tensor linear8(const Tensor& x, const Tensor& q, const Tensor& e, const Maybe& b
     TORCH_CHECK(!b.defined() || (b.scalar_type() == x.scalar_type() && b.dim() == 1 && b.size(0) == n), "linear8: bias must be ", x.scalar_type(), " [", n, "], got ",
                 b.defined() ? b.scalar_type() : x.scalar_type(), " ", b.defined() ? b.sizes() : x.sizes());
     TORCH_CHECK_NOT_IMPLEMENTED(!wants_grad({&x, &b}), "linear8 is an inference-only path: call it under torch.no_grad() or on tensors that need no gradient");
+    no_tangents("linear8", {&x, &b});
     one_device({&x, &q, &e, &b});
     TORCH_CHECK(q.is_contiguous() && e.is_contiguous(), "linear8: expected a contiguous weight and scales");
     const c10::DeviceGuard guard(x.device());

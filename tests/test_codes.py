@@ -427,3 +427,25 @@ def test_a_missing_binding_is_an_error(monkeypatch, tmp_path):
     monkeypatch.setattr(L, "_HERE", str(tmp_path))
     with pytest.raises(RuntimeError, match="the binding is not built"):
         codes.lookup(torch.zeros(3, dtype=torch.int64), torch.zeros(4, 5))
+
+
+def test_lookup_refuses_forward_mode_tangents():
+    from torch.autograd import forward_ad
+    with forward_ad.dual_level():
+        table = forward_ad.make_dual(torch.zeros(4, 5), torch.ones(4, 5))
+        with pytest.raises(NotImplementedError, match="lookup has no forward-mode derivative"):
+            codes.lookup(torch.zeros(3, dtype=torch.int64), table)
+        with pytest.raises(RuntimeError, match="HIP device"):            # without its tangent: taken, and what is refused is the device
+            codes.lookup(torch.zeros(3, dtype=torch.int64), forward_ad.unpack_dual(table).primal)
+
+
+@pytest.mark.gpu
+def test_lookup_refuses_a_gradient_with_a_tangent():
+    from torch.autograd import forward_ad
+    table = torch.randn(4, 5, device=dev(), requires_grad=True)
+    out = codes.lookup(torch.tensor([1, 1, 3], device=dev()), table)
+    with forward_ad.dual_level():
+        with pytest.raises(NotImplementedError, match="the gradient of lookup has no forward-mode derivative"):
+            torch.autograd.grad(out, table, forward_ad.make_dual(torch.ones_like(out), torch.ones_like(out)))
+        with pytest.raises(NotImplementedError):
+            codes.lookup(torch.tensor([1], device=dev()), forward_ad.make_dual(table, torch.ones_like(table)))

@@ -342,3 +342,12 @@ def test_linear8_few_columns_scales_non_finite_values_and_replays():
         want = Q.linear8(mine, q, e)
         torch.cuda.synchronize()
         assert torch.equal(out, want)
+
+
+def test_linear8_refuses_forward_mode_tangents():
+    from torch.autograd import forward_ad
+    x, q, e, b = torch.zeros(3, 200), torch.zeros(5, 256, dtype=torch.float8_e4m3fn), torch.zeros(1, 2, dtype=torch.uint8), torch.zeros(5)
+    with forward_ad.dual_level():
+        for args in ((forward_ad.make_dual(x, x.clone()), q, e, None), (x, q, e, forward_ad.make_dual(b, b.clone()))):
+            with pytest.raises(NotImplementedError, match="linear8 has no forward-mode derivative"):
+                Q.linear8(*args)

@@ -591,3 +591,28 @@ def test_residual_sigmoid_in_32_bits_far_from_zero():
     assert bool(y[:, 2::8].isnan().all()) and int(y.isnan().sum()) == 200 * 25
     dgate, = torch.autograd.grad(y, mine["gate"], torch.where(bad.isnan(), 0.0, 1.0).detach())
     assert not dgate[:, :2].any() and not dgate[:, 3:5].any() and bool(dgate[:, 7].ne(0).all())
+
+
+def test_refuses_forward_mode_tangents():
+    from torch.autograd import forward_ad
+    x, w, g = torch.zeros(2, 8), torch.ones(8), torch.zeros(1, 8)
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))      # noqa: E731
+        for args in ((dual(x), w), (x, dual(w))):
+            with pytest.raises(NotImplementedError, match="pre_norm has no forward-mode derivative"):
+                trunk.pre_norm(*args)
+        whole = (x, x, g, w, w)
+        for k in range(5):
+            with pytest.raises(NotImplementedError, match="gated_residual has no forward-mode derivative"):
+                trunk.gated_residual(*(dual(t) if i == k else t for i, t in enumerate(whole)))
+
+
+@pytest.mark.gpu
+def test_residual_refuses_a_gradient_with_a_tangent():
+    from torch.autograd import forward_ad
+    x, w = torch.randn(3, 40, device=dev(), requires_grad=True), torch.ones(40, device=dev())
+    y, u = trunk.gated_residual(x, x, None, w, w)
+    with forward_ad.dual_level():
+        for out in (y, u):
+            with pytest.raises(NotImplementedError, match="the gradient of gated_residual has no forward-mode derivative"):
+                torch.autograd.grad(out, x, forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y)), retain_graph=True)
