@@ -7,9 +7,11 @@
 #include <dlfcn.h>
 
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 #include <ATen/ATen.h>
 
@@ -75,6 +77,13 @@ void no_tangents(const char* what, std::initializer_list<const Tensor*> ts) {
     for (const Tensor* t : ts)
         TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(), what, " has no forward-mode derivative: call it on tensors without a tangent (torch.autograd.forward_ad.unpack_dual)");
 }
+// A tracer sees the output's allocation and not the kernel: what it records would return uninitialised memory.  (A HIP graph captures the kernel itself.)
+void not_recorded(const char* what) {
+    typedef c10::impl::TorchDispatchModeKey Key;
+    bool recorded = torch::jit::tracer::isTracing();
+    for (const Key k : {Key::PROXY, Key::FAKE, Key::FUNCTIONAL}) recorded = recorded || c10::impl::TorchDispatchModeTLS::get_mode(k).has_value();
+    TORCH_CHECK(!recorded, what, " cannot be recorded by torch.jit.trace, torch.fx or torch.export: call it outside the traced function");
+}
 void ok(int64_t rc, const char* what) {
     if (rc == 0) return;
     TORCH_CHECK(false, what, " failed: ", rc == NVP_ERR_BADARG ? std::string("bad argument") : rc == NVP_ERR_UNSUPPORTED ? std::string("unsupported configuration") : "hipError " + std::to_string(rc));
@@ -132,6 +141,7 @@ struct Lookup : torch::autograd::Function<Lookup> {
         return lookup_run(ids, table, scale, (at::ScalarType)type);
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        not_recorded("the gradient of lookup");
         no_tangents("the gradient of lookup", {&grads[0]});
         Tensor ids = ctx->get_saved_variables()[0], dout = grads[0].contiguous();
         const int64_t codes = ctx->saved_data["codes"].toInt(), dim = dout.size(-1), n = ids.numel();
@@ -152,6 +162,7 @@ Tensor lookup(const Tensor& ids, const Tensor& table, double scale, std::optiona
     const at::ScalarType type = dtype.value_or(table.scalar_type());
     TORCH_CHECK(type_number(type) >= 0 && (table.scalar_type() == at::kFloat || type == table.scalar_type()), "lookup: a ", table.scalar_type(), " table cannot be read as ", type);
     TORCH_CHECK(std::isfinite(scale), "lookup: scale must be finite, got ", scale);
+    not_recorded("lookup");
     no_tangents("lookup", {&table});
     one_device({&table, &ids});
     const c10::DeviceGuard guard(table.device());
@@ -208,6 +219,7 @@ struct Residual : torch::autograd::Function<Residual> {
         variable_list out(9);
         const Tensor dy = s.h.defined() ? dense(grads[0]) : Tensor(), du = s.next.defined() ? dense(grads.back()) : Tensor();
         if (!dy.defined() && !du.defined()) return out;
+        not_recorded("the gradient of gated_residual");
         no_tangents("the gradient of gated_residual", {&dy, &du});
         const c10::DeviceGuard guard(s.x.device());
         const Tensor* in[5] = {&s.x, &s.h, &s.gate, &s.post, &s.next};
@@ -254,6 +266,7 @@ int64_t gate_rows(const Tensor& x, const Tensor& gate) {
 variable_list residual(const Tensor& x, const Tensor& h, const Tensor& gate, const Tensor& post, const Tensor& next, double scale, int64_t act, double eps, const char* what) {
     TORCH_CHECK(eps >= 0 && std::isfinite(eps), what, ": eps must be finite and not negative, got ", eps);
     const int64_t grows = gate.defined() ? gate_rows(x, gate) : 1;
+    not_recorded(what);
     no_tangents(what, {&x, &h, &gate, &post, &next});
     one_device({&x, &h, &gate, &post, &next});
     const c10::DeviceGuard guard(x.device());
@@ -295,6 +308,7 @@ Tensor linear8(const Tensor& x, const Tensor& q, const Tensor& e, const Maybe& b
     TORCH_CHECK(!b.defined() || (b.scalar_type() == x.scalar_type() && b.dim() == 1 && b.size(0) == n), "linear8: bias must be ", x.scalar_type(), " [", n, "], got ",
                 b.defined() ? b.scalar_type() : x.scalar_type(), " ", b.defined() ? b.sizes() : x.sizes());
     TORCH_CHECK_NOT_IMPLEMENTED(!wants_grad({&x, &b}), "linear8 is an inference-only path: call it under torch.no_grad() or on tensors that need no gradient");
+    not_recorded("linear8");
     no_tangents("linear8", {&x, &b});
     one_device({&x, &q, &e, &b});
     TORCH_CHECK(q.is_contiguous() && e.is_contiguous(), "linear8: expected a contiguous weight and scales");
@@ -316,6 +330,7 @@ Tensor linear8(const Tensor& x, const Tensor& q, const Tensor& e, const Maybe& b
 PYBIND11_MODULE(nvp_binding, m) {
     namespace py = pybind11;
     m.def("bind", &bind);
+    m.def("not_recorded", &not_recorded);
     m.def("lookup", &lookup, py::call_guard<py::gil_scoped_release>());
     m.def("pre_norm", &pre_norm, py::call_guard<py::gil_scoped_release>());
     m.def("gated_residual", &gated_residual, py::call_guard<py::gil_scoped_release>());

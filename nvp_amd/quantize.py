@@ -83,6 +83,7 @@ def quantize_blocks(v: torch.Tensor, rows: int = 1):
     if rows not in (1, BLOCK):
         raise RuntimeError(f"quantize_blocks: a block has 1 or {BLOCK} rows, got {rows}")
     ty = L.stream_type(v, "quantize_blocks")
+    L.binding().not_recorded("quantize_blocks")
     with L.on_device_of(v):
         v = v.detach().contiguous()
         r, k = v.shape
@@ -105,6 +106,7 @@ def dequantize_blocks(q: torch.Tensor, e: torch.Tensor, k: int, rows: int = 1, d
     _check_blocks(q, e, k, rows, "dequantize_blocks")
     if rows not in (1, BLOCK):
         raise RuntimeError(f"dequantize_blocks: a block has 1 or {BLOCK} rows, got {rows}")
+    L.binding().not_recorded("dequantize_blocks")
     with L.on_device_of(q, e):
         out = torch.empty((q.shape[0], k), device=q.device, dtype=dtype)
         ty = L.stream_type(out, "dequantize_blocks")

@@ -616,3 +616,33 @@ def test_residual_refuses_a_gradient_with_a_tangent():
         for out in (y, u):
             with pytest.raises(NotImplementedError, match="the gradient of gated_residual has no forward-mode derivative"):
                 torch.autograd.grad(out, x, forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y)), retain_graph=True)
+
+
+@pytest.mark.filterwarnings("ignore")
+def test_conditioning_operators_refuse_to_be_traced():
+    """A tracer would keep the output's allocation and drop the kernel."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    x, w, ids, table = torch.zeros(2, 8), torch.ones(8), torch.zeros(2, dtype=torch.int64), torch.zeros(3, 8)
+    q, e = torch.zeros(5, 128, dtype=torch.float8_e4m3fn), torch.zeros(1, 1, dtype=torch.uint8)
+    for name, f in (("pre_norm", lambda t: trunk.pre_norm(t, w)), ("gated_residual", lambda t: trunk.gated_residual(t, t, None, w)), ("lookup", lambda t: codes.lookup(ids, t)),
+                    ("linear8", lambda t: quantize.linear8(t, q, e)), ("quantize_blocks", lambda t: quantize.quantize_blocks(t)[0]),
+                    ("dequantize_blocks", lambda t: quantize.dequantize_blocks(q, e, 100, 128) + t.sum())):
+        arg = table if name == "lookup" else x
+        for record in (lambda: torch.jit.trace(f, arg, check_trace=False), lambda: make_fx(f)(arg), lambda: make_fx(f, tracing_mode="fake")(arg)):
+            with pytest.raises(RuntimeError, match=f"{name} cannot be recorded"):
+                record()
+        with pytest.raises(RuntimeError, match="HIP device"):
+            f(arg)
+
+
+@pytest.mark.gpu
+def test_conditioning_operators_traced_gradients_and_compiled_calls():
+    from torch.fx.experimental.proxy_tensor import make_fx
+    x, w = torch.randn(3, 40, device=dev(), requires_grad=True), torch.ones(40, device=dev())
+    table = torch.randn(5, 8, device=dev(), requires_grad=True)
+    for out, leaf in ((trunk.pre_norm(x, w), x), (codes.lookup(torch.tensor([1, 2], device=dev()), table), table)):
+        with pytest.raises(RuntimeError, match="cannot be recorded"):
+            make_fx(lambda d: torch.autograd.grad(out, leaf, d)[0])(torch.ones_like(out))
+    f = lambda t: trunk.pre_norm(t, w) * 2      # noqa: E731
+    with torch.no_grad():
+        assert torch.equal(torch.compile(f, backend="eager")(x), f(x))      # torch.compile leaves the call out of its graphs and makes it as it is
