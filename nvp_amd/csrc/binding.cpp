@@ -161,7 +161,7 @@ Tensor lookup(const Tensor& ids, const Tensor& table, double scale, std::optiona
     stream_type(table, "lookup");
     const at::ScalarType type = dtype.value_or(table.scalar_type());
     TORCH_CHECK(type_number(type) >= 0 && (table.scalar_type() == at::kFloat || type == table.scalar_type()), "lookup: a ", table.scalar_type(), " table cannot be read as ", type);
-    TORCH_CHECK(std::isfinite(scale), "lookup: scale must be finite, got ", scale);
+    TORCH_CHECK(std::isfinite((float)scale), "lookup: scale must be finite in 32 bits, got ", scale);
     not_recorded("lookup");
     no_tangents("lookup", {&table});
     one_device({&table, &ids});
@@ -264,7 +264,7 @@ int64_t gate_rows(const Tensor& x, const Tensor& gate) {
     return rows;
 }
 variable_list residual(const Tensor& x, const Tensor& h, const Tensor& gate, const Tensor& post, const Tensor& next, double scale, int64_t act, double eps, const char* what) {
-    TORCH_CHECK(eps >= 0 && std::isfinite(eps), what, ": eps must be finite and not negative, got ", eps);
+    TORCH_CHECK(eps >= 0 && std::isfinite((float)eps), what, ": eps must be finite in 32 bits and not negative, got ", eps);
     const int64_t grows = gate.defined() ? gate_rows(x, gate) : 1;
     not_recorded(what);
     no_tangents(what, {&x, &h, &gate, &post, &next});
@@ -289,7 +289,7 @@ variable_list gated_residual(const Tensor& x, const Tensor& h, const Maybe& gate
         check_weight(*next, x, what);
         TORCH_CHECK(next->scalar_type() == post.scalar_type(), "gated_residual: the two weights must be of one type, got ", post.scalar_type(), " and ", next->scalar_type());
     }
-    TORCH_CHECK(std::isfinite(scale), "gated_residual: scale must be finite, got ", scale);
+    TORCH_CHECK(std::isfinite((float)scale), "gated_residual: scale must be finite in 32 bits, got ", scale);
     return residual(x, h, gate.value_or(Tensor()), post, next.value_or(Tensor()), scale, act, eps, what);
 }
 

@@ -646,3 +646,17 @@ def test_conditioning_operators_traced_gradients_and_compiled_calls():
     f = lambda t: trunk.pre_norm(t, w) * 2      # noqa: E731
     with torch.no_grad():
         assert torch.equal(torch.compile(f, backend="eager")(x), f(x))      # torch.compile leaves the call out of its graphs and makes it as it is
+
+
+def test_factors_beyond_32_bits_are_refused():
+    """The kernels take scale and eps in 32 bits, where these would be infinite."""
+    x, w = torch.zeros(2, 8), torch.ones(8)
+    for big in (1e39, -1e39, 1.7e308):
+        with pytest.raises(RuntimeError, match="scale must be finite"):
+            trunk.gated_residual(x, x, None, w, scale=big)
+        with pytest.raises(RuntimeError, match="scale must be finite"):
+            codes.lookup(torch.zeros(3, dtype=torch.int64), x, scale=big)
+        with pytest.raises(RuntimeError, match="eps must be finite"):
+            trunk.pre_norm(x, w, eps=abs(big))
+    with pytest.raises(RuntimeError, match="HIP device"):
+        trunk.gated_residual(x, x, None, w, scale=3e38, eps=3e38)
