@@ -90,8 +90,9 @@ void ok(int64_t rc, const char* what) {
 }
 void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
-Tensor dense(const Tensor& t) { return t.defined() ? t.contiguous() : t; }
-Tensor dense(const Maybe& t) { return t && t->defined() ? t->contiguous() : Tensor(); }
+// rows side by side, values as they read (a view that negates, as the imaginary part of a conjugate, keeps its values' other sign in memory)
+Tensor dense(const Tensor& t) { return t.defined() ? t.resolve_neg().contiguous() : t; }
+Tensor dense(const Maybe& t) { return t ? dense(*t) : Tensor(); }
 Tensor workspace(int64_t bytes, const Tensor& like, const char* what) {
     if (bytes < 0) ok(bytes, what);
     return bytes ? at::empty({bytes}, like.options().dtype(at::kByte)) : Tensor();
@@ -143,7 +144,7 @@ struct Lookup : torch::autograd::Function<Lookup> {
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         not_recorded("the gradient of lookup");
         no_tangents("the gradient of lookup", {&grads[0]});
-        Tensor ids = ctx->get_saved_variables()[0], dout = grads[0].contiguous();
+        Tensor ids = ctx->get_saved_variables()[0], dout = dense(grads[0]);
         const int64_t codes = ctx->saved_data["codes"].toInt(), dim = dout.size(-1), n = ids.numel();
         const auto type = (at::ScalarType)ctx->saved_data["type"].toInt();
         const c10::DeviceGuard guard(dout.device());
@@ -170,7 +171,7 @@ Tensor lookup(const Tensor& ids, const Tensor& table, double scale, std::optiona
         const int64_t most = ids.max().item().toLong();
         TORCH_CHECK_INDEX(most < table.size(0), "lookup: id ", most, " in a table of ", table.size(0), " codes");
     }
-    const Tensor i = ids.contiguous(), t = table.contiguous();
+    const Tensor i = dense(ids), t = dense(table);
     return wants_grad({&t}) ? Lookup::apply(i, t, scale, (int64_t)type) : lookup_run(i, t, scale, type);
 }
 
@@ -313,7 +314,7 @@ Tensor linear8(const Tensor& x, const Tensor& q, const Tensor& e, const Maybe& b
     one_device({&x, &q, &e, &b});
     TORCH_CHECK(q.is_contiguous() && e.is_contiguous(), "linear8: expected a contiguous weight and scales");
     const c10::DeviceGuard guard(x.device());
-    const Tensor xc = x.contiguous();
+    const Tensor xc = dense(x);
     const int64_t rows = xc.numel() / k;
     auto shape = x.sizes().vec();
     shape.back() = n;

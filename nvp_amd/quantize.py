@@ -85,7 +85,7 @@ def quantize_blocks(v: torch.Tensor, rows: int = 1):
     ty = L.stream_type(v, "quantize_blocks")
     L.binding().not_recorded("quantize_blocks")
     with L.on_device_of(v):
-        v = v.detach().contiguous()
+        v = v.detach().resolve_neg().contiguous()
         r, k = v.shape
         q = torch.empty((r, _kblocks(k) * BLOCK), device=v.device, dtype=torch.float8_e4m3fn)
         e = torch.empty(((r + rows - 1) // rows, _kblocks(k)), device=v.device, dtype=torch.uint8)

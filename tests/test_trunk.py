@@ -660,3 +660,27 @@ def test_factors_beyond_32_bits_are_refused():
             trunk.pre_norm(x, w, eps=abs(big))
     with pytest.raises(RuntimeError, match="HIP device"):
         trunk.gated_residual(x, x, None, w, scale=3e38, eps=3e38)
+
+
+@pytest.mark.gpu
+def test_views_that_negate_are_read_as_they_are():
+    """A view with torch's negative bit (the imaginary part of a conjugate) holds the other sign in memory."""
+    neg = lambda t: torch._neg_view(t)      # noqa: E731
+    x, h, w, ids = torch.randn(5, 24, device=dev()), torch.randn(5, 24, device=dev()), torch.randn(24, device=dev()), torch.tensor([3, 0, 4, 4], device=dev())
+    for a, b in zip(trunk.gated_residual(neg(x), neg(h), neg(x), neg(w), neg(w), 0.5, "sigmoid"), trunk.gated_residual(-x, -h, -x, -w, -w, 0.5, "sigmoid")):
+        assert torch.equal(a, b)
+    assert torch.equal(trunk.pre_norm(neg(x), w), trunk.pre_norm(-x, w))
+    assert torch.equal(codes.lookup(ids, neg(x)), -x[ids]) and torch.equal(codes.lookup(neg(-ids), x), x[ids])
+    one = torch.complex(x[:, :1], h[:, :1]).conj().imag
+    assert one.is_neg() and torch.equal(codes.lookup(ids, one), -h[ids, :1])
+    (q, e), (p, f) = quantize.quantize_blocks(neg(x), 1), quantize.quantize_blocks(-x, 1)
+    assert torch.equal(q.view(torch.uint8), p.view(torch.uint8)) and torch.equal(e, f)
+    q, e = quantize.quantize_blocks(h, 128)
+    assert torch.equal(quantize.linear8(neg(x), q, e, neg(x[:, 0].clone())), quantize.linear8(-x, q, e, -x[:, 0]))
+    leaf = x.clone().requires_grad_(True)
+    got, = torch.autograd.grad(trunk.pre_norm(neg(leaf), w), leaf, neg(h))
+    want, = torch.autograd.grad(trunk.pre_norm(-leaf, w), leaf, -h)
+    assert torch.equal(got, want)
+    table = x.clone().requires_grad_(True)
+    got, = torch.autograd.grad(codes.lookup(ids, table), table, neg(h[:4]))
+    assert torch.equal(got, torch.autograd.grad(codes.lookup(ids, table), table, -h[:4])[0])
