@@ -123,7 +123,8 @@ def linear8(x: torch.Tensor, q: torch.Tensor, e: torch.Tensor, bias: torch.Tenso
 
 
 class Linear8(nn.Module):
-    """nn.Linear for 8-bit evaluation: holds the weight in block form (buffers `q`, `e`; 8 + 1 / 2048 bits per weight) and the bias."""
+    """nn.Linear for 8-bit evaluation: holds the weight in block form (buffers `q`, `e`; 8 + 1 / 2048 bits per weight) and the bias.  The streams have the bias's
+    type: a cast of the module (`half()`, `to(dtype)`) changes the bias and leaves q and e as they are."""
 
     def __init__(self, in_features: int, out_features: int, bias: bool = True, dtype: torch.dtype = torch.float32, device=None):
         super().__init__()
@@ -143,6 +144,18 @@ class Linear8(nn.Module):
         if b is not None:
             m.bias = b.detach().clone()
         return m
+
+    def _apply(self, fn, recurse=True):
+        """Moves go for everything; casts (`half()`, `to(dtype)`) for the bias alone: q and e are bytes, whatever type the streams have."""
+        held = {n: self._buffers[n] for n in ("q", "e")}
+        try:
+            self._buffers.update(q=None, e=None)
+            super()._apply(fn, recurse)
+            moved = {n: fn(t.view(torch.uint8)) for n, t in held.items()}
+            held = {n: (m if m.dtype == torch.uint8 else held[n].view(torch.uint8).to(m.device)).view(held[n].dtype) for n, m in moved.items()}
+        finally:
+            self._buffers.update(held)
+        return self
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         return linear8(x, self.q, self.e, self.bias)

@@ -351,3 +351,49 @@ def test_linear8_refuses_forward_mode_tangents():
         for args in ((forward_ad.make_dual(x, x.clone()), q, e, None), (x, q, e, forward_ad.make_dual(b, b.clone()))):
             with pytest.raises(NotImplementedError, match="linear8 has no forward-mode derivative"):
                 Q.linear8(*args)
+
+
+@pytest.mark.parametrize("cast", [lambda m: m.half(), lambda m: m.bfloat16(), lambda m: m.double().float(), lambda m: m.to(torch.float16), lambda m: m.to("cpu", torch.bfloat16),
+                                  lambda m: m.type(torch.float16), lambda m: m.to("meta"), lambda m: m.to_empty(device="cpu"), lambda m: torch.nn.Sequential(m).half()[0]])
+def test_linear8_module_keeps_its_weight_through_casts(cast):
+    """Casts concern the bias: the weight's bytes and scales stay what they are, wherever the module is in a tree."""
+    m = Q.Linear8(200, 130)
+    raw = torch.arange(130 * 256).to(torch.uint8).view(130, 256)
+    m.q, m.e, m.bias = raw.view(torch.float8_e4m3fn), torch.tensor([[1, 2], [3, 4]], dtype=torch.uint8), torch.arange(130.0)
+    names = list(m.state_dict())
+    m = cast(m)
+    assert m.q.dtype == torch.float8_e4m3fn and m.e.dtype == torch.uint8 and m.q.shape == (130, 256) and m.e.shape == (2, 2)
+    assert m.q.device == m.e.device == m.bias.device and list(m.state_dict()) == names
+    if m.q.device.type == "cpu" and not cast.__code__.co_names[0] == "to_empty":
+        assert torch.equal(m.q.view(torch.uint8), raw) and m.e.tolist() == [[1, 2], [3, 4]] and torch.equal(m.bias.float(), torch.arange(130.0))
+    assert m.bias.dtype != torch.float64
+    bare = Q.Linear8(5, 5, bias=False).half()
+    assert bare.bias is None and bare.q.dtype == torch.float8_e4m3fn
+
+
+def test_linear8_module_is_whole_after_a_move_that_fails():
+    m = Q.Linear8(200, 130)
+    q, e = m.q, m.e
+
+    def fails(t):
+        raise ValueError("no")
+    with pytest.raises(ValueError):
+        m._apply(fails)
+    assert m.q is q and m.e is e
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_linear8_module_of_every_stream_type(dtype):
+    """An fp32 layer's 8-bit form, cast to the stream's type: the weight in the same bytes, and the call's result that of the operator."""
+    torch.manual_seed(1)
+    lin = torch.nn.Linear(300, 70).to(dev())
+    m = Q.Linear8.from_linear(lin)
+    q, e = m.q.clone(), m.e.clone()
+    m = m.to(dtype).cpu().to(dev())
+    x = torch.randn(40, 300, device=dev()).to(dtype)
+    assert torch.equal(m.q.view(torch.uint8), q.view(torch.uint8)) and torch.equal(m.e, e)
+    y = m(x)
+    assert y.dtype == dtype and torch.equal(y, Q.linear8(x, q, e, lin.bias.detach().to(dtype)))
+    want, s = plain_linear(x.cpu(), lin.weight, lin.bias.detach().to(dtype))
+    within(y, want, s, 300, dtype)

@@ -684,3 +684,22 @@ def test_views_that_negate_are_read_as_they_are():
     table = x.clone().requires_grad_(True)
     got, = torch.autograd.grad(codes.lookup(ids, table), table, neg(h[:4]))
     assert torch.equal(got, torch.autograd.grad(codes.lookup(ids, table), table, -h[:4])[0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [B16, F16])
+def test_trunk_in_eight_bits_on_16_bit_streams(dtype):
+    """to_8bit() and a cast, in either order: the layers' weights are quantised from what the trunk holds at that time."""
+    torch.manual_seed(3)
+    stack = trunk.Trunk(96, 2).to(dev())
+    x = torch.randn(20, 96, device=dev()).to(dtype)
+    with torch.no_grad():
+        got = stack.to_8bit().to(dtype)(x)
+        want = stack.to_8bit()(x.float())
+        assert got.dtype == dtype
+        # the same 8-bit weights; streams rounded to 16 bits some eight times a block, and activations that then round to another e4m3 number (2^-4) where they lay near a
+        # border, a share of about 2^-9 / 2^-4 of them: 2 blocks * (8 * 2^-9 + 3 products * 2^-4 * (2^-5)^0.5) = 0.1 of the latent's size at the most
+        assert float((got.float() - want).norm() / want.norm()) <= 0.1
+        late = trunk.Trunk(96, 2).to(dev())
+        late.load_state_dict(stack.state_dict())
+        assert late.to(dtype).to_8bit()(x).dtype == dtype
