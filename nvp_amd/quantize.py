@@ -108,9 +108,10 @@ def dequantize_blocks(q: torch.Tensor, e: torch.Tensor, k: int, rows: int = 1, d
         raise RuntimeError(f"dequantize_blocks: a block has 1 or {BLOCK} rows, got {rows}")
     L.binding().not_recorded("dequantize_blocks")
     with L.on_device_of(q, e):
+        q, e = q.contiguous(), e.contiguous()                       # held until the launch: a copy that is let go is handed to the next one
         out = torch.empty((q.shape[0], k), device=q.device, dtype=dtype)
         ty = L.stream_type(out, "dequantize_blocks")
-        L.check(L.load().nvp_dequantize_blocks(L.ptr(q.contiguous(), q.dtype), L.ptr(e.contiguous(), e.dtype), L.ptr(out, dtype), ty, q.shape[0], k, rows, L.stream_ptr()),
+        L.check(L.load().nvp_dequantize_blocks(L.ptr(q, q.dtype), L.ptr(e, e.dtype), L.ptr(out, dtype), ty, q.shape[0], k, rows, L.stream_ptr()),
                 "nvp_dequantize_blocks")
     return out
 

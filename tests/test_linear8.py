@@ -397,3 +397,23 @@ def test_linear8_module_of_every_stream_type(dtype):
     assert y.dtype == dtype and torch.equal(y, Q.linear8(x, q, e, lin.bias.detach().to(dtype)))
     want, s = plain_linear(x.cpu(), lin.weight, lin.bias.detach().to(dtype))
     within(y, want, s, 300, dtype)
+
+
+def other_layouts(q, e):
+    """The block form (q, e) in other places: a slice of wider rows, a contiguous matrix at an odd address, a transposed one; scales transposed."""
+    raw = q.view(torch.uint8)
+    r, k = raw.shape
+    wide = torch.zeros(r, k + 600, device=q.device, dtype=torch.uint8)
+    wide[:, 3:3 + k] = raw
+    odd = torch.zeros(r * k + 1, device=q.device, dtype=torch.uint8)[1:].view(r, k)
+    odd.copy_(raw)
+    turned, scales = raw.t().contiguous().t(), e.t().contiguous().t()
+    assert odd.is_contiguous() and odd.data_ptr() % 16 == 1 and not turned.is_contiguous() and not scales.is_contiguous()
+    return [(t.view(torch.float8_e4m3fn), scales) for t in (wide[:, 3:3 + k], odd, turned)]
+
+
+@pytest.mark.gpu
+def test_dequantize_blocks_of_any_stride_and_alignment():
+    q, e = Q.quantize_blocks(torch.randn(140, 300, device=dev()), 128)
+    want = Q.dequantize_blocks(q, e, 300, 128)
+    assert all(torch.equal(Q.dequantize_blocks(p, f, 300, 128), want) for p, f in other_layouts(q, e))
