@@ -16,6 +16,7 @@
 #include <ATen/ATen.h>
 
 #include <cmath>
+#include <cstdint>
 #include <string>
 #include <tuple>
 #include <vector>
@@ -312,9 +313,10 @@ Tensor linear8(const Tensor& x, const Tensor& q, const Tensor& e, const Maybe& b
     not_recorded("linear8");
     no_tangents("linear8", {&x, &b});
     one_device({&x, &q, &e, &b});
-    TORCH_CHECK(q.is_contiguous() && e.is_contiguous(), "linear8: expected a contiguous weight and scales");
     const c10::DeviceGuard guard(x.device());
-    const Tensor xc = dense(x);
+    const Tensor xc = dense(x), ec = e.contiguous();
+    Tensor qc = q.contiguous();
+    if (reinterpret_cast<uintptr_t>(qc.data_ptr()) % 16) qc = qc.clone();      // (the kernel's 16-byte loads; the allocator's addresses are aligned)
     const int64_t rows = xc.numel() / k;
     auto shape = x.sizes().vec();
     shape.back() = n;
@@ -322,7 +324,7 @@ Tensor linear8(const Tensor& x, const Tensor& q, const Tensor& e, const Maybe& b
     if (rows == 0) return y;
     const int64_t need = api.linear8_ws(rows, k, n);
     Tensor ws = workspace(need, x, "nvp_linear8_workspace_bytes");
-    ok(api.linear8(ptr(xc), type, static_cast<const uint8_t*>(ptr(q)), static_cast<const uint8_t*>(ptr(e)), ptr(b), ptr(y), rows, k, n, ptr(ws), need, stream_of(x)), "nvp_linear8");
+    ok(api.linear8(ptr(xc), type, static_cast<const uint8_t*>(ptr(qc)), static_cast<const uint8_t*>(ptr(ec)), ptr(b), ptr(y), rows, k, n, ptr(ws), need, stream_of(x)), "nvp_linear8");
     return y;
 }
 

@@ -417,3 +417,12 @@ def test_dequantize_blocks_of_any_stride_and_alignment():
     q, e = Q.quantize_blocks(torch.randn(140, 300, device=dev()), 128)
     want = Q.dequantize_blocks(q, e, 300, 128)
     assert all(torch.equal(Q.dequantize_blocks(p, f, 300, 128), want) for p, f in other_layouts(q, e))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [3, 100, 5000])
+def test_linear8_weights_of_any_stride_and_alignment(m):
+    x = torch.randn(m, 300, device=dev())
+    q, e = Q.quantize_blocks(torch.randn(140, 300, device=dev()), 128)
+    want = Q.linear8(x, q, e)
+    assert all(torch.equal(Q.linear8(x, p, f), want) for p, f in other_layouts(q, e))
