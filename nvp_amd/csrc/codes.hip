@@ -708,14 +708,17 @@ template <typename F> void with_team(int team, F f) {
     else f(std::integral_constant<int, 64>());
 }
 
+constexpr int64_t kMaxGroups = ((1ll << 32) - 1) / 256;                                     // workgroups of 256 threads: a launch has fewer than 2^32 threads along x
 template <typename T, typename O, typename I, int V>
 int fwd(const I* ids, const T* table, O* out, int64_t n, int64_t codes, int dim, float scale, hipStream_t st) {
     const int team = team_of((dim + V - 1) / V);
-    const int64_t blocks = (n + 4 * (256 / team) - 1) / (4 * (256 / team));
-    if (blocks > 0x7fffffff) return NVP_ERR_UNSUPPORTED;
-    const dim3 g((unsigned)blocks), wg(256);
-    with_team(team, [&](auto t) { hipLaunchKernelGGL((lookup_fwd_kernel<T, O, I, decltype(t)::value, V>), g, wg, 0, st, ids, table, out, n, codes, dim, scale); });
-    NVP_LAUNCH_CHECK();
+    const int64_t per = 4 * (256 / team), most = kMaxGroups * per;                            // rows of a workgroup, of a launch
+    for (int64_t r = 0; r < n; r += most) {
+        const int64_t here = n - r < most ? n - r : most;
+        const dim3 g((unsigned)((here + per - 1) / per)), wg(256);
+        with_team(team, [&](auto t) { hipLaunchKernelGGL((lookup_fwd_kernel<T, O, I, decltype(t)::value, V>), g, wg, 0, st, ids + r, table, out + r * dim, here, codes, dim, scale); });
+        NVP_LAUNCH_CHECK();
+    }
     return 0;
 }
 
@@ -724,7 +727,7 @@ int sum_level(const uint2* sorted, const unsigned* keys, const S* rows, T* dtabl
               bool filled, hipStream_t st) {
     const int team = team_of((dim + V - 1) / V), teams = 256 / team;
     const int64_t sums = (chunks + teams - 1) / teams, fill = FIRST && !filled ? (codes + 255) / 256 : 0, cols = (dim + team * V - 1) / (team * V);
-    if (sums + fill > 0x7fffffff || cols > 65535) return NVP_ERR_UNSUPPORTED;
+    if (sums + fill > kMaxGroups || cols > 65535) return NVP_ERR_UNSUPPORTED;
     with_team(team, [&](auto t) {
         hipLaunchKernelGGL((sum_runs_kernel<S, T, FIRST, decltype(t)::value, V>), dim3((unsigned)(sums + fill), (unsigned)cols), dim3(256), 0, st, sorted, keys, rows, dtable, nkeys, nrows, m,
                            per_chunk, chunks, sums, codes, dim, scale);
@@ -759,7 +762,7 @@ int sums_local(const Plan& P, const I* ids, const S* dout, T* dtable, uint8_t* w
     float* const part = (float*)ws;
     uint8_t* const there = ws + P.off_total;
     const int team = team_of((dim + V - 1) / V);
-    if (P.chunks[0] > 0x7fffffff) return NVP_ERR_UNSUPPORTED;
+    if (P.chunks[0] > kMaxGroups / 4) return NVP_ERR_UNSUPPORTED;
     with_team(team, [&](auto t) {
         hipLaunchKernelGGL((sum_local_kernel<I, S, decltype(t)::value, V>), dim3((unsigned)P.chunks[0]), dim3(64 * kLocalWaves), 0, st, ids, dout, part, there, n, P.per_chunk, (int)codes, dim, P.bits);
     });
@@ -781,7 +784,7 @@ int bwd(const I* ids, const S* dout, T* dtable, int64_t n, int64_t codes, int di
     // 65 536 codes x 1024: 512 ids 48 / 40, 16 384 ids 110 / 99;  65 536 codes x 512: 32 768 ids 59 / 63, 65 536 ids 80 / 85
     const int64_t bytes = codes * (int64_t)dim * (int64_t)sizeof(T), launches = P.small ? 1 : 3 * P.passes;
     const int64_t slice = ((bytes + launches - 1) / launches + kFillBytes - 1) / kFillBytes * kFillBytes;
-    const bool filled = n && codes >= 4 * n && slice / kFillBytes < 0x3fffffff;
+    const bool filled = n && codes >= 4 * n && slice / kFillBytes < (1 << 21);      // (workgroups of up to 1024 threads)
     int64_t done = 0;
     const auto next = [&](int64_t work, int64_t& grid) {                         // the launch's grid with its part of the table
         const int64_t len = filled ? (bytes - done < slice ? bytes - done : slice) : 0;

@@ -619,10 +619,12 @@ __global__ __launch_bounds__(64 * WM * WN) void linear8_tile_kernel(const uint8_
     }
 }
 
+// A launch has fewer than 2^32 threads along x.
+constexpr int64_t kMaxThreads = (1ll << 32) - 1, kMaxGroups = kMaxThreads / 256;             // (workgroups of 256)
 template <typename T, int BM, int BN, int WM, int WN, int STAGES>
 int launch_tile(const uint8_t* qx, const uint8_t* ex, const uint8_t* qw, const uint8_t* ew, const void* bias, void* y, int64_t rows, int64_t k, int64_t n, hipStream_t st) {
     const int64_t tm = (rows + BM - 1) / BM, tn = (n + BN - 1) / BN;
-    if (tm * tn > 0x3fffffff || kblocks(k) * 128 * BM > 0xffffffffll || kblocks(k) * 128 * BN > 0xffffffffll) return NVP_ERR_UNSUPPORTED;      // 32-bit offsets inside a tile
+    if (tm * tn * (64 * WM * WN) > kMaxThreads || kblocks(k) * 128 * BM > 0xffffffffll || kblocks(k) * 128 * BN > 0xffffffffll) return NVP_ERR_UNSUPPORTED;      // 32-bit offsets inside a tile
     constexpr size_t lds = tile_lds<BM, BN, STAGES>();
     // (HIP on gfx950 takes more than 64 KiB of dynamic LDS with or without the attribute: a refusal must not fail the call)
     static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(linear8_tile_kernel<T, BM, BN, WM, WN, STAGES>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
@@ -636,7 +638,7 @@ int64_t rows_lds(int64_t rows, int64_t k) { return rows * (kblocks(k) * 129 + 16
 template <typename T, int MT, int NT, int WAVES, bool FUSED>
 int launch_rows(const T* x, const uint8_t* qx, const uint8_t* ex, const uint8_t* qw, const uint8_t* ew, const void* bias, void* y, int64_t rows, int64_t k, int64_t n, hipStream_t st) {
     const int64_t gx = (n + 16 * NT - 1) / (16 * NT), gy = (rows + 16 * MT - 1) / (16 * MT);
-    if (gy > 65535 || gx > 0x7fffffff) return NVP_ERR_UNSUPPORTED;
+    if (gy > 65535 || gx * (64 * WAVES) > kMaxThreads) return NVP_ERR_UNSUPPORTED;
     const int64_t xbytes = FUSED ? rows_lds(rows < 16 * MT ? rows : 16 * MT, k) : 0, pbytes = WAVES * MT * 16 * (NT * 16 + 1) * 4;
     hipLaunchKernelGGL((linear8_rows_kernel<T, MT, NT, WAVES, FUSED>), dim3((unsigned)gx, (unsigned)gy), dim3(64 * WAVES), (size_t)(xbytes > pbytes ? xbytes : pbytes), st, x, qx, ex, qw, ew,
                        (const T*)bias, (T*)y, rows, k, n);
@@ -695,13 +697,18 @@ int linear8(const T* x, const uint8_t* qw, const uint8_t* ew, const void* bias, 
         case 256: return launch_narrow<T, 16>(x, qw, ew, bias, y, rows, k, n, st);
     }
     const int64_t kb = kblocks(k), kbp = kb4(k), nb = (n + 127) / 128;
-    uint8_t* qx = ws;
-    uint8_t* ex = qx + xq_bytes(rows, kb);
-    uint8_t* ewp = ex + rows * kbp;                                                          // rows * kbp is a multiple of 4
-    const int64_t groups = (rows * kb + 15) / 16, tail = (nb * kbp + 255) / 256;
-    if (groups + tail > 0x7fffffff) return NVP_ERR_UNSUPPORTED;
-    hipLaunchKernelGGL((quant_rows_kernel<T>), dim3((unsigned)(groups + tail)), dim3(256), 0, st, x, qx, ex, rows, k, groups, ew, ewp, nb * kbp);
-    NVP_LAUNCH_CHECK();
+    uint8_t* const qx = ws;
+    uint8_t* const ex = qx + xq_bytes(rows, kb);
+    uint8_t* const ewp = ex + rows * kbp;                                                    // rows * kbp is a multiple of 4
+    // the weights' scales with the first rows; as many rows a launch as it may have workgroups (a multiple of 8: those share a piece of the workspace)
+    const int64_t tail = (nb * kbp + 255) / 256, most = (kMaxGroups - tail) * 16 / kb / 8 * 8;
+    if (most < 8) return NVP_ERR_UNSUPPORTED;
+    for (int64_t r = 0; r < rows; r += most) {
+        const int64_t here = rows - r < most ? rows - r : most, groups = (here * kb + 15) / 16;
+        hipLaunchKernelGGL((quant_rows_kernel<T>), dim3((unsigned)(groups + (r ? 0 : tail))), dim3(256), 0, st, x + r * k, qx + xq_bytes(r, kb), ex + r * kbp, here, k, groups, ew, ewp,
+                           nb * kbp);
+        NVP_LAUNCH_CHECK();
+    }
     switch (path) {
         case kRows: {
             const bool narrow = (n + 31) / 32 < 256;                                         // 16 columns per workgroup where 32 would leave CUs without one
@@ -713,6 +720,26 @@ int linear8(const T* x, const uint8_t* qw, const uint8_t* ew, const void* bias, 
         case kTiles128x2: return launch_tile<T, 128, 128, 2, 2, 2>(qx, ex, qw, ewp, bias, y, rows, k, n, st);
         default: return launch_tile<T, 256, 256, 2, 4, 2>(qx, ex, qw, ewp, bias, y, rows, k, n, st);
     }
+}
+
+// as many rows a launch as it may have workgroups: k is at most 2^24, so that is at least 127 blocks of rows, and 255 rows of values
+template <typename T> int quant_blocks(const T* x, uint8_t* q, uint8_t* e, int64_t rows, int64_t k, int block_rows, hipStream_t st) {
+    const int64_t kb = kblocks(k), most = kMaxGroups / kb * block_rows;
+    for (int64_t r = 0; r < rows; r += most) {
+        const int64_t here = rows - r < most ? rows - r : most, groups = (here + block_rows - 1) / block_rows * kb;
+        hipLaunchKernelGGL((quant_blocks_kernel<T>), dim3((unsigned)groups), dim3(256), 0, st, x + r * k, q + r * kb * 128, e + r / block_rows * kb, here, k, block_rows);
+        NVP_LAUNCH_CHECK();
+    }
+    return 0;
+}
+template <typename T> int dequant_blocks(const uint8_t* q, const uint8_t* e, T* x, int64_t rows, int64_t k, int block_rows, hipStream_t st) {
+    const int64_t kb = kblocks(k), most = kMaxGroups * 256 / k / block_rows * block_rows;
+    for (int64_t r = 0; r < rows; r += most) {
+        const int64_t here = rows - r < most ? rows - r : most, groups = (here * k + 255) / 256;
+        hipLaunchKernelGGL((dequant_blocks_kernel<T>), dim3((unsigned)groups), dim3(256), 0, st, q + r * kb * 128, e + r / block_rows * kb, x + r * k, here, k, block_rows);
+        NVP_LAUNCH_CHECK();
+    }
+    return 0;
 }
 
 bool sizes_ok(int64_t rows, int64_t k, int64_t n) { return rows >= 0 && n >= 1 && k >= 1 && rows <= (1ll << 31) - 1 && n <= (1ll << 31) - 1 && k <= (1ll << 24); }
@@ -743,28 +770,18 @@ extern "C" int nvp_quantize_blocks(const void* x, int32_t type, uint8_t* q, uint
     if (!sizes_ok(rows, k, 1) || !nvp_type_size(type) || (block_rows != 1 && block_rows != 128)) return NVP_ERR_BADARG;
     if (rows == 0) return 0;
     if (!x || !q || !e) return NVP_ERR_BADARG;
-    const int64_t g = (rows + block_rows - 1) / block_rows * kblocks(k);
-    if (g > 0x7fffffff) return NVP_ERR_UNSUPPORTED;
     const hipStream_t st = (hipStream_t)stream;
-    const dim3 grid((unsigned)g), wg(256);
-    if (type == NVP_F32) hipLaunchKernelGGL((quant_blocks_kernel<float>), grid, wg, 0, st, (const float*)x, q, e, rows, k, block_rows);
-    else if (type == NVP_BF16) hipLaunchKernelGGL((quant_blocks_kernel<nvp_bf16>), grid, wg, 0, st, (const nvp_bf16*)x, q, e, rows, k, block_rows);
-    else hipLaunchKernelGGL((quant_blocks_kernel<nvp_f16>), grid, wg, 0, st, (const nvp_f16*)x, q, e, rows, k, block_rows);
-    NVP_LAUNCH_CHECK();
-    return 0;
+    if (type == NVP_F32) return quant_blocks<float>((const float*)x, q, e, rows, k, block_rows, st);
+    if (type == NVP_BF16) return quant_blocks<nvp_bf16>((const nvp_bf16*)x, q, e, rows, k, block_rows, st);
+    return quant_blocks<nvp_f16>((const nvp_f16*)x, q, e, rows, k, block_rows, st);
 }
 
 extern "C" int nvp_dequantize_blocks(const uint8_t* q, const uint8_t* e, void* x, int32_t type, int64_t rows, int64_t k, int32_t block_rows, void* stream) {
     if (!sizes_ok(rows, k, 1) || !nvp_type_size(type) || (block_rows != 1 && block_rows != 128)) return NVP_ERR_BADARG;
     if (rows == 0) return 0;
     if (!x || !q || !e) return NVP_ERR_BADARG;
-    const int64_t g = (rows * k + 255) / 256;
-    if (g > 0x7fffffff) return NVP_ERR_UNSUPPORTED;
     const hipStream_t st = (hipStream_t)stream;
-    const dim3 grid((unsigned)g), wg(256);
-    if (type == NVP_F32) hipLaunchKernelGGL((dequant_blocks_kernel<float>), grid, wg, 0, st, q, e, (float*)x, rows, k, block_rows);
-    else if (type == NVP_BF16) hipLaunchKernelGGL((dequant_blocks_kernel<nvp_bf16>), grid, wg, 0, st, q, e, (nvp_bf16*)x, rows, k, block_rows);
-    else hipLaunchKernelGGL((dequant_blocks_kernel<nvp_f16>), grid, wg, 0, st, q, e, (nvp_f16*)x, rows, k, block_rows);
-    NVP_LAUNCH_CHECK();
-    return 0;
+    if (type == NVP_F32) return dequant_blocks<float>(q, e, (float*)x, rows, k, block_rows, st);
+    if (type == NVP_BF16) return dequant_blocks<nvp_bf16>(q, e, (nvp_bf16*)x, rows, k, block_rows, st);
+    return dequant_blocks<nvp_f16>(q, e, (nvp_f16*)x, rows, k, block_rows, st);
 }

@@ -449,3 +449,19 @@ def test_lookup_refuses_a_gradient_with_a_tangent():
             torch.autograd.grad(out, table, forward_ad.make_dual(torch.ones_like(out), torch.ones_like(out)))
         with pytest.raises(NotImplementedError):
             codes.lookup(torch.tensor([1], device=dev()), forward_ad.make_dual(table, torch.ones_like(table)))
+
+
+@pytest.mark.gpu
+def test_lookup_of_more_rows_than_one_launch_takes():
+    """16 rows a workgroup of 256 threads: 2^28 rows are 2^32 threads."""
+    n, dim = (1 << 28) + 1000, 257
+    if torch.cuda.mem_get_info()[0] < 160 << 30:
+        pytest.skip("needs 140 GiB of device memory")
+    table = torch.randn(50, dim, device=dev(), dtype=B16)
+    ids = torch.randint(-1, 50, (n,), device=dev(), dtype=torch.int32)
+    out = codes.lookup(ids, table)
+    for a in (0, (1 << 28) - 600, (1 << 28) - 16, n - 1000):
+        i = ids[a:a + 1000].long()
+        assert torch.equal(out[a:a + 1000], table[i.clamp(min=0)] * (i >= 0)[:, None]), a
+    del out, ids
+    torch.cuda.empty_cache()

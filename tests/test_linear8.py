@@ -426,3 +426,51 @@ def test_linear8_weights_of_any_stride_and_alignment(m):
     q, e = Q.quantize_blocks(torch.randn(140, 300, device=dev()), 128)
     want = Q.linear8(x, q, e)
     assert all(torch.equal(Q.linear8(x, p, f), want) for p, f in other_layouts(q, e))
+
+
+@pytest.mark.gpu
+def test_block_form_of_more_blocks_and_values_than_one_launch_takes():
+    """2^24 blocks of a row each (2^32 threads) and more than 2^32 values: the parts on both sides of a launch's end, and the last rows, as the same rows alone."""
+    rows, k = (1 << 24) + 77, 260                                   # three blocks a row; 4.36e9 values
+    v = torch.randn(rows, k, device=dev(), dtype=torch.bfloat16)
+    spots = [0, (1 << 24) // 3 - 20, (1 << 25) // 3 - 20, (1 << 32) // k - 20, (1 << 24) - 20, rows - 40]
+    q, e = Q.quantize_blocks(v, 1)
+    back = Q.dequantize_blocks(q, e, k, 1, torch.bfloat16)
+    for a in spots:
+        p, f = Q.quantize_blocks(v[a:a + 40], 1)
+        assert torch.equal(q[a:a + 40].view(torch.uint8), p.view(torch.uint8)) and torch.equal(e[a:a + 40], f), a
+        assert torch.equal(back[a:a + 40], Q.dequantize_blocks(p, f, k, 1, torch.bfloat16)), a
+    del q, e, back
+    q, e = Q.quantize_blocks(v, 128)
+    back = Q.dequantize_blocks(q, e, k, 128, torch.bfloat16)
+    for a in spots:
+        a = a // 128 * 128
+        p, f = Q.quantize_blocks(v[a:a + 256], 128)
+        n = p.shape[0]
+        assert torch.equal(q[a:a + n].view(torch.uint8), p.view(torch.uint8)) and torch.equal(e[a // 128:a // 128 + f.shape[0]], f), a
+        assert torch.equal(back[a:a + n], Q.dequantize_blocks(p, f, k, 128, torch.bfloat16)), a
+    del v, q, e, back
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.gpu
+def test_linear8_of_more_blocks_than_one_launch_quantises():
+    """2^21 rows of 128 blocks and some more: 16 lanes a block are 2^32 threads.  The rows on both sides of the first launch's end as they come out alone."""
+    rows, k, n = (1 << 21) + 300, 16384, 20
+    if torch.cuda.mem_get_info()[0] < 130 << 30:
+        pytest.skip("needs 110 GiB of device memory")
+    x = torch.empty(rows, k, device=dev(), dtype=torch.bfloat16)
+    x.view(torch.int32)[:] = 0x3f80bf80                             # -1 and 1 in turn
+    q, e = Q.quantize_blocks(torch.randn(n, k, device=dev()), 128)
+    for a in ((1 << 21) - 80, rows - 100):
+        x[a:a + 80] = torch.randn(80, k, device=dev()).to(torch.bfloat16)
+    y = Q.linear8(x, q, e)
+    for a in (0, (1 << 21) - 100, (1 << 21) - 20, rows - 100):
+        # another tile: the same products, in another order: either is within the tolerance above of the exact sum; e4m3 makes |x| larger by 2^-4 at most
+        alone = Q.linear8(x[a:a + 100], q, e)
+        s = (1 + 2.0 ** -4) * x[a:a + 100].abs().double() @ Q.dequantize_blocks(q, e, k, 128).abs().double().t()
+        err = (y[a:a + 100].double() - alone.double()).abs()
+        assert bool((err <= 2 * ((k + 1) * 2.0 ** -23 + 7 * 2.0 ** -13) * (1 + 2.0 ** -8) * s + 2 * 2.0 ** -8 * (1 + 2.0 ** -7) * alone.double().abs()).all()), a
+        assert float(err.norm() / alone.double().norm()) <= 2 * (2.5e-4 + 2.0 ** -8)
+    del x, y
+    torch.cuda.empty_cache()
