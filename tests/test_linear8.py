@@ -474,3 +474,59 @@ def test_linear8_of_more_blocks_than_one_launch_quantises():
         assert float(err.norm() / alone.double().norm()) <= 2 * (2.5e-4 + 2.0 ** -8)
     del x, y
     torch.cuda.empty_cache()
+
+
+# rows and columns of every path: few rows (x quantised in the workgroup), up to 32 rows, the four tiles, few columns
+PATHS = [(2, 2100), (20, 2100), (40, 500), (511, 4100), (1500, 4100), (4100, 2100), (50001, 40), (20000, 130)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("kind", ["outliers", "log-normal"])
+@pytest.mark.parametrize("m,n", PATHS)
+def test_linear8_channels_of_very_different_size(m, n, kind, dtype):
+    """Some channels of x 30 times the others, or sizes spread over e^6: the small products beside a large one in a group of 8 are what the 8-bit instruction drops.  The
+    tolerance holds whatever the sizes: the dropped parts are below 2^-13 G each, at most seven beside the group's largest product G, so their rms is at most
+    (7 / 3)^0.5 2^-13 = 1.9e-4 of G, and with random signs the result's is G's at least."""
+    g = torch.Generator().manual_seed(m + n)
+    k = 643
+    size = torch.where(torch.rand(k, generator=g) < 0.05, 30.0, 1.0) if kind == "outliers" else torch.exp(torch.randn(k, generator=g).clamp(-3, 3))
+    x = (torch.randn(m, k, generator=g) * size).to(dtype)
+    w = torch.randn(n, k, generator=g) * k ** -0.5
+    q, e = Q.quantize_blocks(w.to(dev()), 128)
+    want, s = plain_linear(x, w, None)
+    within(Q.linear8(x.to(dev()), q, e), want, s, k, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES[1:])
+@pytest.mark.parametrize("m,n", PATHS)
+def test_linear8_scales_far_apart_on_16_bit_streams(m, n, dtype):
+    """16-bit streams hand the scale bytes to the matrix instruction: blocks of x and of the weight whose scales lie far apart (as far as fp16 results allow)."""
+    g = torch.Generator().manual_seed(m)
+    k, (a, b) = 128 * 5 + 3, (12, 12) if dtype == torch.bfloat16 else (5, 3)
+    x = torch.randn(m, k, generator=g) * torch.exp2(torch.randint(-a, a + 1, (m, -(-k // 128)), generator=g).float()).repeat_interleave(128, 1)[:, :k]
+    up = torch.exp2(torch.randint(-b, b + 1, (-(-n // 128), -(-k // 128)), generator=g).float())
+    w = torch.randn(n, k, generator=g) * up.repeat_interleave(128, 0)[:n].repeat_interleave(128, 1)[:, :k]
+    x = x.to(dtype)
+    q, e = Q.quantize_blocks(w.to(dev()), 128)
+    want, s = plain_linear(x, w, None)
+    within(Q.linear8(x.to(dev()), q, e), want, s, k, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES[1:])
+@pytest.mark.parametrize("m,n", PATHS)
+def test_linear8_non_finite_rows_on_16_bit_streams(m, n, dtype):
+    """Rows with an infinity or a NaN, the first and the last, become rows of NaN; every other row keeps its bits.  A weight row with a NaN makes its column NaN."""
+    g = torch.Generator().manual_seed(m)
+    x, w = torch.randn(m, 643, generator=g).to(dtype).to(dev()), torch.randn(n, 643, generator=g).to(dev())
+    q, e = Q.quantize_blocks(w, 128)
+    y = Q.linear8(x, q, e)
+    bad = x.clone()
+    bad[0, 5], bad[m - 1, 642] = float("inf"), float("nan")
+    z = Q.linear8(bad, q, e)
+    assert bool(z[0].isnan().all()) and bool(z[m - 1].isnan().all()) and torch.equal(z[1:m - 1], y[1:m - 1])
+    w[n - 1, 300] = float("nan")
+    z = Q.linear8(x, *Q.quantize_blocks(w, 128))
+    assert bool(z[:, n - 1].isnan().all()) and bool(z[:, :n - 1].isfinite().all())

@@ -703,3 +703,13 @@ def test_trunk_in_eight_bits_on_16_bit_streams(dtype):
         late = trunk.Trunk(96, 2).to(dev())
         late.load_state_dict(stack.state_dict())
         assert late.to(dtype).to_8bit()(x).dtype == dtype
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,wdtype", TYPES[1:])
+@pytest.mark.parametrize("shape,gate", [((4, 6, 32), (4, 1, 32)), ((3, 2, 5, 40), (3, 1, 1, 40)), ((2, 4000, 24), (2, 1, 24)), ((700, 3, 130), (700, 1, 130)), ((2, 1500, 1030), (2, 1, 1030)),
+                                        ((1, 900, 4096), (1, 1, 4096)), ((4, 5, 6, 2048), (4, 1, 1, 2048))])
+def test_residual_shared_gates_of_16_bits(shape, gate, dtype, wdtype):
+    for form, act in (("both", "sigmoid"), ("last", None)):
+        leaf, seeds = make(shape, dtype, wdtype, form, gate, sum(shape))
+        check(leaf, seeds, -0.5, act)
