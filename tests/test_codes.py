@@ -12,6 +12,7 @@ from nvp_amd import _lib as L
 from nvp_amd import codes
 
 F32, B16, F16 = torch.float32, torch.bfloat16, torch.float16
+E = 2.0 ** -24
 PAIRS = [(F32, F32), (F32, B16), (F32, F16), (B16, B16), (F16, F16)]
 
 
@@ -465,3 +466,74 @@ def test_lookup_of_more_rows_than_one_launch_takes():
         assert torch.equal(out[a:a + 1000], table[i.clamp(min=0)] * (i >= 0)[:, None]), a
     del out, ids
     torch.cuda.empty_cache()
+
+
+# ---- the whole batch's sort (1024 codes or more, or wide rows), where fewer codes go chunk by chunk ------------------------------------------------
+# one workgroup's sort (n <= 1024) and radix passes, one or two levels of sums; from codes >= 4 n on the zeros are written beside the sort
+SORTED = [(700, 1500, 48), (9000, 1500, 48), (70000, 5000, 32), (700, 4000, 48), (9000, 40000, 130), (70000, 300000, 16)]
+
+
+def sorted_step(ids, table, dout):
+    t = table.detach().requires_grad_(True)
+    out = codes.lookup(ids, t, 2.0)
+    return out.detach(), torch.autograd.grad(out, t, dout)[0]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,n_codes,dim", SORTED)
+def test_lookup_gradient_by_the_whole_sort_captured_and_replayed(n, n_codes, dim):
+    table = torch.randn(n_codes, dim, device=dev())
+    ids, dout = torch.randint(0, n_codes, (n,), device=dev()), torch.randn(n, dim, device=dev())
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        sorted_step(ids, table, dout)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = sorted_step(ids, table, dout)
+    for k in range(4):
+        ids.copy_(torch.randint(-2, n_codes, (n,), device=dev()) // (1 + 1000 * (k == 2)))
+        dout.copy_(torch.randn(n, dim, device=dev()))
+        got[1].fill_(float("nan"))                                  # rows that a replay leaves out would show
+        graph.replay()
+        want = sorted_step(ids, table, dout)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        grad, s, c = plain_grad(ids, dout, n_codes, 2.0)
+        assert bool(((got[1].double().cpu() - grad).abs() <= (c + 1) * 2.0 ** -24 * s * (1 + E) + E * grad.abs()).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,n_codes,dim", SORTED)
+def test_lookup_gradient_by_the_whole_sort_on_two_streams(n, n_codes, dim):
+    tables = [torch.randn(n_codes, dim, device=dev()) for _ in range(2)]
+    ids = [torch.randint(0, n_codes, (n,), device=dev()) for _ in range(2)]
+    dout = [torch.randn(n, dim, device=dev()) for _ in range(2)]
+    want = [sorted_step(ids[i], tables[i], dout[i])[1] for i in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(4):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got.append((i, sorted_step(ids[i], tables[i], dout[i])[1]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want[i]) for i, g in got)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["one id", "random", "two", "sorted"])
+@pytest.mark.parametrize("n,n_codes,dim", [(800_000, 5000, 32), (1_000_000, 70_000, 24), (1_300_000, 2000, 8), (300_000, 1100, 520)])
+def test_lookup_gradient_of_a_long_list_by_the_whole_sort(n, n_codes, dim, kind):
+    """The first two have three levels of sums, the third into the first one's list: with 32 entries a team, 800 000 positions leave a list of 50 000 partial rows, that one
+    of 3126, more than the last launch takes, that one of 196.  Integers: exact in any order."""
+    g = torch.Generator().manual_seed(n)
+    i = torch.arange(n)
+    ids = {"one id": torch.full((n,), n_codes - 1), "random": torch.randint(-1, n_codes, (n,), generator=g), "two": i % 2 * (n_codes - 1), "sorted": i * n_codes // n}[kind].to(dev())
+    dout = torch.randint(-8, 9, (n, dim), generator=g).float().to(dev())
+    t = torch.zeros(n_codes, dim, device=dev(), requires_grad=True)
+    got, = torch.autograd.grad(codes.lookup(ids, t), t, dout)
+    want = torch.zeros(n_codes, dim, dtype=torch.float64, device=dev())
+    want.index_add_(0, ids[ids >= 0], dout[ids >= 0].double())
+    assert torch.equal(got.double(), want)
