@@ -524,7 +524,7 @@ def test_lookup_gradient_by_the_whole_sort_on_two_streams(n, n_codes, dim):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", ["one id", "random", "two", "sorted"])
-@pytest.mark.parametrize("n,n_codes,dim", [(800_000, 5000, 32), (1_000_000, 70_000, 24), (1_300_000, 2000, 8), (300_000, 1100, 520)])
+@pytest.mark.parametrize("n,n_codes,dim", [(800_000, 5000, 32), (1_000_000, 70_000, 24), (1_300_000, 2000, 8), (300_000, 1100, 260)])
 def test_lookup_gradient_of_a_long_list_by_the_whole_sort(n, n_codes, dim, kind):
     """The first two have three levels of sums, the third into the first one's list: with 32 entries a team, 800 000 positions leave a list of 50 000 partial rows, that one
     of 3126, more than the last launch takes, that one of 196.  Integers: exact in any order."""
@@ -534,6 +534,4 @@ def test_lookup_gradient_of_a_long_list_by_the_whole_sort(n, n_codes, dim, kind)
     dout = torch.randint(-8, 9, (n, dim), generator=g).float().to(dev())
     t = torch.zeros(n_codes, dim, device=dev(), requires_grad=True)
     got, = torch.autograd.grad(codes.lookup(ids, t), t, dout)
-    want = torch.zeros(n_codes, dim, dtype=torch.float64, device=dev())
-    want.index_add_(0, ids[ids >= 0], dout[ids >= 0].double())
-    assert torch.equal(got.double(), want)
+    assert torch.equal(got.double().cpu(), plain_grad(ids, dout, n_codes, 1.0)[0])
