@@ -713,3 +713,17 @@ def test_residual_shared_gates_of_16_bits(shape, gate, dtype, wdtype):
     for form, act in (("both", "sigmoid"), ("last", None)):
         leaf, seeds = make(shape, dtype, wdtype, form, gate, sum(shape))
         check(leaf, seeds, -0.5, act)
+
+
+@pytest.mark.gpu
+def test_the_readmes_example_runs():
+    import os
+    import re
+    from nvp_amd import modulation
+    text = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "README.md")).read()
+    code, = [b for b in re.findall(r"```python\n(.*?)```", text, re.S) if "CodeTable" in b]
+    net = modulation.SirenNet(dim_in=1, dim_hidden=128, dim_out=3, num_layers=3, w0_initial=30.)
+    ids = torch.randint(-1, 600, (500,), device=dev())
+    names = {"torch": torch, "siren_wrapper": modulation.SirenWrapper(net, latent_dim=114).to(dev()), "coords": ids[:, None].float() / 600, "frame_ids": ids}
+    exec(code, names)
+    assert names["rgb"].shape == (500, 3) and bool(names["rgb"].isfinite().all()) and not names["rgb"].requires_grad
