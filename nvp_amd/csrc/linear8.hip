@@ -211,7 +211,7 @@ __global__ __launch_bounds__(256) void dequant_blocks_kernel(const uint8_t* __re
 // times 4096 columns is 256 workgroups x 8 waves that read disjoint weights: bound by the bytes of the weights, which are on their way (kAhead blocks)
 // before anything else happens.  FUSED: the workgroup quantises its rows of x into LDS itself - no workspace, no second launch; each workgroup repeats
 // that, which pays while there are few workgroups or few rows.  1 x 4096 x 4096 bf16: 5.6 us (16.8 MB, 3 TB/s: one round of loads, whose latency is most of
-// it); 32 x 4096 x 4096: 12.3 us with the quantising launch.
+// it); 32 x 4096 x 4096: 2.2 us for the quantising launch and 10.1: the same round of weight loads, x's rows from L2 behind it (the waves wait 74 % of their life).
 // Operand order: lane (i = lane & 15, g = lane >> 4) holds columns 16 g .. 16 g + 15 and 64 + 16 g .. of its row's block, the same for both
 // operands: which k a register byte stands for cancels in the sum, and each load instruction covers 64 contiguous bytes of a row.
 constexpr int rows_ahead(int mt, int nt) { return mt * nt >= 4 ? 2 : 4; }
@@ -475,9 +475,11 @@ __global__ __launch_bounds__(256, NT <= 8 ? 3 : 2) void linear8_narrow_kernel(co
 // (BM / WM) x (BN / WN) with 32x32x64 instructions.  One barrier per block, at its start: behind it the block has landed for everyone (every wave waits for
 // its own loads, counted: those of later blocks stay in flight) and the stage of the block before has been read, so that its refill is issued at once.
 // The scales come through LDS too: a load into registers would be waited for together with all fills before it.
-// Measured, with the quantising launch: 8192 x 8192 x 8192 bf16 490 us, 2.24 PFLOP/s (the 256 x 256 tile; the matrix units are busy 57 - 60 % of the cycles of a
-// clock that their power holds at 1.8 - 2.0 GHz of 2.4: finer interleaving of loads, reads and products, in 4 or 8 waves, was not faster); 256 x 4096 x 4096
-// 15.3 us (the 64 x 64 tile, bound by the bytes through LDS: 128 MB; splitting a tile's blocks over two or four teams of waves was not faster).
+// Measured, with the quantising launch: 8192 x 8192 x 8192 bf16 490 us, 2.24 PFLOP/s (the 256 x 256 tile; the matrix units are busy 57 % of the cycles of a
+// clock that their power holds at 1.8 GHz of 2.4: finer interleaving of loads, reads and products, in 4 or 8 waves, was not faster); 256 x 4096 x 4096
+// 15.3 us, the tile kernel 13: 256 tiles, so one wave per SIMD, whose 32 blocks take 800 cycles each: 330 of them to fill a stage (16 KB at 50 bytes per clock), 140 of LDS reads,
+// 130 of products, one behind the other behind a barrier (counters: the waves wait 45 % of their life, the matrix units are busy 16 % of it, LDS 17 %); splitting a tile's
+// blocks over two or four teams of waves was not faster.
 // LDS rows are 128 bytes; the 16-byte piece c of row r lies at place c ^ (r >> 1 & 7): of any 16 rows that one 256-byte LDS cycle serves (0 - 15, or
 // 0-3, 12-15, 20-23, 24-27) no two share a bank (measured: no conflicts; with c ^ (r & 7) a third of the LDS cycles were conflicts).  The loads swizzle on
 // their global side (LDS writes are linear).

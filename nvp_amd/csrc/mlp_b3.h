@@ -110,7 +110,7 @@ __device__ __forceinline__ void split8(const float (&x)[8], const float s, BOp& 
         b.p[0][p] = hh;
         b.p[1][p] = ll;
 #elif NVP_SPLIT_ASM == 2
-        // hi from hipcc's v_pk_mul_f32 + v_cvt_pk_f16_f32; the two residuals as v_fma_mix{lo,hi}_f16 whose addend is the matching
+        // hi from hipcc's two multiplications + v_cvt_pk_f16_f32; the two residuals as v_fma_mix{lo,hi}_f16 whose addend is the matching
         // HALF of the packed hi register (op_sel) - hipcc's own selection converts hi a second time, once per half
         const f16x2 h = {(_Float16)(a * s), (_Float16)(c * s)};
         const unsigned hh = __builtin_bit_cast(unsigned, h);
