@@ -92,7 +92,7 @@ void ok(int64_t rc, const char* what) {
 void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 // rows side by side, values as they read (a view that negates, as the imaginary part of a conjugate, keeps its values' other sign in memory)
-Tensor dense(const Tensor& t) { return t.defined() ? t.resolve_neg().contiguous() : t; }
+Tensor dense(const Tensor& t) { return t.defined() ? (t.is_neg() ? t.resolve_neg() : t).contiguous() : t; }
 Tensor dense(const Maybe& t) { return t ? dense(*t) : Tensor(); }
 Tensor workspace(int64_t bytes, const Tensor& like, const char* what) {
     if (bytes < 0) ok(bytes, what);
