@@ -554,7 +554,8 @@ def test_residual_wide_rows_do_not_depend_on_their_neighbours():
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype,wdtype", TYPES)
-@pytest.mark.parametrize("shape,gate", [((40, 228), (40, 228)), ((9, 115), (9, 115)), ((6, 50, 114), (6, 1, 114)), ((2, 1500, 130), (1, 1, 130)), ((3, 4100), (3, 4100)), ((2, 30, 8190), (2, 1, 8190))])
+@pytest.mark.parametrize("shape,gate", [((40, 228), (40, 228)), ((9, 115), (9, 115)), ((6, 50, 114), (6, 1, 114)), ((2, 1500, 130), (1, 1, 130)), ((3, 4100), (3, 4100)), ((2, 30, 8190), (2, 1, 8190)),
+                                        ((3, 5003), (3, 5003)), ((2, 8190), (2, 8190)), ((3, 8192), (3, 8192))])
 def test_residual_gates_far_open_and_far_closed(shape, gate, dtype, wdtype, monkeypatch):
     """A sigmoid's derivative is a (1 - a) whichever side a is near: every gradient to the tolerance above, of numbers down to 1e-13.  The 64-bit sigmoid is written
     out here, because autograd differentiates 1 / (1 + exp(-g)) without a difference, while torch.sigmoid's own backward has 1 - a (1e-3 off at 30, in 64 bits)."""
